@@ -29,8 +29,10 @@ extern "C" {
  * library's.  2: K and V carry separate strides in the prefill and code-predictor entry points.  3: q3a_prefill_append.  4: q3a_paged_decode_append_rope.
  * 5: q3a_prefill_dense_append.  6: q3a_prefill_dense_append_rope, q3a_prefill_append_rope,
  * q3a_cp_attn_append_rope.  7: the decode path codes below (negative split_tokens).  8: per-frame decode plans
- * (q3a_paged_decode_plan_bytes, q3a_paged_decode_plan, Q3A_DECODE_PLANNED). */
-#define Q3A_ABI_VERSION 8
+ * (q3a_paged_decode_plan_bytes, q3a_paged_decode_plan, Q3A_DECODE_PLANNED).  9: the 8-bit pool (q3a_paged_write_fp8,
+ * q3a_paged_read_fp8, q3a_paged_decode_fp8, q3a_paged_decode_fp8_append) and q3a_paged_decode_tree with its workspace
+ * query. */
+#define Q3A_ABI_VERSION 9
 
 /* Decode decomposition codes, passed as split_tokens to the q3a_paged_decode* entry points (0 lets the library
  * choose, a positive multiple of 16 is a fixed split of that many tokens):
@@ -432,6 +434,101 @@ int q3a_prefill_append_rope(
     int page_size, const int32_t* block_table, int64_t bt_stride_b, int max_pages_per_seq, void* out,
     int64_t o_stride_t, int64_t o_stride_h, void* workspace, size_t workspace_bytes, int num_seqs, int total_tokens,
     int max_seqlen, int num_q_heads, int num_kv_heads, int head_dim, float softmax_scale, int causal, void* stream);
+
+/*
+ * The 8-bit K/V pool.  No counterpart in the reference, whose pools are bf16 (engine/talker.py:30-31); a pool of half the
+ * bytes holds twice the contexts, and its decode reads half as much.
+ *
+ *   k_cache, v_cache  [num_pages, page_size, Hkv, 128] e4m3 codes (OCP, finite), strides kv_stride_page / kv_stride_tok /
+ *                     kv_stride_head in bytes (= elements), dim stride 1, shared by the two pools
+ *   k_scale, v_scale  [num_pages, Hkv, page_size] one exponent byte s per (token, KV head), strides scale_stride_page /
+ *                     scale_stride_head, token stride 1, shared
+ *
+ * An element is code * 2^(s - 127).  A written row x[0..127] gets the smallest power of two 2^(s-127) >= 2^-117 with
+ * max |x_d| <= 448 * 2^(s-127) over its finite elements, and codes e4m3(x_d * 2^(127-s)) rounded to nearest even (at s = 247 at
+ * most 240, so that none stands for more than bf16 holds); elements that are not finite are held as NaN.  Every value read back is a bf16 number, so attention over the pool is attention over
+ * the bf16 rows read back.  Bytes outside 10..247 are not written by q3a_paged_write_fp8 and stand for no value.
+ * Requirements: page_size a multiple of 16, caches 16-byte aligned with strides multiples of 16, token stride in
+ * [128, 2^26]; scales 4-byte aligned with strides multiples of 4.  Any layout with these strides serves; with a page's tokens
+ * of one head next to each other (strides page: Hkv * page_size * 128, head: page_size * 128, token: 128) a head's page is
+ * one run of memory.
+ *
+ * q3a_paged_write_fp8 quantises rows k, v [T, Hkv, 128] bf16 (token and head strides) into slots [T] int64, slot = page *
+ * page_size + offset; tokens with a slot outside [0, num_pages * page_size) are not written.  A slot named by two tokens holds
+ * a mix of both afterwards: only a scratch slot that nothing reads may be.  Replaces, for this pool, the index_copy_ pair of
+ * engine/talker.py:72-73 and :161-162.  T * Hkv at most 2^28.
+ *
+ * q3a_paged_read_fp8 writes the rows of slots [T] back as bf16 k, v [T, Hkv, 128]; slots outside the pool read zeros.
+ */
+int q3a_paged_write_fp8(const void* k, int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
+                        int64_t v_stride_h, const int64_t* slots, void* k_cache, void* v_cache, int64_t kv_stride_page,
+                        int64_t kv_stride_tok, int64_t kv_stride_head, void* k_scale, void* v_scale,
+                        int64_t scale_stride_page, int64_t scale_stride_head, int num_pages, int page_size,
+                        int64_t num_tokens, int num_kv_heads, int head_dim, void* stream);
+int q3a_paged_read_fp8(const void* k_cache, const void* v_cache, int64_t kv_stride_page, int64_t kv_stride_tok,
+                       int64_t kv_stride_head, const void* k_scale, const void* v_scale, int64_t scale_stride_page,
+                       int64_t scale_stride_head, int num_pages, int page_size, const int64_t* slots, void* k,
+                       int64_t k_stride_t, int64_t k_stride_h, void* v, int64_t v_stride_t, int64_t v_stride_h,
+                       int64_t num_tokens, int num_kv_heads, int head_dim, void* stream);
+
+/*
+ * Decode attention over the 8-bit pool: q3a_paged_decode's semantics (rows with ctx <= 0 give zeros, ctx is clamped to
+ * max_pages_per_seq * page_size, a page index outside [0, num_pages) contributes no tokens) for any Hq that is a multiple of
+ * Hkv, up to 16 query heads to a KV head and 64 KV heads.  q and out [B, Hq, 128] bf16.
+ *
+ * The append form quantises k_new, v_new [B, Hkv, 128] bf16 into position cache_seqlens[b] of row b as
+ * q3a_paged_write_fp8 does, and attends over tokens 0 .. cache_seqlens[b], the new one with the value that the pool now holds.
+ * Rows with cache_seqlens < 0, or whose new token would fall past the table, are skipped: zero output, nothing written.  A
+ * new token whose page index is outside [0, num_pages) is neither written nor attended.  The page that receives a row's new
+ * token must not be read by another row of the same call.
+ *
+ * workspace: q3a_paged_decode_tree_workspace_bytes(batch, 1, ...) bytes, 16-byte aligned, uninitialised (0: may be NULL);
+ * calls that overlap need one each.  batch at most 65,535; a table of at most 2^30 tokens a row.
+ */
+int q3a_paged_decode_fp8(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k_cache, const void* v_cache,
+                         int64_t kv_stride_page, int64_t kv_stride_tok, int64_t kv_stride_head, const void* k_scale,
+                         const void* v_scale, int64_t scale_stride_page, int64_t scale_stride_head, int num_pages,
+                         int page_size, const int32_t* cache_seqlens, const int32_t* block_table, int64_t bt_stride_b,
+                         int max_pages_per_seq, void* out, int64_t o_stride_b, int64_t o_stride_h, void* workspace,
+                         size_t workspace_bytes, int batch, int num_q_heads, int num_kv_heads, int head_dim,
+                         float softmax_scale, void* stream);
+int q3a_paged_decode_fp8_append(
+    const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k_new, int64_t kn_stride_b, int64_t kn_stride_h,
+    const void* v_new, int64_t vn_stride_b, int64_t vn_stride_h, void* k_cache, void* v_cache, int64_t kv_stride_page,
+    int64_t kv_stride_tok, int64_t kv_stride_head, void* k_scale, void* v_scale, int64_t scale_stride_page,
+    int64_t scale_stride_head, int num_pages, int page_size, const int32_t* cache_seqlens, const int32_t* block_table,
+    int64_t bt_stride_b, int max_pages_per_seq, void* out, int64_t o_stride_b, int64_t o_stride_h, void* workspace,
+    size_t workspace_bytes, int batch, int num_q_heads, int num_kv_heads, int head_dim, float softmax_scale, void* stream);
+
+/*
+ * Attention for trees of drafted tokens (speculative decoding's check of several candidate continuations in one pass) over
+ * the paged pool.  No counterpart in the reference, which decodes one token a row (engine/talker.py:77).
+ *
+ * Row b has N drafted tokens (nodes), N <= 256, whose k and v are not in the pool.  Node n sees the row's first
+ * cache_seqlens[b] cached tokens and node j's k_new, v_new if tree_mask[b][n][j] != 0 (tree_mask NULL: if j <= n, a chain).
+ *
+ *   q            [B, N, Hq, 128] bf16, strides b, n, h;   k_new, v_new [B, N, Hkv, 128] bf16, strides each
+ *   tree_mask    bytes, row b node n at mask_stride_b * b + mask_stride_n * n, node stride 1 (mask_stride_b 0: one for all)
+ *   k_scale,     NULL: k_cache, v_cache are the bf16 pool [num_pages, page_size, Hkv, 128] of q3a_paged_decode (strides in
+ *   v_scale      elements, 16-byte aligned rows); else the 8-bit pool above
+ *   out          [B, N, Hq, 128] bf16, strides b, n, h
+ *
+ * cache_seqlens[b] < 0 skips row b (zero output); 0 leaves the nodes' own keys.  A node that sees nothing gives zeros.  What
+ * a masked k_new or v_new row holds (NaN, infinities) does not reach the nodes that do not see it.  Nothing is written but
+ * out: the rows of the accepted nodes are written afterwards (q3a_paged_write_fp8 or, in bf16, as the caller appends).
+ * Shapes, workspace (q3a_paged_decode_tree_workspace_bytes) and pool semantics as q3a_paged_decode_fp8.
+ */
+size_t q3a_paged_decode_tree_workspace_bytes(int batch, int num_nodes, int num_q_heads, int num_kv_heads, int head_dim,
+                                             int max_pages_per_seq, int page_size);
+int q3a_paged_decode_tree(
+    const void* q, int64_t q_stride_b, int64_t q_stride_n, int64_t q_stride_h, const void* k_new, int64_t kn_stride_b,
+    int64_t kn_stride_n, int64_t kn_stride_h, const void* v_new, int64_t vn_stride_b, int64_t vn_stride_n, int64_t vn_stride_h,
+    const uint8_t* tree_mask, int64_t mask_stride_b, int64_t mask_stride_n, const void* k_cache, const void* v_cache,
+    int64_t kv_stride_page, int64_t kv_stride_tok, int64_t kv_stride_head, const void* k_scale, const void* v_scale,
+    int64_t scale_stride_page, int64_t scale_stride_head, int num_pages, int page_size, const int32_t* cache_seqlens,
+    const int32_t* block_table, int64_t bt_stride_b, int max_pages_per_seq, void* out, int64_t o_stride_b, int64_t o_stride_n,
+    int64_t o_stride_h, void* workspace, size_t workspace_bytes, int batch, int num_nodes, int num_q_heads, int num_kv_heads,
+    int head_dim, float softmax_scale, void* stream);
 
 #ifdef __cplusplus
 }

@@ -12,6 +12,9 @@ Entry points (each a drop-in for the reference call it names):
   * ``prefill_append_rope``                          -- + the prompt's q/k norm and RoPE (engine/talker.py:157-169)
   * ``prefill_dense_append``                         -- admission K/V into the pool + prefill (engine/arrivals.py:144-148)
   * ``prefill_dense_append_rope``                    -- + the admission q/k norm, RoPE and K/V concat (engine/arrivals.py:112-118)
+  * ``fp8_cache`` / ``paged_write_fp8`` / ``paged_read_fp8`` -- the 8-bit K/V pool: buffers, quantising write, read back
+  * ``paged_decode_fp8`` / ``paged_decode_fp8_append`` -- decode attention over the 8-bit pool, and with the step's write
+  * ``paged_decode_tree``                            -- attention for trees of drafted tokens over a bf16 or 8-bit pool
   * ``PagePool``                                     -- 16-token pages per seat from a free list, device block table
 """
 import torch  # noqa: F401  (loads the HIP runtime the library binds to)
@@ -19,9 +22,12 @@ import torch  # noqa: F401  (loads the HIP runtime the library binds to)
 from ._lib import LIB_PATH, Q3AttnError, lib  # noqa: F401
 from .cp_attn import (cp_attn, cp_attn_append, cp_attn_append_op, cp_attn_append_rope,  # noqa: F401
                       cp_attn_append_rope_op, cp_attn_op)
+from .fp8 import (fp8_cache, paged_decode_fp8, paged_decode_fp8_append, paged_read_fp8,  # noqa: F401
+                  paged_write_fp8)
 from .ops import (DECODE_CHUNKS, DECODE_PLANNED, DECODE_ROW, DECODE_STREAMK, decode_plan,  # noqa: F401
                   flash_attn_with_kvcache, paged_decode,  # noqa: F401
                   paged_decode_append, paged_decode_append_rope)
 from .pages import PagePool, PoolExhausted  # noqa: F401
 from .prefill import (flash_attn_func, flash_attn_varlen_func, prefill, prefill_append, prefill_dense,  # noqa: F401
                       prefill_append_rope, prefill_dense_append, prefill_dense_append_rope)
+from .tree import paged_decode_tree  # noqa: F401

@@ -13,7 +13,7 @@ import threading
 import torch  # noqa: F401  (must precede the library load, see above)
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libq3attn.so")
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 _c_i64 = ctypes.c_int64
 _c_int = ctypes.c_int
@@ -166,6 +166,48 @@ SIGNATURES = {
         _c_vp, _c_i64, _c_i64, _c_i64,                         # out, o strides (seq, tok, head)
         _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,        # num_seqs, seqlen_q, seqlen_k, Hq, Hkv, D
         _c_float, _c_int, _c_vp,                               # softmax_scale, causal, stream
+    ]),
+    "q3a_paged_write_fp8": (_c_int, [
+        _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_vp,   # k, strides (tok, head), v, strides, slots
+        _c_vp, _c_vp, _c_i64, _c_i64, _c_i64,                  # k_cache, v_cache, cache strides (page, tok, head)
+        _c_vp, _c_vp, _c_i64, _c_i64,                          # k_scale, v_scale, scale strides (page, head)
+        _c_int, _c_int, _c_i64, _c_int, _c_int, _c_vp,         # num_pages, page_size, num_tokens, Hkv, D, stream
+    ]),
+    "q3a_paged_read_fp8": (_c_int, [
+        _c_vp, _c_vp, _c_i64, _c_i64, _c_i64,                  # k_cache, v_cache, cache strides (page, tok, head)
+        _c_vp, _c_vp, _c_i64, _c_i64,                          # k_scale, v_scale, scale strides (page, head)
+        _c_int, _c_int, _c_vp,                                 # num_pages, page_size, slots
+        _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64,          # k, strides (tok, head), v, strides
+        _c_i64, _c_int, _c_int, _c_vp,                         # num_tokens, Hkv, D, stream
+    ]),
+    "q3a_paged_decode_tree_workspace_bytes": (_c_size, [_c_int] * 7),
+    "q3a_paged_decode_fp8": (_c_int, [
+        _c_vp, _c_i64, _c_i64,                                 # q, strides (row, head)
+        _c_vp, _c_vp, _c_i64, _c_i64, _c_i64,                  # k_cache, v_cache, cache strides (page, tok, head)
+        _c_vp, _c_vp, _c_i64, _c_i64,                          # k_scale, v_scale, scale strides (page, head)
+        _c_int, _c_int, _c_vp, _c_vp, _c_i64, _c_int,          # num_pages, page_size, seqlens, block_table, stride, max pages
+        _c_vp, _c_i64, _c_i64, _c_vp, _c_size,                 # out, strides (row, head), workspace, bytes
+        _c_int, _c_int, _c_int, _c_int, _c_float, _c_vp,       # batch, Hq, Hkv, D, softmax_scale, stream
+    ]),
+    "q3a_paged_decode_fp8_append": (_c_int, [
+        _c_vp, _c_i64, _c_i64,                                 # q, strides (row, head)
+        _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64,          # k_new, strides (row, head), v_new, strides
+        _c_vp, _c_vp, _c_i64, _c_i64, _c_i64,                  # k_cache, v_cache, cache strides (page, tok, head)
+        _c_vp, _c_vp, _c_i64, _c_i64,                          # k_scale, v_scale, scale strides (page, head)
+        _c_int, _c_int, _c_vp, _c_vp, _c_i64, _c_int,          # num_pages, page_size, seqlens, block_table, stride, max pages
+        _c_vp, _c_i64, _c_i64, _c_vp, _c_size,                 # out, strides (row, head), workspace, bytes
+        _c_int, _c_int, _c_int, _c_int, _c_float, _c_vp,       # batch, Hq, Hkv, D, softmax_scale, stream
+    ]),
+    "q3a_paged_decode_tree": (_c_int, [
+        _c_vp, _c_i64, _c_i64, _c_i64,                         # q, strides (row, node, head)
+        _c_vp, _c_i64, _c_i64, _c_i64,                         # k_new, strides (row, node, head)
+        _c_vp, _c_i64, _c_i64, _c_i64,                         # v_new, strides (row, node, head)
+        _c_vp, _c_i64, _c_i64,                                 # tree_mask, strides (row, node)
+        _c_vp, _c_vp, _c_i64, _c_i64, _c_i64,                  # k_cache, v_cache, cache strides (page, tok, head)
+        _c_vp, _c_vp, _c_i64, _c_i64,                          # k_scale, v_scale, scale strides (page, head)
+        _c_int, _c_int, _c_vp, _c_vp, _c_i64, _c_int,          # num_pages, page_size, seqlens, block_table, stride, max pages
+        _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_size,         # out, strides (row, node, head), workspace, bytes
+        _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_vp,  # batch, nodes, Hq, Hkv, D, softmax_scale, stream
     ]),
 }
 
