@@ -1,7 +1,9 @@
 """Build recipe for the q3attn HIP library (gfx950): ``python build.py`` or ``build()``.
 
 Compiles every ``csrc/*.hip`` with hipcc for gfx950 and links ``q3attn/libq3attn.so`` in-tree, so
-the built library travels with the source tree.  Object files go to ``_build/`` (git-ignored).
+the built library travels with the source tree; ``binding/torch_ops.cpp``, the torch ops that are
+registered from C++, becomes ``q3attn/libq3torch.so`` beside it (host code only).  Object files go to
+``_build/`` (git-ignored).
 """
 from __future__ import annotations
 
@@ -17,10 +19,15 @@ OUT = os.path.join(HERE, "q3attn", "libq3attn.so")
 # HBM probes (measurement infrastructure for bench.py --workload probe), a library of their own
 PROBE_SRC = os.path.join(HERE, "probe", "hbm_probe.hip")
 PROBE_OUT = os.path.join(HERE, "q3attn", "libq3probe.so")
+# torch ops over the C ABI, a library of their own that links libq3attn.so and torch
+TORCH_SRC = os.path.join(HERE, "binding", "torch_ops.cpp")
+TORCH_OUT = os.path.join(HERE, "q3attn", "libq3torch.so")
 BUILD = os.path.join(HERE, "_build")
 ARCH = os.environ.get("Q3A_OFFLOAD_ARCH", "gfx950")
 
+ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+CXX = os.environ.get("CXX", "g++")
 CFLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-fPIC", "-std=c++17", "-mcode-object-version=5",
     "-Wall", "-Wno-unused-function",
@@ -64,20 +71,47 @@ def _compile(src: str) -> str:
     return obj
 
 
+def _run(cmd, what: str) -> None:
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{what} failed:\n{r.stdout}{r.stderr}")
+
+
+def _compile_torch_ops() -> str:
+    import torch
+    root = os.path.dirname(torch.__file__)
+    obj = os.path.join(BUILD, "binding_torch_ops.cpp.o")
+    _run([CXX, "-O2", "-fPIC", "-std=c++17", "-Wall", "-DUSE_ROCM=1", "-D__HIP_PLATFORM_AMD__=1",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-isystem", os.path.join(root, "include"),
+          "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"), "-isystem", os.path.join(ROCM, "include"),
+          "-c", TORCH_SRC, "-o", obj], f"compiling {TORCH_SRC}")
+    return obj
+
+
+def _link_torch_ops(obj: str) -> None:
+    import torch
+    _run([CXX, "-shared", obj, "-L" + os.path.dirname(OUT), "-lq3attn", "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"),
+          "-lc10", "-lc10_hip", "-ltorch_cpu", "-Wl,-rpath,$ORIGIN", "-o", TORCH_OUT + ".tmp"], f"linking {TORCH_OUT}")
+    os.replace(TORCH_OUT + ".tmp", TORCH_OUT)
+
+
 def build(verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     srcs = sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".hip"))
     with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as ex:
+        binding = ex.submit(_compile_torch_ops)
         objs = list(ex.map(_compile, srcs + [PROBE_SRC]))
+        binding = binding.result()
     for out, parts in ((OUT, objs[:-1]), (PROBE_OUT, objs[-1:])):
         tmp = out + ".tmp"
-        cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", *parts, "-o", tmp]
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError(f"link failed:\n{r.stdout}{r.stderr}")
+        soname = ["-Wl,-soname," + os.path.basename(out)]
+        _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", *soname, *parts, "-o", tmp], "link")
         os.replace(tmp, out)
         if verbose:
             print(f"built {out}")
+    _link_torch_ops(binding)
+    if verbose:
+        print(f"built {TORCH_OUT}")
     return OUT
 
 

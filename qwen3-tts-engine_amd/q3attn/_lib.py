@@ -13,6 +13,8 @@ import threading
 import torch  # noqa: F401  (must precede the library load, see above)
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libq3attn.so")
+# The torch ops that are registered from C++ (they link libq3attn.so).
+TORCH_LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libq3torch.so")
 ABI_VERSION = 9
 
 _c_i64 = ctypes.c_int64
@@ -246,3 +248,22 @@ def check(rc: int, what: str) -> None:
     if rc != 0:
         msg = lib().q3a_last_error().decode(errors="replace")
         raise Q3AttnError(f"{what} failed ({rc}): {msg}")
+
+
+def torch_ops(*names: str):
+    """The ops ``q3attn::name`` that libq3torch.so registers; without the built libraries, functions that raise."""
+    if os.path.exists(LIB_PATH) and os.path.exists(TORCH_LIB_PATH):
+        lib()
+        torch.ops.load_library(TORCH_LIB_PATH)
+        return [getattr(torch.ops.q3attn, name).default for name in names]
+
+    def missing(*args, **kwargs):
+        raise Q3AttnError(f"q3attn: {LIB_PATH} or {TORCH_LIB_PATH} was not built when q3attn was imported; build them first "
+                          "(python qwen3-tts-engine_amd/build.py or __graft_entry__.build())")
+    return [missing] * len(names)
+
+
+def register_fake(op, fn) -> None:
+    """fn as ``op``'s implementation on fake tensors (shapes only), if the op is there."""
+    if isinstance(op, torch._ops.OpOverload):
+        torch.library.register_fake(op._schema.name, fn)

@@ -236,3 +236,35 @@ def test_refusals(cuda_device):
     for kk, vv in ((k[:1], k), (k, k.float()), (k, k[:, :4])):
         with pytest.raises(RuntimeError, match="q3a|q3attn"):
             q3attn.paged_decode_fp8_append(q, kk, vv, *pool, lens, table, 0.1)
+
+
+def test_compiled_step_writes_the_callers_pool(cuda_device):
+    """Inside torch.compile: the write, the read and the append form mutate the caller's pool in place, without a copy of it."""
+    lens = [3, 40, 17]
+    pool = q3attn.fp8_cache(4096, device=cuda_device)
+    eager_pool = [t.clone() for t in pool]
+    table = torch.arange(3 * 4, dtype=torch.int32, device=cuda_device).view(3, 4)
+    g = torch.Generator().manual_seed(3)
+    q = torch.randn((3, 16, 128), generator=g).to(torch.bfloat16).to(cuda_device)
+    k = torch.randn((60, 8, 128), generator=g).to(torch.bfloat16).to(cuda_device)
+    slots = torch.cat([torch.arange(n) + 64 * b for b, n in enumerate(lens)]).to(cuda_device)
+    lens_t = torch.tensor(lens, dtype=torch.int32, device=cuda_device)
+
+    def step(q, k, kc, vc, ks, vs):
+        q3attn.paged_write_fp8(k, k * 2, slots, kc, vc, ks, vs)
+        out = q3attn.paged_decode_fp8_append(q + 1, k[:3] - 1, k[3:6], kc, vc, ks, vs, lens_t, table, 0.1)
+        return out * 2, q3attn.paged_read_fp8(kc, vc, ks, vs, slots[:5])[0]
+
+    want = step(q, k, *eager_pool)
+    compiled = torch.compile(step, dynamic=False)
+    compiled(q, k, *[t.clone() for t in pool])
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    got = compiled(q, k, *pool)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - before < pool[0].numel() // 2
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    for a, b in zip(pool, eager_pool):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
