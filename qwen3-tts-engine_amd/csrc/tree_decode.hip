@@ -7,16 +7,23 @@
 //   s_mj = scale q_m . k_j,   o_m = sum_j exp(s_mj - max_j s_mj) v_j / sum_j exp(s_mj - max_j s_mj);   zeros if nothing is seen.
 //
 // A step is 32 keys (two 16-token subtiles, each inside one page) by 16 kMT query rows, on one wave, from registers alone:
-//   S^T = K Q^T   v_mfma_f32_16x16x32_bf16, A = 16 keys x 32 dims, B = Q^T.  Lane l holds key l % 16 and, of each 32 dims,
-//                 the 8 that its quarter g = l / 16 takes: any split of the 128 dims over (step, quarter) is right as long
-//                 as Q has the same, so each quarter takes 16 codes in a row and a load is 16 B (8-bit), 8 dims (bf16).
+//   S^T = K Q^T   A = 16 keys, B = Q^T.  bf16: v_mfma_f32_16x16x32_bf16; lane l holds key l % 16 and, of each 32 dims, the 8
+//                 that its quarter g = l / 16 takes: any split of the 128 dims over (step, quarter) is right as long as Q has
+//                 the same.  8-bit: one v_mfma_scale_f32_16x16x128_f8f6f4 on the codes as they are stored, K's exponent byte
+//                 being its scale operand, against Q in two e4m3 parts (converting K to bf16 first took 444 cycles a step
+//                 instead of 188).
 //   O^T = V^T P^T A = V^T: lane l holds for dim index l % 16 the 8 keys 4 g .. 4 g + 3 of both subtiles, which are the keys
 //                 whose P its S^T registers hold, so P needs no lane moves.  Row i of MFMA j stands for dim 8 i + j: the
 //                 lane loads 8 dims in a row of its 8 keys, and the transpose is byte permutes within the lane.
-// Lane l of O^T then holds 32 dims in a row of query row l % 16.  K is multiplied by its scale as it is converted (exact);
-// V's scale goes onto P.  Scores, statistics and O are fp32; P is rounded to bf16 for the product (2^-8 of each term at
-// worst, the sum l is of the unrounded ones), as the prefill kernel does.
+// Lane l of O^T then holds 32 dims in a row of query row l % 16.  V's scale goes onto P.  Scores, statistics and O are fp32; P
+// is rounded to bf16 for the product (2^-8 of each term at worst, the sum l is of the unrounded ones), as the prefill kernel
+// does.
+#include <float.h>
+#include <limits.h>
+#include <math.h>
+
 #include <algorithm>
+#include <type_traits>
 
 #include "fp8_common.h"
 #include "../../include/q3attn.h"
@@ -32,10 +39,13 @@ constexpr int kD = kRowDims;
 constexpr int kStep = 32;       // keys per step
 constexpr int kWindow = 32;     // steps whose page ids a wave holds at once (one id a lane)
 constexpr int kMergeRow = kD + 4;  // floats per row of the merge buffer (16-byte rows off the bank period)
+constexpr int kRecord = kD + 2;    // floats per query row of a record: o[128], m, l
 enum { kNoKeys = 0, kTree = 1, kAppend = 2 };
 
 typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8_t;
 typedef __attribute__((__vector_size__(4 * sizeof(float)))) float f32x4_t;
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
 
 struct TreeArgs {
   const uint16_t* q;
@@ -56,13 +66,38 @@ struct TreeArgs {
   int max_pages;
   uint16_t* out;
   int64_t o_sb, o_sn, o_sh;
-  float* ws;
-  int nodes, group, hkv, M;
-  int mblocks, nchunk, min_steps;
-  float scale_log2;
+  void* ws;
+  float* rec;  // in ws
+  int batch, nodes, group, hkv, M;
+  uint32_t per_group;  // m / group = m * per_group >> 20 for m < 4096
+  int mblocks;
+  int units, target;  // rows, or chunks at most and as many as there should be
+  int xcd_units;
+  float scale_log2;   // positive
+  uint32_t q_sign;    // turns the signs of a pair of bf16, or nothing
 };
 
+// Query row m's node.
+__device__ __forceinline__ int node_of(const TreeArgs& a, int m) { return (int)(((uint32_t)m * a.per_group) >> 20); }
+
+// The lane's number, worked out where it is asked for.  What derives from it only where rows start and end would else be
+// computed once and hold registers through the loops between.
+__device__ __forceinline__ int lane_now() {
+  int zero = 0;
+  asm volatile("" : "+v"(zero));
+  return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, (uint32_t)zero));
+}
+
 __device__ __forceinline__ int readlane(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+
+// The kernel's arguments read again from where they are passed.  The compiler loads every argument at a kernel's start and
+// holds it in scalar registers, which run out (and spill); what only the end of a row needs goes through here instead.
+__device__ __forceinline__ const TreeArgs& args_again() {
+  typedef __attribute__((address_space(4))) const TreeArgs karg;
+  auto p = (karg*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const TreeArgs*)p;
+}
 
 // The first of the 8 dims that MFMA step c's operand holds in quarter g, and the 16 B piece of the row it lies in.
 template <bool kFp8>
@@ -70,103 +105,188 @@ __device__ __forceinline__ int dim_of(int c, int g) {
   return kFp8 ? (c >> 1) * 64 + g * 16 + (c & 1) * 8 : c * 32 + g * 8;
 }
 
-// A step's keys in registers: the 8-bit pool's codes, or bf16.
+// A step's K and V in registers: the 8-bit pool's codes, or bf16.
 template <bool kFp8>
-struct Keys;
+struct KeyTile;
 template <>
-struct Keys<true> {
-  uint4 k[2][2];
-  uint2 v[2][4];
-  uint32_t ks[2], vs[2];  // K: the scale byte of key l % 16; V: those of keys 4 g .. 4 g + 3
-  int valid[2];           // keys of the subtile that are seen
+struct KeyTile<true> {
+  i32x8_t k[2];
+  uint32_t ks[2];  // scale byte of key l % 16
 };
 template <>
-struct Keys<false> {
+struct KeyTile<false> {
   uint4 k[2][4];
+};
+template <bool kFp8>
+struct ValueTile;
+template <>
+struct ValueTile<true> {
+  uint2 v[2][4];
+  uint32_t vs[2];  // scale bytes of keys 4 g .. 4 g + 3
+};
+template <>
+struct ValueTile<false> {
   uint4 v[2][4];
-  int valid[2];
 };
 
-// One row (b), KV head and block of 16 kMT query rows: where its steps are.
+// Where a step's two subtiles lie in the pool, the same on every lane.
+struct Place {
+  int64_t at[2];    // byte offset of the first key,
+  uint32_t sat[2];  // and of its scale byte
+  int valid[2];     // keys that are seen
+};
+
+// The pool places of a wave's next kWindow steps, one subtile a lane: worked out by the lanes at once, so that a step reads
+// its two with a few lane reads (on the scalar unit it took 120 instructions a step, more than the step's arithmetic).
+struct Window {
+  uint32_t at, sat;  // offset of the first key in 16 bytes, and of its scale byte
+  int valid;         // keys that are seen: 0 past the row's end, and where the table has no page
+};
+
+// Lane l's subtile: half l & 1 of step `step` of row b with L cached tokens; `on`: there is such a step.
+template <bool kFp8>
+__device__ __forceinline__ Window window_of(int b, int L, int step, bool on, int lane) {
+  const TreeArgs& a = args_again();
+  const int tok = kStep * step + 16 * (lane & 1);
+  Window w = {0u, 0u, 0};
+  const int pi = (int)((uint32_t)tok / (uint32_t)a.page_size);
+  if (on && pi < a.max_pages) {
+    const int off = tok - pi * a.page_size;
+    const int page = a.bt[(int64_t)b * a.bt_sb + pi];
+    if ((unsigned)page < (unsigned)a.num_pages) {
+      w.at = (uint32_t)(((int64_t)page * a.sp + (int64_t)off * a.st) >> 4);
+      if constexpr (kFp8) w.sat = (uint32_t)(page * a.ss_p + off);
+      w.valid = max(0, min(16, L - tok));
+    }
+  }
+  return w;
+}
+
+// One row (b), KV head and block of 16 kMT query rows.
 struct Work {
   int b, h, mb;
-  int L;       // cached tokens that are attended; < 0: the row is skipped
-  int Tc, T;   // steps of cached keys, and with the own keys'
+  int L;   // cached tokens that are attended
+  int Tc;  // steps of cached keys; the own keys' come behind them
 };
 
 template <int kMT>
 struct State {
   f32x4_t o[kMT][8];
-  float m[kMT], l[kMT];  // of query row l % 16; l: this quarter's keys only, until the merge
+  float m[kMT], l[kMT];  // of query row l % 16: maximum of the unscaled scores; sum, of this quarter's keys until the merge
 };
 
-// How the row's T steps split over chunks: `size` steps each, the first `live` chunks not empty.
-__device__ __forceinline__ void split_of(const TreeArgs& a, int T, int& size, int& live) {
-  size = max((T + a.nchunk - 1) / a.nchunk, a.min_steps);
-  live = (T + size - 1) / size;
-}
-
-__device__ __forceinline__ int row_tokens(const TreeArgs& a, int b, int mode) {
+__device__ __forceinline__ int row_tokens(int b, int mode) {
+  const TreeArgs& a = args_again();
   const int n = a.seqlens[b];
   const int cap = a.max_pages * a.page_size;
   if (mode == kAppend) return n < cap ? n : -1;  // no room for the new row: skipped
   return min(n, cap);
 }
 
-__device__ __forceinline__ int steps_of(const TreeArgs& a, int L, int mode) {
+__device__ __forceinline__ int steps_of(int L, int mode) {
   if (L < 0) return 0;
+  const TreeArgs& a = args_again();
   return (L + kStep - 1) / kStep + (mode == kTree ? (a.nodes + kStep - 1) / kStep : mode == kAppend ? 1 : 0);
 }
 
+// Cache policy of the pool's loads.  Non-temporal where a load instruction takes whole 128-byte lines that no other workgroup
+// reads.
+constexpr int kNt = 2;
+
+// A step's keys are loaded from the pool by three functions.
+//
+// A line is 8 lanes' 16 bytes, but an A operand has a row on 4 lanes only, so loading operand rows as they are takes each line
+// in two halves by two instructions, which the non-temporal policy does not suit (a twentieth of the decode's time).  So two
+// lanes that hold neighbouring rows load from one key at a time:
+//   8-bit codes   load i: half r & 1 of key (r & ~1) + i.  The two lanes then exchange what is the other's (two DPP selects a
+//                 register, before the product).
+//   bf16, kPaired (16 query rows): operand row r of a load holds half (r & 1) of a line of key (r & ~3) + 2 i + ((r >> 1) & 1),
+//                 i the load's pair.  Even rows have to meet Q's dims of the lines' first half, odd rows the second's: two
+//                 products of which each uses half, and the score of a key is the sum of two neighbouring rows, which one lane
+//                 holds.  The lane's four keys stay 4 g .. 4 g + 3.  With more query rows the second product costs too much.
+//
+// No branches and always the same loads, also for a step that is not there (its page ids are -1): only so does the compiler
+// know how many newer loads may be in flight when older ones are waited for, and not wait for all.
+// `live`: there is such a step; its places are not used else.  tokens: what the row has from the step on.
 template <bool kFp8>
-__device__ __forceinline__ void load_cached(const TreeArgs& a, const Work& w, int step, int slot, int pid, int poff, int lane,
-                                            Keys<kFp8>& x) {
+__device__ __forceinline__ Place place_of(const Window& w, int slot, bool live, int tokens) {
+  Place p;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    p.at[u] = (int64_t)(uint32_t)readlane((int)w.at, 2 * slot + u) << 4;
+    if constexpr (kFp8) p.sat[u] = (uint32_t)readlane((int)w.sat, 2 * slot + u);
+    const int n = readlane(w.valid, 2 * slot + u), left = tokens - 16 * u;
+    p.valid[u] = live ? (n < left ? n : left < 0 ? 0 : left) : 0;  // (min as a chain of scalar selects)
+  }
+  return p;
+}
+
+// Descriptors end with the last seen key: what lies past it is not read and comes as zeros.
+template <bool kFp8>
+__device__ __forceinline__ uint32_t extent(const TreeArgs& a, int valid) {
+  return valid > 0 ? (uint32_t)(valid - 1) * (uint32_t)a.st + (kFp8 ? kD : 2 * kD) : 0u;
+}
+
+template <bool kOnce>
+__device__ __forceinline__ void load_k(const TreeArgs& a, const Place& p, int lane, KeyTile<true>& x) {
   const int r = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    const int page = readlane(pid, 2 * slot + u), off = readlane(poff, 2 * slot + u);
-    int nv = min(16, w.L - (kStep * step + 16 * u));
-    if ((unsigned)page >= (unsigned)a.num_pages) nv = 0;
-    nv = max(nv, 0);
-    x.valid[u] = nv;
-    // Descriptors that end with the last seen key: what lies past it is not read and comes as zeros.
-    const int64_t at = nv > 0 ? (int64_t)page * a.sp + (int64_t)w.h * a.sh + (int64_t)off * a.st : 0;
-    const uint32_t bytes = nv > 0 ? (uint32_t)(nv - 1) * (uint32_t)a.st + (kFp8 ? kD : 2 * kD) : 0u;
-    const auto rk = make_rsrc(a.kc + at, bytes), rv = make_rsrc(a.vc + at, bytes);
-    const uint32_t krow = (uint32_t)r * (uint32_t)a.st, vrow = (uint32_t)(4 * g) * (uint32_t)a.st;
-    if constexpr (kFp8) {
+    const auto rk = make_rsrc(a.kc + p.at[u], extent<true>(a, p.valid[u]));
+    const uint32_t row = (uint32_t)(r & ~1) * (uint32_t)a.st + 64 * (r & 1) + 16 * g;
+    auto ld = [&](uint32_t o) {
+      return __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rk, (int)o, 0, kOnce ? kNt : 0));
+    };
+    x.k[u] = __builtin_shufflevector(ld(row), ld(row + (uint32_t)a.st), 0, 1, 2, 3, 4, 5, 6, 7);
+    const auto rs = make_rsrc(a.ks + p.sat[u], p.valid[u] > 0 ? 16 : 0);
+    x.ks[u] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rs, r, 0, 0);
+  }
+}
+template <bool kPaired>
+__device__ __forceinline__ void load_k(const TreeArgs& a, const Place& p, int lane, KeyTile<false>& x) {
+  const int r = lane & 15, g = lane >> 4;
+  const uint32_t st = (uint32_t)a.st;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) x.k[u][i] = buffer_load16(rk, krow + 64 * i + 16 * g);
+  for (int u = 0; u < 2; ++u) {
+    const auto rk = make_rsrc(a.kc + p.at[u], extent<false>(a, p.valid[u]));
+    if constexpr (kPaired) {
+      const uint32_t row = (uint32_t)((r & ~3) + ((r >> 1) & 1)) * st + 64 * (r & 1) + 16 * g;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        x.v[u][i] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rv, (int)(vrow + i * a.st + 8 * r), 0, 0));
-      const int64_t sat = nv > 0 ? (int64_t)page * a.ss_p + (int64_t)w.h * a.ss_h + off : 0;
-      const auto rs = make_rsrc(a.ks + sat, nv > 0 ? 16 : 0), rt = make_rsrc(a.vs + sat, nv > 0 ? 16 : 0);
-      x.ks[u] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rs, r, 0, 0);
-      x.vs[u] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rt, 4 * g, 0, 0);
+      for (int i = 0; i < 4; ++i)  // pair i >> 1, line i & 1
+        x.k[u][i] = buffer_load16_stream(rk, row + 2 * (i >> 1) * st + 128 * (i & 1));
     } else {
+      const uint32_t row = (uint32_t)r * st + 16 * g;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x.k[u][i] = buffer_load16(rk, krow + 64 * i + 16 * g);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x.v[u][i] = buffer_load16(rv, vrow + i * a.st + 16 * r);
+      for (int i = 0; i < 4; ++i) x.k[u][i] = buffer_load16(rk, row + 64 * i);
     }
   }
 }
 
-// The A operand of S^T at MFMA step c.
-__device__ __forceinline__ bf16x8_t k_operand(const Keys<true>& x, int u, int c) {
-  const uint4 w = x.k[u][c >> 1];
-  const uint32_t lo = (c & 1) ? w.z : w.x, hi = (c & 1) ? w.w : w.y;
-  const float f = fp8_scale(x.ks[u]);
-  return __builtin_bit_cast(bf16x8_t, make_uint4(fp8_pair<false>(lo, f), fp8_pair<true>(lo, f), fp8_pair<false>(hi, f),
-                                                 fp8_pair<true>(hi, f)));
-}
-__device__ __forceinline__ bf16x8_t k_operand(const Keys<false>& x, int u, int c) {
-  return __builtin_bit_cast(bf16x8_t, x.k[u][c]);
+template <bool kFp8, bool kOnce>
+__device__ __forceinline__ void load_v(const TreeArgs& a, const Place& p, int lane, ValueTile<kFp8>& x) {
+  const int r = lane & 15, g = lane >> 4;
+  const uint32_t st = (uint32_t)a.st;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const auto rv = make_rsrc(a.vc + p.at[u], extent<kFp8>(a, p.valid[u]));
+    const uint32_t row = (uint32_t)(4 * g) * st + (kFp8 ? 8 : 16) * r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (kFp8) {
+        x.v[u][i] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rv, (int)(row + i * st), 0, kOnce ? kNt : 0));
+      } else {
+        x.v[u][i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rv, (int)(row + i * st), 0, kOnce ? kNt : 0));
+      }
+    }
+    if constexpr (kFp8) {
+      const auto rt = make_rsrc(a.vs + p.sat[u], p.valid[u] > 0 ? 16 : 0);
+      x.vs[u] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rt, 4 * g, 0, 0);
+    }
+  }
 }
 
 // The A operands of O^T for dims 8 i + j, j = jj and jj + 1 (jj even): the pairs of keys (0, 1), (2, 3) of both subtiles.
-__device__ __forceinline__ void v_operands(const Keys<true>& x, int jj, bf16x8_t& a0, bf16x8_t& a1) {
+__device__ __forceinline__ void v_operands(const ValueTile<true>& x, int jj, bf16x8_t& a0, bf16x8_t& a1) {
   uint32_t p0[4], p1[4];
 #pragma unroll
   for (int u = 0; u < 2; ++u)
@@ -183,7 +303,7 @@ __device__ __forceinline__ void v_operands(const Keys<true>& x, int jj, bf16x8_t
   a1 = __builtin_bit_cast(bf16x8_t, make_uint4(p1[0], p1[1], p1[2], p1[3]));
 }
 __device__ __forceinline__ uint32_t word_of(const uint4& w, int i) { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
-__device__ __forceinline__ void v_operands(const Keys<false>& x, int jj, bf16x8_t& a0, bf16x8_t& a1) {
+__device__ __forceinline__ void v_operands(const ValueTile<false>& x, int jj, bf16x8_t& a0, bf16x8_t& a1) {
   uint32_t p0[4], p1[4];
 #pragma unroll
   for (int u = 0; u < 2; ++u)
@@ -197,62 +317,212 @@ __device__ __forceinline__ void v_operands(const Keys<false>& x, int jj, bf16x8_
   a1 = __builtin_bit_cast(bf16x8_t, make_uint4(p1[0], p1[1], p1[2], p1[3]));
 }
 
-__device__ __forceinline__ float v_scale(const Keys<true>& x, int u, int i) { return fp8_scale((x.vs[u] >> (8 * i)) & 0xffu); }
-__device__ __forceinline__ float v_scale(const Keys<false>&, int, int) { return 1.f; }
 
-// One step.  kMasked: seen[t] tells which of the lane's 8 keys (bit 4 u + i) its query row sees; else every valid one.
-template <bool kFp8, bool kScaledV, bool kMasked, int kMT>
-__device__ __forceinline__ void step(const Keys<kFp8>& x, const bf16x8_t (&q)[kMT][4], const uint32_t (&seen)[kMT], float scale,
-                                     int lane, State<kMT>& st) {
-  const int g = lane >> 4;
-  f32x4_t s[kMT][2];
+// Q^T as B operands: bf16 as it is, or, against 8-bit keys, in two e4m3 parts.
+//
+// The matrix instruction takes K's codes and its power-of-two scale (one byte a key) as they are, with Q as hi + lo: of q's 8
+// significant bits hi = e4m3(q / 2^e) holds the upper 4 and lo = e4m3(16 (q / 2^e - hi)) at 2^(e - 4) the rest.  That is q
+// itself down to 2^-14 of its row's largest element and 2^-22 of that element below, so the scores are those of the bf16 row,
+// and a step's two products (K = 128 each) replace 32 conversions and 8 products in bf16.
+template <bool kFp8, int kMT>
+struct Query;
+template <int kMT>
+struct Query<false, kMT> {
+  bf16x8_t v[kMT][4];
+};
+template <int kMT>
+struct Query<true, kMT> {
+  i32x8_t hi[kMT], lo[kMT];
+  int s[kMT];  // the exponent byte of hi; lo's is 4 less
+};
+
+// The largest over the four lanes of a query row (small integers order as floats do).
+__device__ __forceinline__ uint32_t row_max(uint32_t x) {
+  return (uint32_t)__float_as_int(max_xor32(max_xor16(__int_as_float((int)x))));
+}
+template <int kMT>
+__device__ __forceinline__ void prepare(const bf16x8_t (&q)[kMT][4], Query<false, kMT>& x) {
 #pragma unroll
-  for (int u = 0; u < 2; ++u)
+  for (int t = 0; t < kMT; ++t)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const bf16x8_t kf = k_operand(x, u, c);
-#pragma unroll
-      for (int t = 0; t < kMT; ++t)
-        s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[t][c], c == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : s[t][u], 0, 0, 0);
-    }
-  bf16x8_t pb[kMT];
+    for (int c = 0; c < 4; ++c) x.v[t][c] = q[t][c];
+}
+template <int kMT>
+__device__ __forceinline__ void prepare(const bf16x8_t (&q)[kMT][4], Query<true, kMT>& x) {
 #pragma unroll
   for (int t = 0; t < kMT; ++t) {
-    float y[2][4], top = -INFINITY;
+    uint32_t w[16];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint4 e = __builtin_bit_cast(uint4, q[t][c]);
+      w[4 * c] = e.x;
+      w[4 * c + 1] = e.y;
+      w[4 * c + 2] = e.z;
+      w[4 * c + 3] = e.w;
+    }
+    uint32_t top = 0;  // of the magnitude bits, whatever they are
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = pk_max_u16(top, w[i] & 0x7fff7fffu);
+    top = row_max(halves_max(top));
+    // Rows with infinities and NaN, or close to the largest bf16, are rare: their codes need care.
+    const bool rare = __builtin_amdgcn_ballot_w64(top >= 0x7f00u) != 0;
+    if (rare) top = row_max(halves_max(bf16_amax_pair(w)));
+    const uint32_t sb = fp8_scale_byte(top);
+    const float inv = fp8_inv_scale(sb);
+    x.s[t] = (int)sb;
+    int hi[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      hi[i] = __builtin_amdgcn_cvt_pk_fp8_f32(bf16_lo(w[2 * i]) * inv, bf16_hi(w[2 * i]) * inv, 0, false);
+      hi[i] = __builtin_amdgcn_cvt_pk_fp8_f32(bf16_lo(w[2 * i + 1]) * inv, bf16_hi(w[2 * i + 1]) * inv, hi[i], true);
+    }
+    if (rare) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) hi[i] = (int)fp8_codes4(w[2 * i], w[2 * i + 1], sb);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const auto h0 = __builtin_amdgcn_cvt_pk_f32_fp8(hi[i], false), h1 = __builtin_amdgcn_cvt_pk_f32_fp8(hi[i], true);
+      auto rest = [&](float y, float h) { return __builtin_fmaf(y, inv, -h) * 16.f; };  // at most 256 (at byte 247: 240)
+      int lo = __builtin_amdgcn_cvt_pk_fp8_f32(rest(bf16_lo(w[2 * i]), h0[0]), rest(bf16_hi(w[2 * i]), h0[1]), 0, false);
+      lo = __builtin_amdgcn_cvt_pk_fp8_f32(rest(bf16_lo(w[2 * i + 1]), h1[0]), rest(bf16_hi(w[2 * i + 1]), h1[1]), lo, true);
+      x.hi[t][i] = hi[i];
+      x.lo[t][i] = lo;
+    }
+  }
+}
+
+// A step's scores S^T, unscaled.  kSwapped: the keys are as load_k left them.
+template <bool kSwapped, int kMT>
+__device__ __forceinline__ void scores(const KeyTile<true>& x, const Query<true, kMT>& q, f32x4_t (&s)[kMT][2]) {
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    i32x8_t k = x.k[u];
+    if constexpr (kSwapped) {
+      const bool odd = (threadIdx.x & 1) != 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int even_gets = __builtin_amdgcn_update_dpp(0, k[i], kDppXor1, 0xF, 0xF, false);
+        const int odd_gets = __builtin_amdgcn_update_dpp(0, k[i + 4], kDppXor1, 0xF, 0xF, false);
+        k[i + 4] = odd ? k[i + 4] : even_gets;
+        k[i] = odd ? odd_gets : k[i];
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < kMT; ++t) {
+      const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+      s[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q.lo[t], zero, 0, 0, 0, (int)x.ks[u], 0, q.s[t] - 4);
+      s[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q.hi[t], s[t][u], 0, 0, 0, (int)x.ks[u], 0, q.s[t]);
+    }
+  }
+}
+template <bool kPaired, int kMT>
+__device__ __forceinline__ void scores(const KeyTile<false>& x, const Query<false, kMT>& q, f32x4_t (&s)[kMT][2]) {
+  const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    if constexpr (kPaired) {
+      static_assert(kMT == 1, "paired rows cost a second product");
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        f32x4_t even = zero, odd = zero;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {  // line e
+          const bf16x8_t kf = __builtin_bit_cast(bf16x8_t, x.k[u][2 * i + e]);
+          even = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q.v[0][2 * e], even, 0, 0, 0);
+          odd = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q.v[0][2 * e + 1], odd, 0, 0, 0);
+        }
+        s[0][u][2 * i] = even[0] + odd[1];
+        s[0][u][2 * i + 1] = even[2] + odd[3];
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int t = 0; t < kMT; ++t)
+          s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x.k[u][c]), q.v[t][c],
+                                                            c == 0 ? zero : s[t][u], 0, 0, 0);
+    }
+  }
+}
+
+// The scores to probabilities: scaled, masked, exp2 of them minus the running maximum, which with the sum is updated and O
+// rescaled to.
+// kMasked: seen[t] tells which of the lane's 8 keys (bit 4 u + i) its query row sees; else the subtiles' valid ones.
+template <bool kMasked, int kMT>
+__device__ __forceinline__ void softmax(const int (&valid)[2], const uint32_t (&seen)[kMT], float scale,
+                                        f32x4_t (&s)[kMT][2], State<kMT>& st) {
+  const bool full = valid[0] == 16 && valid[1] == 16;
+#pragma unroll
+  for (int t = 0; t < kMT; ++t) {
+    if (kMasked || !full) {
+      const int g = lane_now() >> 4;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool ok = kMasked ? ((seen[t] >> (4 * u + i)) & 1) != 0 : 4 * g + i < valid[u];
+          s[t][u][i] = ok ? s[t][u][i] : -INFINITY;
+        }
+    }
+    float top = fmaxf(fmaxf(fmaxf(s[t][0][0], s[t][0][1]), fmaxf(s[t][0][2], s[t][0][3])),
+                      fmaxf(fmaxf(s[t][1][0], s[t][1][1]), fmaxf(s[t][1][2], s[t][1][3])));
+    top = max_xor32(max_xor16(top));
+    // O and l are rescaled only when some query row's maximum has grown (a factor of 1 changes nothing).
+    if (__builtin_amdgcn_ballot_w64(top > st.m[t]) != 0) {
+      const float m = fmaxf(st.m[t], top);
+      const float alpha = fast_exp2((st.m[t] - (m == -INFINITY ? 0.f : m)) * scale);
+      st.m[t] = m;
+      st.l[t] *= alpha;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st.o[t][j][i] *= alpha;
+    }
+    const float base = st.m[t] == -INFINITY ? 0.f : st.m[t] * scale;  // nothing seen so far: every exp2 below is of -inf
+    float sum = 0.f;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const bool ok = kMasked ? ((seen[t] >> (4 * u + i)) & 1) != 0 : 4 * g + i < x.valid[u];
-        y[u][i] = ok ? s[t][u][i] * scale : -INFINITY;
-        top = fmaxf(top, y[u][i]);
+        s[t][u][i] = fast_exp2(__builtin_fmaf(s[t][u][i], scale, -base));
+        sum += s[t][u][i];
       }
-    top = max_xor32(max_xor16(top));
-    const float m = fmaxf(st.m[t], top);
-    const float base = m == -INFINITY ? 0.f : m;  // nothing seen so far: every exp2 below is of -inf
-    const float alpha = fast_exp2(st.m[t] - base);
-    st.m[t] = m;
-    float sum = 0.f;
+    st.l[t] += sum;
+  }
+}
+
+// O^T += V^T P^T.
+template <bool kFp8, int kMT>
+__device__ __forceinline__ void values(const ValueTile<kFp8>& x, const int (&valid)[2], int lane, const f32x4_t (&p)[kMT][2],
+                                       State<kMT>& st) {
+  const int g = lane >> 4;
+  float f[2][4];  // V's scales
+  if constexpr (kFp8) {
+    uint32_t bytes[2] = {x.vs[0], x.vs[1]};
+    if (valid[0] != 16 || valid[1] != 16) {  // the scale byte of a key that is not seen may be anything
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int left = max(0, min(4, valid[u] - 4 * g));
+        bytes[u] &= (uint32_t)((1ull << (8 * left)) - 1);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[u][i] = fp8_scale((bytes[u] >> (8 * i)) & 0xffu);
+  }
+  bf16x8_t pb[kMT];
+#pragma unroll
+  for (int t = 0; t < kMT; ++t) {
     uint32_t pk[4];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      float pv[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float p = fast_exp2(y[u][i] - base);
-        sum += p;
-        const bool ok = kMasked ? ((seen[t] >> (4 * u + i)) & 1) != 0 : 4 * g + i < x.valid[u];
-        pv[i] = kScaledV ? (ok ? p * v_scale(x, u, i) : 0.f) : p;  // the scale byte of a key not seen may be anything
-      }
-      pk[2 * u] = pack_bf16x2(pv[0], pv[1]);
-      pk[2 * u + 1] = pack_bf16x2(pv[2], pv[3]);
+      auto scaled = [&](int i) { return kFp8 ? p[t][u][i] * f[u][i] : p[t][u][i]; };
+      pk[2 * u] = pack_bf16x2(scaled(0), scaled(1));
+      pk[2 * u + 1] = pack_bf16x2(scaled(2), scaled(3));
     }
-    st.l[t] = st.l[t] * alpha + sum;
     pb[t] = __builtin_bit_cast(bf16x8_t, make_uint4(pk[0], pk[1], pk[2], pk[3]));
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) st.o[t][j][i] *= alpha;
   }
 #pragma unroll
   for (int jj = 0; jj < 8; jj += 2) {
@@ -282,9 +552,10 @@ __device__ __forceinline__ uint32_t halves_of_kind(uint32_t w, int kind) {
 }
 
 // Adds to O what the own V elements that are not finite give the rows that see their keys: for each kind, a product of
-// zeros and ones counts them.
+// zeros and ones counts them.  (The elements are read again: holding them would cost every call 32 registers.)
 template <int kMT>
-__device__ __forceinline__ void add_not_finite(const Keys<false>& v, const uint32_t (&seen)[kMT], State<kMT>& st) {
+__device__ __forceinline__ void add_not_finite(const uint16_t* vb, int ts, const uint32_t (&seen)[kMT], State<kMT>& st) {
+  const TreeArgs& a = args_again();
   bf16x8_t sees[kMT];
 #pragma unroll
   for (int t = 0; t < kMT; ++t) {
@@ -296,13 +567,15 @@ __device__ __forceinline__ void add_not_finite(const Keys<false>& v, const uint3
   }
 #pragma unroll 1
   for (int kind = 0; kind < 3; ++kind) {
+    const int lane = lane_now();  // (nothing of the elements is computed ahead of the loop)
     const float what = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __builtin_nanf("");
-    Keys<false> x;
+    ValueTile<false> x;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint4 e = v.v[u][i];
+        const int j = kStep * ts + 16 * u + 4 * (lane >> 4) + i;
+        const uint4 e = ld16(vb + (int64_t)min(j, a.nodes - 1) * a.vn_sn + 8 * (lane & 15));  // a key of none is not seen
         x.v[u][i] = make_uint4(halves_of_kind(e.x, kind), halves_of_kind(e.y, kind), halves_of_kind(e.z, kind),
                                halves_of_kind(e.w, kind));
       }
@@ -326,76 +599,103 @@ __device__ __forceinline__ void add_not_finite(const Keys<false>& v, const uint3
 // The nodes' own keys 32 ts .. + 31, in bf16, with each lane's query rows' view of its 8 keys.  An own V element that is
 // not finite must not reach the rows that do not see its key (0 * inf in the product): such elements are zeroed in the
 // product and added afterwards for the rows that see them.
-template <bool kFp8, int kMT>
-__device__ void tree_step(const TreeArgs& a, const Work& w, int ts, const bf16x8_t (&q)[kMT][4], int lane, State<kMT>& st) {
+template <bool kFp8, int kMT, bool kTight>
+__device__ __forceinline__ void tree_step(const Work& w, int ts, const Query<false, kMT>& q, State<kMT>& st) {
+  const int lane = lane_now();
   const int r = lane & 15, g = lane >> 4;
+  const TreeArgs& a = args_again();
   const uint16_t* kb = a.kn + (int64_t)w.b * a.kn_sb + (int64_t)w.h * a.kn_sh;
   const uint16_t* vb = a.vn + (int64_t)w.b * a.vn_sb + (int64_t)w.h * a.vn_sh;
-  Keys<false> x;
-  bool odd = false;
+  KeyTile<false> x;
+  ValueTile<false> y;
+  // Rows past the last node read the last one's, without a branch: no query row sees them, and their V is zeroed.
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    const int j0 = kStep * ts + 16 * u;
-    x.valid[u] = max(0, min(16, a.nodes - j0));
-    const int jk = j0 + r;
+    const int j = min(kStep * ts + 16 * u + r, a.nodes - 1);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      x.k[u][c] = make_uint4(0u, 0u, 0u, 0u);
-      if (jk < a.nodes) x.k[u][c] = ld16(kb + (int64_t)jk * a.kn_sn + dim_of<kFp8>(c, g));
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int jv = j0 + 4 * g + i;
-      x.v[u][i] = make_uint4(0u, 0u, 0u, 0u);
-      if (jv < a.nodes) x.v[u][i] = ld16(vb + (int64_t)jv * a.vn_sn + 8 * r);
-      const uint4 e = x.v[u][i];
-      odd = odd || not_finite_pair(e.x) || not_finite_pair(e.y) || not_finite_pair(e.z) || not_finite_pair(e.w);
-    }
+    for (int c = 0; c < 4; ++c) x.k[u][c] = ld16(kb + (int64_t)j * a.kn_sn + dim_of<kFp8>(c, g));
   }
-  const bool any_odd = __builtin_amdgcn_ballot_w64(odd) != 0;
-  Keys<false> kinds;
-  if (any_odd) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint4 e = x.v[u][i];
-        kinds.v[u][i] = e;
-        x.v[u][i] = make_uint4(finite_halves(e.x), finite_halves(e.y), finite_halves(e.z), finite_halves(e.w));
-      }
-  }
-  uint32_t seen[kMT];
-#pragma unroll
-  for (int t = 0; t < kMT; ++t) {
-    const int m = (w.mb * kMT + t) * 16 + r;
-    const int n = m / a.group;
-    seen[t] = 0;
+  auto load_values = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int j = kStep * ts + 16 * u + 4 * g + i;
-        bool ok = n < a.nodes && j < a.nodes;
-        if (ok) ok = a.mask != nullptr ? a.mask[(int64_t)w.b * a.m_sb + (int64_t)n * a.m_sn + j] != 0 : j <= n;
-        seen[t] |= ok ? 1u << (4 * u + i) : 0u;
+        const uint4 e = ld16(vb + (int64_t)min(j, a.nodes - 1) * a.vn_sn + 8 * r);
+        const uint32_t keep = j < a.nodes ? ~0u : 0u;
+        y.v[u][i] = make_uint4(e.x & keep, e.y & keep, e.z & keep, e.w & keep);
+      }
+  };
+  if constexpr (!kTight) load_values();
+  uint32_t seen[kMT];
+#pragma unroll
+  for (int t = 0; t < kMT; ++t) {
+    const int n = node_of(a, (w.mb * kMT + t) * 16 + r);
+    seen[t] = 0;
+    if (a.mask != nullptr) {
+      const uint8_t* row = a.mask + (int64_t)w.b * a.m_sb + (int64_t)min(n, a.nodes - 1) * a.m_sn;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          seen[t] |= (row[min(kStep * ts + 16 * u + 4 * g + i, a.nodes - 1)] != 0 ? 1u : 0u) << (4 * u + i);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) seen[t] |= (kStep * ts + 16 * u + 4 * g + i <= n ? 1u : 0u) << (4 * u + i);
+    }
+    // keys past the last node, and query rows of none
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int left = n < a.nodes ? max(0, min(4, a.nodes - (kStep * ts + 16 * u + 4 * g))) : 0;
+      seen[t] &= ~(((0xfu << left) & 0xfu) << (4 * u));
+    }
+  }
+  const int any[2] = {16, 16};
+  f32x4_t sc[kMT][2];
+  scores<false, kMT>(x, q, sc);
+  if constexpr (kTight) {  // the registers do not hold V beside K
+    __builtin_amdgcn_sched_barrier(0);
+    load_values();
+  }
+  softmax<true, kMT>(any, seen, a.scale_log2, sc, st);
+  bool odd = false;
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 e = y.v[u][i];
+      odd = odd || not_finite_pair(e.x) || not_finite_pair(e.y) || not_finite_pair(e.z) || not_finite_pair(e.w);
+    }
+  const bool any_odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+  if (any_odd) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint4 e = y.v[u][i];
+        y.v[u][i] = make_uint4(finite_halves(e.x), finite_halves(e.y), finite_halves(e.z), finite_halves(e.w));
       }
   }
-  step<false, false, true, kMT>(x, q, seen, a.scale_log2, lane, st);
-  if (any_odd) add_not_finite<kMT>(kinds, seen, st);
+  values<false, kMT>(y, any, lane, sc, st);
+  if (any_odd) add_not_finite<kMT>(vb, ts, seen, st);
 }
 
 // The append form's new row, quantised as the write kernel does and stored, then attended as a cached subtile of one key.
-__device__ __forceinline__ void append_keys(const TreeArgs& a, const Work& w, int lane, bool store, Keys<true>& x) {
+__device__ __forceinline__ void append_keys(const TreeArgs& a, const Work& w, bool store, KeyTile<true>& x, ValueTile<true>& y, int& valid) {
+  const int lane = lane_now();
   const int r = lane & 15, g = lane >> 4;
-  const uint16_t* kb = a.kn + (int64_t)w.b * a.kn_sb + (int64_t)w.h * a.kn_sh;
-  const uint16_t* vb = a.vn + (int64_t)w.b * a.vn_sb + (int64_t)w.h * a.vn_sh;
-  const int pi = w.L / a.page_size, off = w.L - pi * a.page_size;
-  const int page = a.bt[(int64_t)w.b * a.bt_sb + pi];
+  const TreeArgs& more = args_again();
+  const uint16_t* kb = more.kn + (int64_t)w.b * more.kn_sb + (int64_t)w.h * more.kn_sh;
+  const uint16_t* vb = more.vn + (int64_t)w.b * more.vn_sb + (int64_t)w.h * more.vn_sh;
+  const int pi = w.L / more.page_size, off = w.L - pi * more.page_size;
+  const int page = more.bt[(int64_t)w.b * more.bt_sb + pi];
   const bool ok = (unsigned)page < (unsigned)a.num_pages;
   uint32_t kw[16], vw[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint4 e = ld16(kb + 64 * (i >> 1) + 16 * g + 8 * (i & 1));
+    const uint4 e = ld16(kb + dim_of<true>(i, g));
     kw[4 * i] = e.x;
     kw[4 * i + 1] = e.y;
     kw[4 * i + 2] = e.z;
@@ -407,7 +707,7 @@ __device__ __forceinline__ void append_keys(const TreeArgs& a, const Work& w, in
   vw[2] = e.z;
   vw[3] = e.w;
   uint32_t km = halves_max(bf16_amax_pair(kw)), vm = halves_max(bf16_amax_pair(vw));
-  km = (uint32_t)__float_as_int(max_xor32(max_xor16(__int_as_float((int)km))));  // small integers order as floats do
+  km = row_max(km);
   vm = dpp_max_u32<kDppXor1>(vm);
   vm = dpp_max_u32<kDppXor2>(vm);
   vm = dpp_max_u32<kDppHalfMirror>(vm);
@@ -415,13 +715,11 @@ __device__ __forceinline__ void append_keys(const TreeArgs& a, const Work& w, in
   const uint32_t ks = fp8_scale_byte(km), vs = fp8_scale_byte(vm);
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    x.valid[u] = 0;
     x.ks[u] = ks;
-    x.vs[u] = vs;
+    y.vs[u] = vs;
+    x.k[u] = i32x8_t{0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < 2; ++i) x.k[u][i] = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x.v[u][i] = make_uint2(0u, 0u);
+    for (int i = 0; i < 4; ++i) y.v[u][i] = make_uint2(0u, 0u);
   }
   uint4 kc[2];
 #pragma unroll
@@ -429,18 +727,17 @@ __device__ __forceinline__ void append_keys(const TreeArgs& a, const Work& w, in
     kc[i] = make_uint4(fp8_codes4(kw[8 * i], kw[8 * i + 1], ks), fp8_codes4(kw[8 * i + 2], kw[8 * i + 3], ks),
                        fp8_codes4(kw[8 * i + 4], kw[8 * i + 5], ks), fp8_codes4(kw[8 * i + 6], kw[8 * i + 7], ks));
   const uint2 vc = make_uint2(fp8_codes4(vw[0], vw[1], vs), fp8_codes4(vw[2], vw[3], vs));
-  x.valid[0] = ok ? 1 : 0;
+  valid = ok ? 1 : 0;
   if (r == 0) {
-    x.k[0][0] = kc[0];
-    x.k[0][1] = kc[1];
+    x.k[0] = __builtin_shufflevector(__builtin_bit_cast(i32x4_t, kc[0]), __builtin_bit_cast(i32x4_t, kc[1]), 0, 1, 2, 3, 4, 5, 6, 7);
   }
-  if (g == 0) x.v[0][0] = vc;
+  if (g == 0) y.v[0][0] = vc;
   if (store && ok) {
-    const int64_t at = (int64_t)page * a.sp + (int64_t)w.h * a.sh + (int64_t)off * a.st;
-    const int64_t sat = (int64_t)page * a.ss_p + (int64_t)w.h * a.ss_h + off;
+    const int64_t at = (int64_t)page * a.sp + (int64_t)off * a.st;
+    const int64_t sat = (int64_t)page * a.ss_p + off;
     if (r == 0) {
-      st16(a.kc + at + 16 * g, kc[0]);
-      st16(a.kc + at + 64 + 16 * g, kc[1]);
+      st16(a.kc + at + dim_of<true>(0, g), kc[0]);
+      st16(a.kc + at + dim_of<true>(2, g), kc[1]);
     }
     if (g == 0) *reinterpret_cast<u32x2*>(a.vc + at + 8 * r) = __builtin_bit_cast(u32x2, vc);
     if (lane == 0) {
@@ -450,32 +747,8 @@ __device__ __forceinline__ void append_keys(const TreeArgs& a, const Work& w, in
   }
 }
 
-// Workgroup: (chunk of a row's steps, KV head, block of 16 kMT query rows).  Its kW waves take the chunk's steps in turn,
-// each with a state of its own, and merge in LDS.  A row of one live chunk is finished here; otherwise the chunk's
-// (m, l, o) goes into the workspace for the merge kernel.  The KV head is the fastest grid dimension: workgroups go to the
-// 8 XCDs in turn, so with 8 heads each L2 holds one head's keys for all their readers.
-template <bool kFp8, int kMode, int kMT, int kW>
-__global__ __launch_bounds__(64 * kW) void tree_kernel(const TreeArgs a) {
-  __shared__ __align__(16) float s_o[kW][16][kMergeRow];
-  __shared__ float s_m[kW][16], s_l[kW][16];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r = lane & 15, g = lane >> 4;
-  Work w;
-  int x = blockIdx.x;
-  w.h = x % a.hkv;
-  x /= a.hkv;
-  w.mb = x % a.mblocks;
-  const int chunk = x / a.mblocks;
-  w.b = blockIdx.y;
-  w.L = row_tokens(a, w.b, kMode);
-  w.T = steps_of(a, w.L, kMode);
-  w.Tc = w.L > 0 ? (w.L + kStep - 1) / kStep : 0;
-  int size, live;
-  split_of(a, w.T, size, live);
-  if (chunk >= max(live, 1)) return;
-  const int s0 = chunk * size, s1 = min(w.T, s0 + size);
-
-  State<kMT> st;
+template <int kMT>
+__device__ __forceinline__ void clear(State<kMT>& st) {
 #pragma unroll
   for (int t = 0; t < kMT; ++t) {
     st.m[t] = -INFINITY;
@@ -483,113 +756,165 @@ __global__ __launch_bounds__(64 * kW) void tree_kernel(const TreeArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) st.o[t][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
+}
 
-  if (s0 + wave < s1) {
-    bf16x8_t q[kMT][4];
-#pragma unroll
-    for (int t = 0; t < kMT; ++t) {
-      const int m = (w.mb * kMT + t) * 16 + r;
-      const int n = m / a.group;
-      const uint16_t* qp = a.q + (int64_t)w.b * a.q_sb + (int64_t)n * a.q_sn + (int64_t)(w.h * a.group + m - n * a.group) * a.q_sh;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (m < a.M) v = ld16(qp + dim_of<kFp8>(c, g));
-        q[t][c] = __builtin_bit_cast(bf16x8_t, v);
-      }
-    }
-    uint32_t all[kMT] = {};
-    const int c1 = min(s1, w.Tc);  // cached steps end here
-    int s = s0 + wave;
-    while (s < c1) {
-      // The page ids of this wave's next kWindow steps, one subtile a lane.
-      const int n_here = min(kWindow, (c1 - s + kW - 1) / kW);
-      int pid = -1, poff = 0;
-      {
-        const int tok = kStep * (s + kW * (lane >> 1)) + 16 * (lane & 1);
-        if ((lane >> 1) < n_here && tok < w.L) {
-          const int pi = tok / a.page_size;
-          poff = tok - pi * a.page_size;
-          pid = a.bt[(int64_t)w.b * a.bt_sb + pi];
-        }
-      }
-      // Two register tiles in turn: the next step's loads are issued before this step is computed.
-      Keys<kFp8> ka, kb;
-      load_cached<kFp8>(a, w, s, 0, pid, poff, lane, ka);
-      for (int i = 0; i < n_here; i += 2) {
-        if (i + 1 < n_here) load_cached<kFp8>(a, w, s + kW * (i + 1), i + 1, pid, poff, lane, kb);
-        __builtin_amdgcn_sched_barrier(0);
-        step<kFp8, kFp8, false, kMT>(ka, q, all, a.scale_log2, lane, st);
-        if (i + 1 < n_here) {
-          if (i + 2 < n_here) load_cached<kFp8>(a, w, s + kW * (i + 2), i + 2, pid, poff, lane, ka);
-          __builtin_amdgcn_sched_barrier(0);
-          step<kFp8, kFp8, false, kMT>(kb, q, all, a.scale_log2, lane, st);
-        }
-      }
-      s += kW * n_here;
-    }
-    if constexpr (kMode == kTree) {
-      for (; s < s1; s += kW) tree_step<kFp8, kMT>(a, w, s - w.Tc, q, lane, st);
-    }
-    if constexpr (kMode == kAppend) {
-      if (s < s1) {
-        Keys<true> kn;
-        append_keys(a, w, lane, w.mb == 0, kn);
-        step<true, true, false, kMT>(kn, q, all, a.scale_log2, lane, st);
-      }
-    }
-  }
-
-  // Merge the waves: 16 query rows at a time through LDS.
-  float* rec = nullptr;
-  if (live > 1) rec = a.ws + (((int64_t)w.b * a.hkv + w.h) * a.nchunk + chunk) * (int64_t)a.M * (kD + 2);
+// Q^T of the row's block of query rows as B operands.
+template <bool kFp8, int kMT>
+__device__ __forceinline__ void load_q(const Work& w, bf16x8_t (&q)[kMT][4]) {
+  const int lane = lane_now();
+  const TreeArgs& a = args_again();
+  const int r = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int t = 0; t < kMT; ++t) {
-    if ((w.mb * kMT + t) * 16 >= a.M) break;
-    if (t > 0) __syncthreads();
-    const float l = sum_xor32(sum_xor16(st.l[t]));
-    if (g == 0) {
-      s_m[wave][r] = st.m[t];
-      s_l[wave][r] = l;
-    }
+    const int m = (w.mb * kMT + t) * 16 + r;
+    const int n = node_of(a, m);
+    const uint16_t* qp = a.q + (int64_t)w.b * a.q_sb + (int64_t)n * a.q_sn + (int64_t)(w.h * a.group + m - n * a.group) * a.q_sh;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      *reinterpret_cast<f32x4_t*>(&s_o[wave][r][32 * g + 8 * i]) =
-          f32x4_t{st.o[t][0][i], st.o[t][1][i], st.o[t][2][i], st.o[t][3][i]};
-      *reinterpret_cast<f32x4_t*>(&s_o[wave][r][32 * g + 8 * i + 4]) =
-          f32x4_t{st.o[t][4][i], st.o[t][5][i], st.o[t][6][i], st.o[t][7][i]};
+    for (int c = 0; c < 4; ++c) {
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (m < a.M) v = ld16(qp + dim_of<kFp8>(c, g));
+      v = make_uint4(v.x ^ a.q_sign, v.y ^ a.q_sign, v.z ^ a.q_sign, v.w ^ a.q_sign);
+      q[t][c] = __builtin_bit_cast(bf16x8_t, v);
     }
-    __syncthreads();
-    if (threadIdx.x < 256) {
-      const int row = threadIdx.x >> 4, d0 = 8 * (threadIdx.x & 15);
-      const int m = (w.mb * kMT + t) * 16 + row;
-      if (m < a.M) {
+  }
+}
+
+// A wave's cached steps in registers: a step's K is loaded while the one before it has its softmax and V product, its V behind
+// that product.
+template <bool kFp8, int kMT>
+struct Stream {
+  static constexpr bool kOnce = kMT == 1;            // else other blocks of query rows may read the keys too
+  static constexpr bool kLayout = kFp8 || kMT == 1;  // swapped, or paired
+  KeyTile<kFp8> k;
+  ValueTile<kFp8> v;
+  int valid[2];
+
+  __device__ __forceinline__ void load(const TreeArgs& a, const Place& p, int lane) {
+    load_k<kOnce>(a, p, lane, k);
+    load_v<kFp8, kOnce>(a, p, lane, v);
+    valid[0] = p.valid[0];
+    valid[1] = p.valid[1];
+  }
+  // Computes the step and loads the next one.
+  __device__ __forceinline__ void turn(const TreeArgs& a, const Place& next, const Query<kFp8, kMT>& q, int lane, State<kMT>& st) {
+    const uint32_t all[kMT] = {};
+    f32x4_t s[kMT][2];
+    scores<kLayout, kMT>(k, q, s);
+    __builtin_amdgcn_sched_barrier(0);
+    load_k<kOnce>(a, next, lane, k);
+    __builtin_amdgcn_sched_barrier(0);
+    softmax<false, kMT>(valid, all, a.scale_log2, s, st);
+    values<kFp8, kMT>(v, valid, lane, s, st);
+    __builtin_amdgcn_sched_barrier(0);
+    load_v<kFp8, kOnce>(a, next, lane, v);
+    __builtin_amdgcn_sched_barrier(0);
+    valid[0] = next.valid[0];
+    valid[1] = next.valid[1];
+  }
+};
+
+// The append form's step: the new row.
+template <int kMT>
+__device__ __forceinline__ void append_step(const TreeArgs& a, const Work& w, const Query<true, kMT>& q, int lane, State<kMT>& st) {
+  const uint32_t all[kMT] = {};
+  f32x4_t s[kMT][2];
+  KeyTile<true> x;
+  ValueTile<true> y;
+  int one[2] = {0, 0};
+  append_keys(a, w, w.mb == 0, x, y, one[0]);
+  scores<false, kMT>(x, q, s);
+  softmax<false, kMT>(one, all, a.scale_log2, s, st);
+  values<true, kMT>(y, one, lane, s, st);
+}
+
+// A clear state, Q, and this wave's own steps s, s + kW, ... before T.
+template <bool kFp8, int kMode, int kMT, int kW>
+__device__ __forceinline__ void first_steps(const TreeArgs& a, const Work& w, int s, int T, int lane, Query<kFp8, kMT>& q,
+                                            State<kMT>& st) {
+  Query<false, kMT> raw;
+  load_q<kFp8, kMT>(w, raw.v);
+  if constexpr (kMode == kTree) {
+    clear(st);
+    for (; s < T; s += kW) tree_step<kFp8, kMT, kMT == 2>(w, s - w.Tc, raw, st);
+  }
+  prepare(raw.v, q);
+  if constexpr (kMode != kTree) {
+    __builtin_amdgcn_sched_barrier(0);
+    clear(st);  // (not before: Q's two parts and what they come from fill the registers)
+  }
+  if constexpr (kMode == kAppend) {
+    if (s < T) append_step<kMT>(a, w, q, lane, st);
+  }
+}
+
+// Query rows that the waves merge at once, 34 KB of them.
+template <int kW>
+struct MergeLds {
+  static constexpr int kRows = 64 / kW;
+  float o[kW][kRows][kMergeRow];
+  float m[kW][kRows], l[kW][kRows];
+};
+
+__device__ __forceinline__ uint16_t* out_row(int b, int h, int m) {
+  const TreeArgs& a = args_again();
+  const int n = node_of(a, m);
+  return a.out + (int64_t)b * a.o_sb + (int64_t)n * a.o_sn + (int64_t)(h * a.group + m - n * a.group) * a.o_sh;
+}
+
+__device__ __forceinline__ void store_out(uint16_t* op, const float (&acc)[8], float sum) {
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  st16(op, make_uint4(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv),
+                      pack_bf16x2(acc[4] * inv, acc[5] * inv), pack_bf16x2(acc[6] * inv, acc[7] * inv)));
+}
+
+// Merges the waves' states through LDS into the output (rec == nullptr) or a record of (o[128], m, l) floats a query row.
+template <int kMT, int kW>
+__device__ __forceinline__ void merge_waves(const Work& w, const State<kMT>& st, float* rec, int wave, MergeLds<kW>& s) {
+  const int lane = lane_now(), thread = 64 * wave + lane;
+  constexpr int kRows = MergeLds<kW>::kRows;
+  const int r = lane & 15, g = lane >> 4;
+  const int M = args_again().M;
+  const float scale = args_again().scale_log2;
+#pragma unroll
+  for (int t = 0; t < kMT; ++t) {
+    const float l = sum_xor32(sum_xor16(st.l[t]));
+#pragma unroll
+    for (int i0 = 0; i0 < 16; i0 += kRows) {
+      const int m0 = (w.mb * kMT + t) * 16 + i0;
+      if (m0 >= M) break;
+      __syncthreads();  // the buffer's last readers
+      if ((unsigned)(r - i0) < (unsigned)kRows) {
+        if (g == 0) {
+          s.m[wave][r - i0] = st.m[t] * scale;
+          s.l[wave][r - i0] = l;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float* o = &s.o[wave][r - i0][32 * g + 8 * i];
+          *reinterpret_cast<f32x4_t*>(o) = f32x4_t{st.o[t][0][i], st.o[t][1][i], st.o[t][2][i], st.o[t][3][i]};
+          *reinterpret_cast<f32x4_t*>(o + 4) = f32x4_t{st.o[t][4][i], st.o[t][5][i], st.o[t][6][i], st.o[t][7][i]};
+        }
+      }
+      __syncthreads();
+      const int row = thread >> 4, d0 = 8 * (thread & 15), m = m0 + row;
+      if (row < kRows && m < M) {
         float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < kW; ++i) top = fmaxf(top, s_m[i][row]);
+        for (int i = 0; i < kW; ++i) top = fmaxf(top, s.m[i][row]);
         const float base = top == -INFINITY ? 0.f : top;
         float acc[8] = {}, sum = 0.f;
 #pragma unroll
         for (int i = 0; i < kW; ++i) {
-          const float f = fast_exp2(s_m[i][row] - base);
-          sum += f * s_l[i][row];
+          const float f = fast_exp2(s.m[i][row] - base);
+          sum += f * s.l[i][row];
 #pragma unroll
-          for (int d = 0; d < 8; ++d) acc[d] += f * s_o[i][row][d0 + d];
+          for (int d = 0; d < 8; ++d) acc[d] += f * s.o[i][row][d0 + d];
         }
         if (rec == nullptr) {
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          const int n = m / a.group;
-          uint16_t* op = a.out + (int64_t)w.b * a.o_sb + (int64_t)n * a.o_sn +
-                         (int64_t)(w.h * a.group + m - n * a.group) * a.o_sh + d0;
-          st16(op, make_uint4(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv),
-                              pack_bf16x2(acc[4] * inv, acc[5] * inv), pack_bf16x2(acc[6] * inv, acc[7] * inv)));
+          store_out(out_row(w.b, w.h, m) + d0, acc, sum);
         } else {
-          float* o = rec + (int64_t)m * (kD + 2);
-          if (d0 == 0) {
-            o[kD] = top;
-            o[kD + 1] = sum;
-          }
-          // rows of 130 floats: 8-byte aligned
+          float* o = rec + (16 * t + i0 + row) * kRecord;
+          if (d0 == 0) *reinterpret_cast<float2*>(o + kD) = make_float2(top, sum);
 #pragma unroll
           for (int d = 0; d < 8; d += 2) *reinterpret_cast<float2*>(o + d0 + d) = make_float2(acc[d], acc[d + 1]);
         }
@@ -598,68 +923,280 @@ __global__ __launch_bounds__(64 * kW) void tree_kernel(const TreeArgs a) {
   }
 }
 
-// Merges the chunks' records of rows that have more than one: 16 lanes a query row, 8 dims a lane.
-template <int kMode>
-__global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
-  const int b = blockIdx.y;
-  const int mt = (a.M + 15) / 16;
-  const int h = blockIdx.x / mt, m = (blockIdx.x - h * mt) * 16 + (threadIdx.x >> 4), d0 = 8 * (threadIdx.x & 15);
-  int size, live;
-  split_of(a, steps_of(a, row_tokens(a, b, kMode), kMode), size, live);
-  if (live <= 1 || m >= a.M) return;
-  const int64_t rec = (int64_t)a.M * (kD + 2);
-  const float* base = a.ws + ((int64_t)b * a.hkv + h) * a.nchunk * rec + (int64_t)m * (kD + 2);
-  float top = -INFINITY;
-  for (int c = 0; c < live; ++c) top = fmaxf(top, base[c * rec + kD]);
-  const float ref = top == -INFINITY ? 0.f : top;
-  float acc[8] = {}, sum = 0.f;
-  for (int c = 0; c < live; ++c) {
-    const float* o = base + c * rec;
-    const float f = fast_exp2(o[kD] - ref);
-    sum += f * o[kD + 1];
-#pragma unroll
-    for (int d = 0; d < 8; d += 2) {
-      const float2 e = *reinterpret_cast<const float2*>(o + d0 + d);
-      acc[d] += f * e.x;
-      acc[d + 1] += f * e.y;
-    }
+__device__ __forceinline__ void zero_rows(int b, int h, int mb, int rows) {
+  const int row = threadIdx.x >> 4, d0 = 8 * (threadIdx.x & 15);
+  for (int i = row; i < rows; i += blockDim.x >> 4) {
+    const int m = mb * rows + i;
+    if (m < args_again().M) st16(out_row(b, h, m) + d0, make_uint4(0u, 0u, 0u, 0u));
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const int n = m / a.group;
-  uint16_t* op = a.out + (int64_t)b * a.o_sb + (int64_t)n * a.o_sn + (int64_t)(h * a.group + m - n * a.group) * a.o_sh + d0;
-  st16(op, make_uint4(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv),
-                      pack_bf16x2(acc[4] * inv, acc[5] * inv), pack_bf16x2(acc[6] * inv, acc[7] * inv)));
+}
+
+// The arguments with the pools at KV head h.
+__device__ __forceinline__ TreeArgs at_head(const TreeArgs& a, int h) {
+  TreeArgs b = a;
+  b.kc += (int64_t)h * a.sh;
+  b.vc += (int64_t)h * a.sh;
+  b.ks += (int64_t)h * a.ss_h;
+  b.vs += (int64_t)h * a.ss_h;
+  return b;
+}
+
+// A workgroup's KV head, block of query rows and unit (a row, or a chunk of one).  Workgroups go to the 8 XCDs in
+// turn.  With many units, unit i goes to XCD i % 8 with all its heads, which follow each other there: their exponent bytes
+// share lines, and their rows of a token-major pool share DRAM pages.  With few units the heads go to different XCDs.
+__device__ __forceinline__ void unit_of(const TreeArgs& a, int& h, int& mb, int& unit) {
+  if (a.xcd_units) {
+    const int y = blockIdx.x >> 3;
+    h = y % a.hkv;
+    mb = y / a.hkv;
+    unit = 8 * blockIdx.y + (blockIdx.x & 7);
+  } else {
+    h = blockIdx.x % a.hkv;
+    mb = blockIdx.x / a.hkv;
+    unit = blockIdx.y;
+  }
+}
+
+// Inclusive sum over the wave's lanes.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  auto add = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+  };
+  using std::integral_constant;
+  add(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});  // lanes 1, 2, 4, 8 below in the row of 16
+  add(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+  add(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+  add(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+  add(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // row 0's last lane to row 1, row 2's to row 3
+  add(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});  // row 1's last to rows 2 and 3
+  return x;
+}
+
+// What the chunked form's workgroup finds for its chunk.
+struct Chunk {
+  int row, L;           // row < 0: there is no such chunk
+  int index, count;     // which of the row's chunks
+};
+
+struct Joined {
+  int first, count;  // a row's chunks
+};
+
+// Rounds of kW steps that a row needs.
+template <int kW>
+__device__ __forceinline__ uint32_t rounds_of(int L, int mode) {
+  return (uint32_t)(steps_of(L, mode) + kW - 1) / kW;
+}
+
+// Chunk `at` of all rows' chunks laid end to end.  A chunk has at most `size` rounds, so many that about a.target chunks come
+// out, and a row has at least one.  64 rows at a time, one a lane; every wave does it.
+template <int kW>
+__device__ __forceinline__ Chunk chunk_at(const TreeArgs& a, uint32_t at, int mode) {
+  const int lane = lane_now(), batch = a.batch;
+  uint32_t total = 0;  // below 2^32: 1024 rows of 2^21
+  int L = -1;
+  for (int b = 0; b < batch; b += 64) {
+    L = b + lane < batch ? row_tokens(b + lane, mode) : -1;
+    total += (uint32_t)readlane((int)wave_scan(rounds_of<kW>(L, mode)), 63);
+  }
+  const uint32_t size = max(1u, (total + (uint32_t)a.target - 1) / (uint32_t)a.target);
+  uint32_t before = 0;
+  for (int b = 0; b < batch; b += 64) {
+    if (batch > 64) L = b + lane < batch ? row_tokens(b + lane, mode) : -1;
+    const uint32_t n = b + lane < batch ? max(1u, (rounds_of<kW>(L, mode) + size - 1) / size) : 0u;
+    const uint32_t upto = before + wave_scan(n);
+    const uint64_t has = __builtin_amdgcn_ballot_w64(at < upto);
+    if (has != 0) {
+      const int j = (int)__builtin_ctzll(has), count = readlane((int)n, j);
+      return {b + j, readlane(L, j), (int)at - (readlane((int)upto, j) - count), count};
+    }
+    before = (uint32_t)readlane((int)upto, 63);
+  }
+  return {-1, 0, 0, 0};
+}
+
+// One workgroup a (row, KV head, block of 16 kMT query rows), its kW waves taking the row's steps in turn; or (kChunked) one of
+// a chunk of a row's steps, which leaves a record for the join kernel unless it is the row's only one.
+template <bool kFp8, int kMode, int kMT, int kW, bool kChunked>
+__global__ __launch_bounds__(64 * kW, kMT == 1 && kFp8 && kMode != kTree ? 3 : 2) void tree_kernel(const TreeArgs args) {
+  __shared__ __align__(16) MergeLds<kW> lds;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Work w;
+  int unit;
+  unit_of(args, w.h, w.mb, unit);
+  if (unit >= args.units) return;
+  Window win;
+  int s0 = 0, s1;  // the chunk's steps
+  float* rec = nullptr;
+  if constexpr (kChunked) {
+    const Chunk c = chunk_at<kW>(args, (uint32_t)unit, kMode);
+    if (c.row < 0) return;
+    w.b = c.row;
+    w.L = c.L;
+    const int T = steps_of(w.L, kMode);
+    const int rounds = ((T + kW - 1) / kW + c.count - 1) / c.count;
+    s0 = min(T, c.index * rounds * kW);
+    s1 = min(T, s0 + rounds * kW);
+    if (c.count > 1)
+      rec = args_again().rec + (((int64_t)unit * args_again().mblocks + w.mb) * args_again().hkv + w.h) * (int64_t)(16 * kMT * kRecord);
+    if (c.index == 0 && w.h == 0 && w.mb == 0 && threadIdx.x == 0)
+      reinterpret_cast<Joined*>(args_again().ws)[w.b] = Joined{unit, c.count};
+    w.Tc = w.L > 0 ? (w.L + kStep - 1) / kStep : 0;
+    const int l = lane >> 1;
+    win = window_of<kFp8>(w.b, w.L, s0 + wave + kW * l, s0 + wave + kW * l < min(s1, w.Tc), lane);
+  } else {
+    w.b = unit;
+    // The first window's page ids do not wait for the row's length.
+    win = window_of<kFp8>(w.b, INT_MAX, wave + kW * (lane >> 1), true, lane);
+    w.L = __builtin_amdgcn_readfirstlane(row_tokens(w.b, kMode));
+    w.Tc = w.L > 0 ? (w.L + kStep - 1) / kStep : 0;
+    s1 = steps_of(w.L, kMode);
+  }
+  const TreeArgs a = at_head(args, w.h);
+  if (s1 == 0) {
+    zero_rows(w.b, w.h, w.mb, 16 * kMT);
+    return;
+  }
+  State<kMT> st;
+  if (s0 + wave >= s1) {
+    clear(st);
+  } else {
+    const int first = s0 + wave;
+    const int n = max(0, (min(s1, w.Tc) - first + kW - 1) / kW);  // this wave's cached steps: first, first + kW, ...
+    const int own = first + n * kW;  // and its first own step, taken ahead of them, while they are on their way
+    auto place = [&](int j) __attribute__((always_inline)) {
+      if ((j & (kWindow - 1)) == 0 && j > 0 && j < n) {
+        const int l = lane_now();
+        win = window_of<kFp8>(w.b, w.L, first + kW * (j + (l >> 1)), j + (l >> 1) < n, l);
+      }
+      return place_of<kFp8>(win, j & (kWindow - 1), j < n, w.L - kStep * (first + kW * j));
+    };
+    Stream<kFp8, kMT> x;
+    Query<kFp8, kMT> q;
+    constexpr bool kEarly = kFp8 || kMT == 1;  // else own steps and a tile do not fit the registers together
+    if constexpr (kEarly) x.load(a, place(0), lane);
+    first_steps<kFp8, kMode, kMT, kW>(a, w, own, s1, lane, q, st);
+    if constexpr (!kEarly) x.load(a, place(0), lane);
+    for (int i = 0; i < n; ++i) x.turn(a, place(i + 1), q, lane, st);
+  }
+  merge_waves<kMT, kW>(w, st, rec, wave, lds);
+}
+
+// Merges a shared row's records.  16 lanes a query row, 8 dims a lane; the thread groups that the query rows leave share the
+// records.
+template <int kMT>
+__global__ __launch_bounds__(256) void tree_join_kernel(const TreeArgs a) {
+  __shared__ float s_o[16][kD + 4];
+  __shared__ float s_m[16], s_l[16];
+  const int h = blockIdx.x % a.hkv, mb = blockIdx.x / a.hkv, b = blockIdx.y;
+  const int tile = 16 * blockIdx.z;  // of the block's query rows
+  const Joined d = reinterpret_cast<const Joined*>(a.ws)[b];
+  const int n = d.count;
+  if (n == 1) return;
+  const int rows = min(16, a.M - mb * 16 * kMT - tile);
+  if (rows <= 0) return;
+  const int64_t size = 16 * kMT * kRecord;
+  const int group = threadIdx.x >> 4, d0 = 8 * (threadIdx.x & 15);
+  const int side = rows > 8 ? 16 : rows > 4 ? 8 : rows > 2 ? 4 : rows;  // query rows at once
+  const int share = 16 / side, mine = group / side;
+  for (int i0 = 0; i0 < rows; i0 += side) {
+    const int i = i0 + group % side;
+    float acc[8] = {}, sum = 0.f, top = -INFINITY;
+    if (i < rows && mine < share) {
+#pragma unroll 4
+      for (int c = mine; c < n; c += share) {
+        const float* o = a.rec + (((int64_t)(d.first + c) * a.mblocks + mb) * a.hkv + h) * size + (int64_t)(tile + i) * kRecord;
+        const float2 ml = *reinterpret_cast<const float2*>(o + kD);
+        float e[8];
+#pragma unroll
+        for (int k = 0; k < 8; k += 2) {
+          const float2 v = *reinterpret_cast<const float2*>(o + d0 + k);
+          e[k] = v.x;
+          e[k + 1] = v.y;
+        }
+        const float m = fmaxf(top, ml.x), base = m == -INFINITY ? 0.f : m;
+        const float f0 = fast_exp2(top - base), f1 = fast_exp2(ml.x - base);
+        top = m;
+        sum = sum * f0 + ml.y * f1;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] = acc[k] * f0 + e[k] * f1;
+      }
+    }
+    if (share > 1) {  // the same for every thread
+      __syncthreads();
+      if (d0 == 0) {
+        s_m[group] = top;
+        s_l[group] = sum;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s_o[group][d0 + k] = acc[k];
+      __syncthreads();
+      if (mine == 0) {
+        float all = -INFINITY;
+        for (int c = 0; c < share; ++c) all = fmaxf(all, s_m[c * side + group]);
+        const float base = all == -INFINITY ? 0.f : all;
+        sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] = 0.f;
+        for (int c = 0; c < share; ++c) {
+          const float f = fast_exp2(s_m[c * side + group] - base);
+          sum += f * s_l[c * side + group];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) acc[k] += f * s_o[c * side + group][d0 + k];
+        }
+      }
+    }
+    if (mine == 0 && i < rows) store_out(out_row(b, h, mb * 16 * kMT + tile + i) + d0, acc, sum);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------- host side
 
 constexpr int kWaves = 4;
 
-int tiles_per_wave(int M) { return M <= 16 ? 1 : M <= 32 ? 2 : 4; }
+int tiles_per_wave(int M) { return M <= 16 ? 1 : 2; }
 
-// Chunks a row's steps are split into at most, from the shape alone (the lengths are on the device).
-int chunks_of(int batch, int hkv, int mblocks, int64_t capacity, int nodes) {
-  const int64_t steps = (capacity + kStep - 1) / kStep + (nodes + kStep - 1) / kStep;
-  const int64_t groups = (int64_t)batch * hkv * mblocks;
-  const int64_t want = std::max<int64_t>(1, (int64_t)num_cus() * 4 / std::max<int64_t>(groups, 1));
-  const int64_t most = std::max<int64_t>(1, steps / (2 * kWaves));
-  return (int)std::min<int64_t>(std::min(want, most), 256);
+
+struct Plan {
+  int mblocks, units, target;  // target == 0: whole rows
+  size_t rows, bytes;
+};
+
+// From the shape alone: the lengths are on the device.
+Plan plan_of(int batch, int nodes, int hq, int hkv, int64_t capacity) {
+  Plan p = {};
+  const int M = nodes * (hq / hkv), tiles = tiles_per_wave(M);
+  p.mblocks = (M + 16 * tiles - 1) / (16 * tiles);
+  p.units = batch;
+  // Whole rows take one launch, but the longest row's steps follow each other on one compute unit; chunks cost the join (3.7 us)
+  // and records.  8 heads x 1 row are equal at 512 tokens (8.5 us, 9.7 as chunks; at 1000: 11.9, 9.8), 256 workgroups at about
+  // 1000 (16.0, 19.3; with up to 1700 tokens and 13 nodes: 26.8, 22.5), 512 above 1500 (22.8, 23.4).  Rows that are more than
+  // the chip holds at once balance by themselves.
+  const int64_t groups = (int64_t)batch * hkv * p.mblocks;
+  if (batch > 1024 || capacity * num_cus() <= 512 * (num_cus() + groups)) return p;
+  const int slots = 2 * num_cus() / (hkv * p.mblocks);  // (one or three a compute unit: within 3 %, either way)
+  p.target = std::max({1, slots - batch / 2, slots / 2});
+  p.units = p.target + batch;
+  p.rows = ((size_t)batch * sizeof(Joined) + 15) & ~(size_t)15;
+  p.bytes = p.rows + (size_t)p.units * p.mblocks * hkv * 16 * tiles * kRecord * sizeof(float);
+  return p;
 }
 
-template <bool kFp8, int kMode>
-int launch(const TreeArgs& a, int batch, const char* who, hipStream_t stream) {
-  const dim3 grid((unsigned)(a.hkv * a.mblocks * a.nchunk), (unsigned)batch);
-  const int tiles = tiles_per_wave(a.M);
-  if constexpr (kMode == kTree) {
-    if (tiles == 2) hipLaunchKernelGGL((tree_kernel<kFp8, kMode, 2, kWaves>), grid, dim3(64 * kWaves), 0, stream, a);
-    if (tiles == 4) hipLaunchKernelGGL((tree_kernel<kFp8, kMode, 4, kWaves>), grid, dim3(64 * kWaves), 0, stream, a);
-  }
-  if (tiles == 1) hipLaunchKernelGGL((tree_kernel<kFp8, kMode, 1, kWaves>), grid, dim3(64 * kWaves), 0, stream, a);
-  hipError_t e = hipGetLastError();
-  if (e == hipSuccess && a.nchunk > 1) {
-    hipLaunchKernelGGL((tree_merge_kernel<kMode>), dim3((unsigned)(a.hkv * ((a.M + 15) / 16)), (unsigned)batch), dim3(256), 0,
-                       stream, a);
+template <bool kFp8, int kMode, int kMT>
+int launch(const TreeArgs& a, const char* who, hipStream_t stream) {
+  hipError_t e;
+  const unsigned heads = (unsigned)(a.hkv * a.mblocks), units = (unsigned)a.units;
+  const dim3 grid = a.xcd_units ? dim3(8 * heads, (units + 7) / 8) : dim3(heads, units);
+  if (a.target == 0) {
+    hipLaunchKernelGGL((tree_kernel<kFp8, kMode, kMT, kWaves, false>), grid, dim3(64 * kWaves), 0, stream, a);
     e = hipGetLastError();
+  } else {
+    hipLaunchKernelGGL((tree_kernel<kFp8, kMode, kMT, kWaves, true>), grid, dim3(64 * kWaves), 0, stream, a);
+    e = hipGetLastError();
+    if (e == hipSuccess) {
+      hipLaunchKernelGGL((tree_join_kernel<kMT>), dim3(heads, (unsigned)a.batch, kMT), dim3(256), 0, stream, a);
+      e = hipGetLastError();
+    }
   }
   return e == hipSuccess ? Q3A_OK : fail(Q3A_ELAUNCH, "%s: %s", who, hipGetErrorString(e));
 }
@@ -672,16 +1209,9 @@ int check_shape(const char* who, int batch, int nodes, int hq, int hkv, int head
     return fail(Q3A_EINVAL, "%s: %d query heads over %d KV heads (a multiple, at most 16 to one; at most 64 KV heads)", who, hq,
                 hkv);
   if (page_size < 16 || page_size % 16 != 0) return fail(Q3A_EINVAL, "%s: page_size %d must be a multiple of 16", who, page_size);
-  if (max_pages < 0 || (int64_t)max_pages * page_size > (1 << 30))
-    return fail(Q3A_EINVAL, "%s: table of %d pages of %d tokens (at most 2^30 tokens a row)", who, max_pages, page_size);
+  if (max_pages < 0 || (int64_t)max_pages * page_size > (1 << 28))
+    return fail(Q3A_EINVAL, "%s: table of %d pages of %d tokens (at most 2^28 tokens a row)", who, max_pages, page_size);
   return Q3A_OK;
-}
-
-size_t workspace_of(int batch, int nodes, int hq, int hkv, int64_t capacity) {
-  const int M = nodes * (hq / hkv);
-  const int per = 16 * tiles_per_wave(M);
-  const int n = chunks_of(batch, hkv, (M + per - 1) / per, capacity, nodes);
-  return n > 1 ? (size_t)batch * hkv * n * M * (kD + 2) * sizeof(float) : 0;
 }
 
 bool misaligned(const void* p, int64_t a, int64_t b, int64_t c) { return ((uintptr_t)p & 15) != 0 || ((a | b | c) & 7) != 0; }
@@ -706,25 +1236,33 @@ int run(const char* who, TreeArgs a, int mode, bool fp8, int batch, int hq, size
   }
   a.group = hq / a.hkv;
   a.M = a.nodes * a.group;
-  const int per = 16 * tiles_per_wave(a.M);
-  a.mblocks = (a.M + per - 1) / per;
-  const int64_t capacity = (int64_t)a.max_pages * a.page_size;
-  a.nchunk = chunks_of(batch, a.hkv, a.mblocks, capacity, a.nodes);
-  a.min_steps = kWaves;
-  const size_t need = workspace_of(batch, a.nodes, hq, a.hkv, capacity);
-  if (need > 0 && (a.ws == nullptr || workspace_bytes < need || ((uintptr_t)a.ws & 15) != 0))
-    return fail(Q3A_ESPACE, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", who, workspace_bytes, need);
+  if (((int64_t)a.num_pages * kv_page + (int64_t)a.page_size * kv_tok) * elem >= (int64_t)1 << 36 ||
+      (fp8 && (int64_t)a.num_pages * a.ss_p >= (int64_t)1 << 32))
+    return fail(Q3A_EINVAL, "%s: a cache of 64 GiB or more, or scales of 4 GiB", who);
+  const Plan p = plan_of(batch, a.nodes, hq, a.hkv, (int64_t)a.max_pages * a.page_size);
+  if (p.bytes > 0 && (a.ws == nullptr || workspace_bytes < p.bytes || ((uintptr_t)a.ws & 15) != 0))
+    return fail(Q3A_ESPACE, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", who, workspace_bytes, p.bytes);
+  a.batch = batch;
+  a.per_group = ((1u << 20) + a.group - 1) / a.group;
+  a.mblocks = p.mblocks;
+  a.units = p.units;
+  a.target = p.target;
+  a.xcd_units = p.units >= 32;
+  a.rec = p.target > 0 ? reinterpret_cast<float*>(static_cast<char*>(a.ws) + p.rows) : nullptr;
   a.sp = kv_page * elem;
   a.st = (int)(kv_tok * elem);
   a.sh = kv_head * elem;
-  a.scale_log2 = softmax_scale * kLog2e;
+  // The kernels take a positive scale (maxima are of the unscaled scores): Q's sign is turned for a negative one, and 0, with
+  // which masked scores of -inf would be NaN, becomes the smallest there is.
+  a.q_sign = softmax_scale < 0.f ? 0x80008000u : 0u;
+  a.scale_log2 = softmax_scale == 0.f ? FLT_MIN : fabsf(softmax_scale) * kLog2e;
   const hipStream_t s = (hipStream_t)stream;
-  if (fp8) {
-    if (mode == kNoKeys) return launch<true, kNoKeys>(a, batch, who, s);
-    if (mode == kAppend) return launch<true, kAppend>(a, batch, who, s);
-    return launch<true, kTree>(a, batch, who, s);
+  if (mode == kNoKeys) return launch<true, kNoKeys, 1>(a, who, s);
+  if (mode == kAppend) return launch<true, kAppend, 1>(a, who, s);
+  switch (tiles_per_wave(a.M)) {
+    case 1: return fp8 ? launch<true, kTree, 1>(a, who, s) : launch<false, kTree, 1>(a, who, s);
+    default: return fp8 ? launch<true, kTree, 2>(a, who, s) : launch<false, kTree, 2>(a, who, s);
   }
-  return launch<false, kTree>(a, batch, who, s);
 }
 
 }  // namespace
@@ -737,7 +1275,7 @@ extern "C" size_t q3a_paged_decode_tree_workspace_bytes(int batch, int num_nodes
   if (check_shape("q3a_paged_decode_tree_workspace_bytes", batch, num_nodes, num_q_heads, num_kv_heads, head_dim,
                   max_pages_per_seq, page_size) != Q3A_OK || batch == 0)
     return 0;
-  return workspace_of(batch, num_nodes, num_q_heads, num_kv_heads, (int64_t)max_pages_per_seq * page_size);
+  return plan_of(batch, num_nodes, num_q_heads, num_kv_heads, (int64_t)max_pages_per_seq * page_size).bytes;
 }
 
 extern "C" int q3a_paged_decode_fp8(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k_cache,
@@ -772,7 +1310,7 @@ extern "C" int q3a_paged_decode_fp8(const void* q, int64_t q_stride_b, int64_t q
   a.out = (uint16_t*)out;
   a.o_sb = o_stride_b;
   a.o_sh = o_stride_h;
-  a.ws = (float*)workspace;
+  a.ws = workspace;
   a.nodes = 1;
   a.hkv = num_kv_heads;
   return run(who, a, kNoKeys, true, batch, num_q_heads, workspace_bytes, kv_stride_page, kv_stride_tok, kv_stride_head,
@@ -817,7 +1355,7 @@ extern "C" int q3a_paged_decode_fp8_append(
   a.out = (uint16_t*)out;
   a.o_sb = o_stride_b;
   a.o_sh = o_stride_h;
-  a.ws = (float*)workspace;
+  a.ws = workspace;
   a.nodes = 1;
   a.hkv = num_kv_heads;
   return run(who, a, kAppend, true, batch, num_q_heads, workspace_bytes, kv_stride_page, kv_stride_tok, kv_stride_head,
@@ -881,7 +1419,7 @@ extern "C" int q3a_paged_decode_tree(
   a.o_sb = o_stride_b;
   a.o_sn = o_stride_n;
   a.o_sh = o_stride_h;
-  a.ws = (float*)workspace;
+  a.ws = workspace;
   a.nodes = num_nodes;
   a.hkv = num_kv_heads;
   return run(who, a, kTree, fp8, batch, num_q_heads, workspace_bytes, kv_stride_page, kv_stride_tok, kv_stride_head,
