@@ -72,6 +72,7 @@ struct TreeArgs {
   uint32_t per_group;  // m / group = m * per_group >> 20 for m < 4096
   int mblocks;
   int units, target;  // rows, or chunks at most and as many as there should be
+  float per_target;     // 1 / target, a little more
   int xcd_units;
   int order;  // whole rows start in the order of their lengths
   float scale_log2;   // positive
@@ -144,21 +145,24 @@ struct Window {
   int valid;         // keys that are seen: 0 past the row's end, and where the table has no page
 };
 
-// Lane l's subtile: half l & 1 of step `step` of row b with L cached tokens; `on`: there is such a step.
-template <bool kFp8>
-__device__ __forceinline__ Window window_of(int b, int L, int step, bool on, int lane) {
+// Lane l's subtile is half l & 1 of step `step` of row b.  Its table entry (-1 past the table), and, once that has come, its
+// place, given the row's L cached tokens; `on`: there is such a step.
+__device__ __forceinline__ int page_at(int b, int step, int lane) {
   const TreeArgs& a = args_again();
-  const int tok = kStep * step + 16 * (lane & 1);
+  const int pi = (int)((uint32_t)(kStep * step + 16 * (lane & 1)) / (uint32_t)a.page_size);
+  if (a.max_pages == 0) return -1;
+  const int page = a.bt[(int64_t)b * a.bt_sb + min(pi, a.max_pages - 1)];
+  return pi < a.max_pages ? page : -1;
+}
+template <bool kFp8>
+__device__ __forceinline__ Window window_of(int page, int L, int step, bool on, int lane) {
+  const TreeArgs& a = args_again();
+  const int tok = kStep * step + 16 * (lane & 1), off = (int)((uint32_t)tok % (uint32_t)a.page_size);
   Window w = {0u, 0u, 0};
-  const int pi = (int)((uint32_t)tok / (uint32_t)a.page_size);
-  if (on && pi < a.max_pages) {
-    const int off = tok - pi * a.page_size;
-    const int page = a.bt[(int64_t)b * a.bt_sb + pi];
-    if ((unsigned)page < (unsigned)a.num_pages) {
-      w.at = (uint32_t)(((int64_t)page * a.sp + (int64_t)off * a.st) >> 4);
-      if constexpr (kFp8) w.sat = (uint32_t)(page * a.ss_p + off);
-      w.valid = max(0, min(16, L - tok));
-    }
+  if (on && (unsigned)page < (unsigned)a.num_pages) {
+    w.at = (uint32_t)(((int64_t)page * a.sp + (int64_t)off * a.st) >> 4);
+    if constexpr (kFp8) w.sat = (uint32_t)(page * a.ss_p + off);
+    w.valid = max(0, min(16, L - tok));
   }
   return w;
 }
@@ -661,14 +665,15 @@ __device__ __forceinline__ void tree_step(const Work& w, int ts, const Query<fal
     load_values();
   }
   softmax<true, kMT>(any, seen, a.scale_log2, sc, st);
-  bool odd = false;
+  uint32_t top = 0;
 #pragma unroll
   for (int u = 0; u < 2; ++u)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint4 e = y.v[u][i];
-      odd = odd || not_finite_pair(e.x) || not_finite_pair(e.y) || not_finite_pair(e.z) || not_finite_pair(e.w);
+      top = pk_max_u16(top, pk_max_u16(pk_max_u16(e.x & 0x7fff7fffu, e.y & 0x7fff7fffu), pk_max_u16(e.z & 0x7fff7fffu, e.w & 0x7fff7fffu)));
     }
+  const bool odd = halves_max(top) >= 0x7f80u;
   const bool any_odd = __builtin_amdgcn_ballot_w64(odd) != 0;
   if (any_odd) {
 #pragma unroll
@@ -759,7 +764,7 @@ __device__ __forceinline__ void clear(State<kMT>& st) {
   }
 }
 
-// Q^T of the row's block of query rows as B operands.
+// Q^T of the row's block of query rows as B operands; columns past the last query row have the last one's again.
 template <bool kFp8, int kMT>
 __device__ __forceinline__ void load_q(const Work& w, bf16x8_t (&q)[kMT][4]) {
   const int lane = lane_now();
@@ -767,16 +772,11 @@ __device__ __forceinline__ void load_q(const Work& w, bf16x8_t (&q)[kMT][4]) {
   const int r = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int t = 0; t < kMT; ++t) {
-    const int m = (w.mb * kMT + t) * 16 + r;
+    const int m = min((w.mb * kMT + t) * 16 + r, a.M - 1);
     const int n = node_of(a, m);
     const uint16_t* qp = a.q + (int64_t)w.b * a.q_sb + (int64_t)n * a.q_sn + (int64_t)(w.h * a.group + m - n * a.group) * a.q_sh;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (m < a.M) v = ld16(qp + dim_of<kFp8>(c, g));
-      v = make_uint4(v.x ^ a.q_sign, v.y ^ a.q_sign, v.z ^ a.q_sign, v.w ^ a.q_sign);
-      q[t][c] = __builtin_bit_cast(bf16x8_t, v);
-    }
+    for (int c = 0; c < 4; ++c) q[t][c] = __builtin_bit_cast(bf16x8_t, ld16(qp + dim_of<kFp8>(c, g)));
   }
 }
 
@@ -828,15 +828,21 @@ __device__ __forceinline__ void append_step(const TreeArgs& a, const Work& w, co
   values<true, kMT>(y, one, lane, s, st);
 }
 
-// A clear state, Q, and this wave's own steps s, s + kW, ... before T.
+// Q as the products take it (raw: as it was loaded), a clear state, and this wave's own steps s, s + kW, ... before T.
 template <bool kFp8, int kMode, int kMT, int kW>
-__device__ __forceinline__ void first_steps(const TreeArgs& a, const Work& w, int s, int T, int lane, Query<kFp8, kMT>& q,
-                                            State<kMT>& st) {
-  Query<false, kMT> raw;
-  load_q<kFp8, kMT>(w, raw.v);
+__device__ __forceinline__ void first_steps(const TreeArgs& a, const Work& w, int s, int T, int lane, Query<false, kMT>& raw,
+                                            Query<kFp8, kMT>& q, State<kMT>& st) {
+  const uint32_t sign = args_again().q_sign;
+#pragma unroll
+  for (int t = 0; t < kMT; ++t)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint4 v = __builtin_bit_cast(uint4, raw.v[t][c]);
+      raw.v[t][c] = __builtin_bit_cast(bf16x8_t, make_uint4(v.x ^ sign, v.y ^ sign, v.z ^ sign, v.w ^ sign));
+    }
   if constexpr (kMode == kTree) {
     clear(st);
-    for (; s < T; s += kW) tree_step<kFp8, kMT, kMT == 2>(w, s - w.Tc, raw, st);
+    for (; s < T; s += kW) tree_step<kFp8, kMT, kMT == 2 && !kFp8>(w, s - w.Tc, raw, st);
   }
   prepare(raw.v, q);
   if constexpr (kMode != kTree) {
@@ -983,28 +989,37 @@ struct Joined {
   int first, count;  // a row's chunks
 };
 
-// Rounds of kW steps that a row needs.
+// Rounds of kW steps that a row's work makes.  (Counting the own ones threefold, as long as they take, made the chunks longer and
+// lost 5 %.)
 template <int kW>
-__device__ __forceinline__ uint32_t rounds_of(int L, int mode) {
-  return (uint32_t)(steps_of(L, mode) + kW - 1) / kW;
+__device__ __forceinline__ uint32_t rounds_of(const TreeArgs& a, int L, int mode) {
+  if (L < 0) return 0;
+  const uint32_t cached = (uint32_t)(L + kStep * kW - 1) / (kStep * kW);
+  return cached + (mode == kTree ? (a.nodes + kStep * kW - 1) / (kStep * kW) : mode == kAppend ? 1 : 0);
 }
 
-// Chunk `at` of all rows' chunks laid end to end.  A chunk has at most `size` rounds, so many that about a.target chunks come
-// out, and a row has at least one.  64 rows at a time, one a lane; every wave does it.
+// Chunk `at` of all rows' chunks laid end to end.  64 rows at a time, one a lane; every wave does it.  A chunk has up to `size`
+// rounds: total / target, rounded up, so that a row's 1 + floor(rounds / size) come to target + batch at most.
 template <int kW>
 __device__ __forceinline__ Chunk chunk_at(const TreeArgs& a, uint32_t at, int mode) {
-  const int lane = lane_now(), batch = a.batch;
+  const int lane = lane_now(), batch = a.batch, cap = a.max_pages * a.page_size;
+  auto tokens = [&](int b) {  // row_tokens
+    const int n = b < batch ? a.seqlens[b] : -1;
+    return mode == kAppend ? (n < cap ? n : -1) : min(n, cap);
+  };
   uint32_t total = 0;  // below 2^32: 1024 rows of 2^21
   int L = -1;
   for (int b = 0; b < batch; b += 64) {
-    L = b + lane < batch ? row_tokens(b + lane, mode) : -1;
-    total += (uint32_t)readlane((int)wave_scan(rounds_of<kW>(L, mode)), 63);
+    L = tokens(b + lane);
+    total += (uint32_t)readlane((int)wave_scan(rounds_of<kW>(a, L, mode)), 63);
   }
-  const uint32_t size = max(1u, (total + (uint32_t)a.target - 1) / (uint32_t)a.target);
+  // (The reciprocals are a little large and a little small: neither count may come out too high.)
+  const float size = fmaxf(1.f, floorf((float)total * a.per_target + 0.999f));
+  const float per_size = __builtin_amdgcn_rcpf(size) * 0.999999f;
   uint32_t before = 0;
   for (int b = 0; b < batch; b += 64) {
-    if (batch > 64) L = b + lane < batch ? row_tokens(b + lane, mode) : -1;
-    const uint32_t n = b + lane < batch ? max(1u, (rounds_of<kW>(L, mode) + size - 1) / size) : 0u;
+    if (batch > 64) L = tokens(b + lane);
+    const uint32_t n = b + lane < batch ? 1 + (uint32_t)((float)rounds_of<kW>(a, L, mode) * per_size) : 0u;
     const uint32_t upto = before + wave_scan(n);
     const uint64_t has = __builtin_amdgcn_ballot_w64(at < upto);
     if (has != 0) {
@@ -1016,17 +1031,17 @@ __device__ __forceinline__ Chunk chunk_at(const TreeArgs& a, uint32_t at, int mo
   return {-1, 0, 0, 0};
 }
 
-// The k-th of up to 64 kW rows by their lengths, longest first.  Workgroups start in the order of their numbers, and the longest
-// rows should start first: 250 rows of 200 to 1200 tokens took 59.4 us as they came, 52.3 so, 256 rows of 8 nodes 122.3 and
-// 115.8; 256 equal ones 109.8 and 111.7.  (With four times the rows a wave, 576 rows of 100 to 1700 gained 2 % and 576 equal
-// ones lost 5 %: more rows than this are taken as they come.)  Rows are told apart by eighths of octaves below the table's
-// length, 64 of them, and stand in their own order within one: each wave counts a part of them in LDS, and the wave whose count
-// the k-th falls into finds it.
+// The k-th of the batch's last rows, from row0 on (up to 64 kW), by their lengths, longest first.  Workgroups start in the order
+// of their numbers, and the last to start should be short: 250 rows of 200 to 1200 tokens took 59.4 us as they came, 51.4 so,
+// 256 rows of 8 nodes 122.3 and 115.4 (equal ones 109.8 and 111.7), 576 rows of 100 to 1700 tokens 105.4 and 103.9 (all 576 in
+// order, with four times the rows a wave: 102, but equal rows lost 5 %).  Rows are told apart by eighths of octaves below the
+// table's length, 64 of them, and stand in their own order within one: each wave counts a part of them in LDS, and the wave
+// whose count the k-th falls into finds it.
 template <int kW>
-__device__ __forceinline__ int kth_longest(const TreeArgs& a, int k, int wave) {
+__device__ __forceinline__ int kth_longest(const TreeArgs& a, int row0, int k, int wave) {
   __shared__ int s_count[kW][64];
   __shared__ int s_row;
-  const int lane = lane_now(), b = 64 * wave + lane;
+  const int lane = lane_now(), b = row0 + 64 * wave + lane;
   const int cap = a.max_pages * a.page_size;
   const int L = a.seqlens[min(b, a.batch - 1)];
   s_count[wave][lane] = 0;
@@ -1065,6 +1080,7 @@ __global__ __launch_bounds__(64 * kW, kMT == 1 && kFp8 && kMode != kTree ? 3 : 2
   unit_of(args, w.h, w.mb, unit);
   if (unit >= args.units) return;
   Window win;
+  Query<false, kMT> raw;
   int s0 = 0, s1;  // the chunk's steps
   float* rec = nullptr;
   if constexpr (kChunked) {
@@ -1073,27 +1089,32 @@ __global__ __launch_bounds__(64 * kW, kMT == 1 && kFp8 && kMode != kTree ? 3 : 2
     w.b = c.row;
     w.L = c.L;
     const int T = steps_of(w.L, kMode);
-    const int rounds = ((T + kW - 1) / kW + c.count - 1) / c.count;
-    s0 = min(T, c.index * rounds * kW);
-    s1 = min(T, s0 + rounds * kW);
+    w.Tc = w.L > 0 ? (w.L + kStep - 1) / kStep : 0;
+    const int steps = (int)((rounds_of<kW>(args, w.L, kMode) + c.count - 1) / c.count) * kW;
+    s0 = min(w.Tc, c.index * steps);
+    s1 = c.index == c.count - 1 ? T : min(w.Tc, s0 + steps);  // the last one has the own steps
     if (c.count > 1)
       rec = args_again().rec + (((int64_t)unit * args_again().mblocks + w.mb) * args_again().hkv + w.h) * (int64_t)(16 * kMT * kRecord);
     if (c.index == 0 && w.h == 0 && w.mb == 0 && threadIdx.x == 0)
-      reinterpret_cast<Joined*>(args_again().ws)[w.b] = Joined{unit, c.count};
-    w.Tc = w.L > 0 ? (w.L + kStep - 1) / kStep : 0;
-    const int l = lane >> 1;
-    win = window_of<kFp8>(w.b, w.L, s0 + wave + kW * l, s0 + wave + kW * l < min(s1, w.Tc), lane);
+      reinterpret_cast<Joined*>(args_again().ws)[w.b] = Joined{unit - c.index, c.count};
+    const int s = s0 + wave + kW * (lane >> 1);
+    const int page = page_at(w.b, s, lane);
+    load_q<kFp8, kMT>(w, raw.v);
+    win = window_of<kFp8>(page, w.L, s, s < min(s1, w.Tc), lane);
   } else {
     w.b = unit;
-    if (args.order) w.b = kth_longest<kW>(args, unit, wave);
+    const int row0 = max(0, args.batch - 64 * kW);
+    if (args.order && unit >= row0) w.b = kth_longest<kW>(args, row0, unit - row0, wave);
     // The first window's page ids do not wait for the row's length.
-    win = window_of<kFp8>(w.b, INT_MAX, wave + kW * (lane >> 1), true, lane);
+    const int s = wave + kW * (lane >> 1), page = page_at(w.b, s, lane);
+    load_q<kFp8, kMT>(w, raw.v);
+    win = window_of<kFp8>(page, INT_MAX, s, true, lane);
     w.L = __builtin_amdgcn_readfirstlane(row_tokens(w.b, kMode));
     w.Tc = w.L > 0 ? (w.L + kStep - 1) / kStep : 0;
     s1 = steps_of(w.L, kMode);
   }
   const TreeArgs a = at_head(args, w.h);
-  if (s1 == 0) {
+  if (s1 == 0 && rec == nullptr) {
     zero_rows(w.b, w.h, w.mb, 16 * kMT);
     return;
   }
@@ -1106,8 +1127,8 @@ __global__ __launch_bounds__(64 * kW, kMT == 1 && kFp8 && kMode != kTree ? 3 : 2
     const int own = first + n * kW;  // and its first own step, taken ahead of them, while they are on their way
     auto place = [&](int j) __attribute__((always_inline)) {
       if ((j & (kWindow - 1)) == 0 && j > 0 && j < n) {
-        const int l = lane_now();
-        win = window_of<kFp8>(w.b, w.L, first + kW * (j + (l >> 1)), j + (l >> 1) < n, l);
+        const int l = lane_now(), s = first + kW * (j + (l >> 1));
+        win = window_of<kFp8>(page_at(w.b, s, l), w.L, s, j + (l >> 1) < n, l);
       }
       return place_of<kFp8>(win, j & (kWindow - 1), j < n, w.L - kStep * (first + kW * j));
     };
@@ -1115,7 +1136,7 @@ __global__ __launch_bounds__(64 * kW, kMT == 1 && kFp8 && kMode != kTree ? 3 : 2
     Query<kFp8, kMT> q;
     constexpr bool kEarly = kFp8 || kMT == 1;  // else own steps and a tile do not fit the registers together
     if constexpr (kEarly) x.load(a, place(0), lane);
-    first_steps<kFp8, kMode, kMT, kW>(a, w, own, s1, lane, q, st);
+    first_steps<kFp8, kMode, kMT, kW>(a, w, own, s1, lane, raw, q, st);
     if constexpr (!kEarly) x.load(a, place(0), lane);
     for (int i = 0; i < n; ++i) x.turn(a, place(i + 1), q, lane, st);
   }
@@ -1287,8 +1308,9 @@ int run(const char* who, TreeArgs a, int mode, bool fp8, int batch, int hq, size
   a.mblocks = p.mblocks;
   a.units = p.units;
   a.target = p.target;
+  a.per_target = p.target > 0 ? 1.000001f / (float)p.target : 0.f;
   a.xcd_units = p.units >= 32;
-  a.order = p.target == 0 && batch <= 64 * kWaves && (int64_t)batch * a.hkv * p.mblocks > num_cus();
+  a.order = p.target == 0 && (int64_t)batch * a.hkv * p.mblocks > num_cus();
   a.rec = p.target > 0 ? reinterpret_cast<float*>(static_cast<char*>(a.ws) + p.rows) : nullptr;
   a.sp = kv_page * elem;
   a.st = (int)(kv_tok * elem);
