@@ -6,6 +6,7 @@
 // custom op with its checks in Python and the C call through ctypes) a read of 77 tokens took 23.8 us on the host, of which
 // the launch is 2.6.
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/library.h>
@@ -21,6 +22,11 @@ using std::optional;
 
 void* stream_of(const c10::Device& d) {
   return (void*)c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(d.index()).stream();
+}
+
+// A contiguous tensor on d.  (Past the dispatcher: 0.7 us of a call's 10 a tensor.)
+Tensor empty_on(const c10::Device& d, at::IntArrayRef shape, c10::ScalarType t) {
+  return at::detail::empty_cuda(shape, t, d, std::nullopt);
 }
 
 void done(int rc, const char* what) { TORCH_CHECK(rc == Q3A_OK, what, " failed (", rc, "): ", q3a_last_error()); }
@@ -96,8 +102,8 @@ std::tuple<Tensor, Tensor> paged_read_fp8(const Tensor& kc, const Tensor& vc, co
   check_slots(who, d, slots);
   const int64_t T = slots.size(0);
   const c10::DeviceGuard guard(d);
-  const auto opts = kc.options().dtype(at::kBFloat16);
-  Tensor k = at::empty({T, kc.size(2), kc.size(3)}, opts), v = at::empty({T, kc.size(2), kc.size(3)}, opts);
+  const int64_t shape[3] = {T, kc.size(2), kc.size(3)};
+  Tensor k = empty_on(d, shape, at::kBFloat16), v = empty_on(d, shape, at::kBFloat16);
   if (T == 0) return {k, v};
   done(q3a_paged_read_fp8(kc.data_ptr(), vc.data_ptr(), kc.stride(0), kc.stride(1), kc.stride(2), ks.data_ptr(), vs.data_ptr(),
                           ks.stride(0), ks.stride(1), (int)kc.size(0), (int)kc.size(1), slots.data_ptr<int64_t>(), k.data_ptr(),
@@ -125,9 +131,9 @@ struct Call {
     page = (int)kc.size(1);
     Hkv = (int)kc.size(2);
     max_pages = (int)bt.size(1);
-    out = at::empty(q.sizes(), q.options());
+    out = empty_on(d, q.sizes(), at::kBFloat16);
     ws_bytes = q.numel() ? q3a_paged_decode_tree_workspace_bytes(B, N, Hq, Hkv, D, max_pages, page) : 0;
-    if (ws_bytes > 0) ws = at::empty({(int64_t)ws_bytes}, q.options().dtype(at::kByte));
+    if (ws_bytes > 0) ws = empty_on(d, {(int64_t)ws_bytes}, at::kByte);
   }
   void* workspace() const { return ws_bytes > 0 ? ws.data_ptr() : nullptr; }
 };

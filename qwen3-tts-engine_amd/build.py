@@ -91,7 +91,7 @@ def _compile_torch_ops() -> str:
 def _link_torch_ops(obj: str) -> None:
     import torch
     _run([CXX, "-shared", obj, "-L" + os.path.dirname(OUT), "-lq3attn", "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"),
-          "-lc10", "-lc10_hip", "-ltorch_cpu", "-Wl,-rpath,$ORIGIN", "-o", TORCH_OUT + ".tmp"], f"linking {TORCH_OUT}")
+          "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-Wl,-rpath,$ORIGIN", "-o", TORCH_OUT + ".tmp"], f"linking {TORCH_OUT}")
     os.replace(TORCH_OUT + ".tmp", TORCH_OUT)
 
 
