@@ -446,8 +446,8 @@ int q3a_prefill_append_rope(
  *
  * An element is code * 2^(s - 127).  A written row x[0..127] gets the smallest power of two 2^(s-127) >= 2^-117 with
  * max |x_d| <= 448 * 2^(s-127) over its finite elements, and codes e4m3(x_d * 2^(127-s)) rounded to nearest even (at s = 247 at
- * most 240, so that none stands for more than bf16 holds); elements that are not finite are held as NaN.  Every value read back is a bf16 number, so attention over the pool is attention over
- * the bf16 rows read back.  Bytes outside 10..247 are not written by q3a_paged_write_fp8 and stand for no value.
+ * most 240, so that none stands for more than bf16 holds); elements that are not finite are held as NaN.  Every value read
+ * back is a bf16 number, so attention over the pool is attention over the bf16 rows read back.  Bytes outside 10..247 are not written by q3a_paged_write_fp8 and stand for no value.
  * Requirements: page_size a multiple of 16, caches 16-byte aligned with strides multiples of 16, token stride in
  * [128, 2^26]; scales 4-byte aligned with strides multiples of 4.  Any layout with these strides serves; with a page's tokens
  * of one head next to each other (strides page: Hkv * page_size * 128, head: page_size * 128, token: 128) a head's page is
@@ -456,7 +456,7 @@ int q3a_prefill_append_rope(
  * q3a_paged_write_fp8 quantises rows k, v [T, Hkv, 128] bf16 (token and head strides) into slots [T] int64, slot = page *
  * page_size + offset; tokens with a slot outside [0, num_pages * page_size) are not written.  A slot named by two tokens holds
  * a mix of both afterwards: only a scratch slot that nothing reads may be.  Replaces, for this pool, the index_copy_ pair of
- * engine/talker.py:72-73 and :161-162.  T * Hkv at most 2^28.
+ * engine/talker.py:72-73 and :161-162.  T * Hkv at most 2^28, Hkv at most 65,536.
  *
  * q3a_paged_read_fp8 writes the rows of slots [T] back as bf16 k, v [T, Hkv, 128]; slots outside the pool read zeros.
  */
