@@ -1297,8 +1297,9 @@ int run(const char* who, TreeArgs a, int mode, bool fp8, int batch, int hq, size
   }
   a.group = hq / a.hkv;
   a.M = a.nodes * a.group;
-  if (((int64_t)a.num_pages * kv_page + (int64_t)a.page_size * kv_tok) * elem >= (int64_t)1 << 36 ||
-      (fp8 && (int64_t)a.num_pages * a.ss_p >= (int64_t)1 << 32))
+  // (in floating point: the products of any strides)
+  if (((double)a.num_pages * (double)kv_page + (double)a.page_size * (double)kv_tok) * elem >= 0x1p36 ||
+      (fp8 && (double)a.num_pages * (double)a.ss_p >= 0x1p32))
     return fail(Q3A_EINVAL, "%s: a cache of 64 GiB or more, or scales of 4 GiB", who);
   const Plan p = plan_of(batch, a.nodes, hq, a.hkv, (int64_t)a.max_pages * a.page_size);
   if (p.bytes > 0 && (a.ws == nullptr || workspace_bytes < p.bytes || ((uintptr_t)a.ws & 15) != 0))
