@@ -238,11 +238,11 @@ __device__ __forceinline__ void load_k(const TreeArgs& a, const Place& p, int la
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const auto rk = make_rsrc(a.kc + p.at[u], extent<true>(a, p.valid[u]));
-    const uint32_t row = (uint32_t)(r & ~1) * (uint32_t)a.st + 64 * (r & 1) + 16 * g;
+    const uint32_t row = kOnce ? (uint32_t)(r & ~1) * (uint32_t)a.st + 64 * (r & 1) + 16 * g : (uint32_t)r * (uint32_t)a.st + 16 * g;
     auto ld = [&](uint32_t o) {
       return __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rk, (int)o, 0, kOnce ? kNt : 0));
     };
-    x.k[u] = __builtin_shufflevector(ld(row), ld(row + (uint32_t)a.st), 0, 1, 2, 3, 4, 5, 6, 7);
+    x.k[u] = __builtin_shufflevector(ld(row), ld(row + (kOnce ? (uint32_t)a.st : 64u)), 0, 1, 2, 3, 4, 5, 6, 7);
     const auto rs = make_rsrc(a.ks + p.sat[u], p.valid[u] > 0 ? 16 : 0);
     x.ks[u] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rs, r, 0, 0);
   }
@@ -451,6 +451,10 @@ __device__ __forceinline__ void scores(const KeyTile<false>& x, const Query<fals
   }
 }
 
+// The larger of two scores as one instruction: fmaxf quiets each operand first.  (Of a NaN and a number the number, of two NaN
+// +inf: a NaN score makes its row NaN either way.)
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
+
 // The scores to probabilities: scaled, masked, exp2 of them minus the running maximum, which with the sum is updated and O
 // rescaled to.
 // kMasked: seen[t] tells which of the lane's 8 keys (bit 4 u + i) its query row sees; else the subtiles' valid ones.
@@ -458,10 +462,10 @@ template <bool kMasked, int kMT>
 __device__ __forceinline__ void softmax(const int (&valid)[2], const uint32_t (&seen)[kMT], float scale,
                                         f32x4_t (&s)[kMT][2], State<kMT>& st) {
   const bool full = valid[0] == 16 && valid[1] == 16;
+  if (kMasked || !full) {
+    const int g = lane_now() >> 4;
 #pragma unroll
-  for (int t = 0; t < kMT; ++t) {
-    if (kMasked || !full) {
-      const int g = lane_now() >> 4;
+    for (int t = 0; t < kMT; ++t)
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -469,13 +473,21 @@ __device__ __forceinline__ void softmax(const int (&valid)[2], const uint32_t (&
           const bool ok = kMasked ? ((seen[t] >> (4 * u + i)) & 1) != 0 : 4 * g + i < valid[u];
           s[t][u][i] = ok ? s[t][u][i] : -INFINITY;
         }
-    }
-    float top = fmaxf(fmaxf(fmaxf(s[t][0][0], s[t][0][1]), fmaxf(s[t][0][2], s[t][0][3])),
-                      fmaxf(fmaxf(s[t][1][0], s[t][1][1]), fmaxf(s[t][1][2], s[t][1][3])));
-    top = max_xor32(max_xor16(top));
-    // O and l are rescaled only when some query row's maximum has grown (a factor of 1 changes nothing).
-    if (__builtin_amdgcn_ballot_w64(top > st.m[t]) != 0) {
-      const float m = fmaxf(st.m[t], top);
+  }
+  float top[kMT];
+  bool grown = false;
+#pragma unroll
+  for (int t = 0; t < kMT; ++t) {
+    top[t] = larger(larger(larger(s[t][0][0], s[t][0][1]), larger(s[t][0][2], s[t][0][3])),
+                    larger(larger(s[t][1][0], s[t][1][1]), larger(s[t][1][2], s[t][1][3])));
+    top[t] = max_xor32(max_xor16(top[t]));
+    grown = grown | (top[t] > st.m[t]);
+  }
+  // O and l are rescaled only when some query row's maximum has grown (a factor of 1 changes nothing).
+  if (__builtin_amdgcn_ballot_w64(grown) != 0) {
+#pragma unroll
+    for (int t = 0; t < kMT; ++t) {
+      const float m = fmaxf(st.m[t], top[t]);
       const float alpha = fast_exp2((st.m[t] - (m == -INFINITY ? 0.f : m)) * scale);
       st.m[t] = m;
       st.l[t] *= alpha;
@@ -484,6 +496,9 @@ __device__ __forceinline__ void softmax(const int (&valid)[2], const uint32_t (&
 #pragma unroll
         for (int i = 0; i < 4; ++i) st.o[t][j][i] *= alpha;
     }
+  }
+#pragma unroll
+  for (int t = 0; t < kMT; ++t) {
     const float base = st.m[t] == -INFINITY ? 0.f : st.m[t] * scale;  // nothing seen so far: every exp2 below is of -inf
     float sum = 0.f;
 #pragma unroll
@@ -604,7 +619,7 @@ __device__ __forceinline__ void add_not_finite(const uint16_t* vb, int ts, const
 // The nodes' own keys 32 ts .. + 31, in bf16, with each lane's query rows' view of its 8 keys.  An own V element that is
 // not finite must not reach the rows that do not see its key (0 * inf in the product): such elements are zeroed in the
 // product and added afterwards for the rows that see them.
-template <bool kFp8, int kMT, bool kTight>
+template <bool kFp8, int kMT>
 __device__ __forceinline__ void tree_step(const Work& w, int ts, const Query<false, kMT>& q, State<kMT>& st) {
   const int lane = lane_now();
   const int r = lane & 15, g = lane >> 4;
@@ -631,7 +646,7 @@ __device__ __forceinline__ void tree_step(const Work& w, int ts, const Query<fal
         y.v[u][i] = make_uint4(e.x & keep, e.y & keep, e.z & keep, e.w & keep);
       }
   };
-  if constexpr (!kTight) load_values();
+  load_values();
   uint32_t seen[kMT];
 #pragma unroll
   for (int t = 0; t < kMT; ++t) {
@@ -660,10 +675,6 @@ __device__ __forceinline__ void tree_step(const Work& w, int ts, const Query<fal
   const int any[2] = {16, 16};
   f32x4_t sc[kMT][2];
   scores<false, kMT>(x, q, sc);
-  if constexpr (kTight) {  // the registers do not hold V beside K
-    __builtin_amdgcn_sched_barrier(0);
-    load_values();
-  }
   softmax<true, kMT>(any, seen, a.scale_log2, sc, st);
   uint32_t top = 0;
 #pragma unroll
@@ -780,12 +791,12 @@ __device__ __forceinline__ void load_q(const Work& w, bf16x8_t (&q)[kMT][4]) {
   }
 }
 
-// A wave's cached steps in registers: a step's K is loaded while the one before it has its softmax and V product, its V behind
-// that product.
+// A wave's cached steps in registers: as soon as a step's K has been multiplied, the next step's K is loaded in its place, and
+// its V behind the V product.  (Two steps in registers ahead of the one computed were no faster, where they fitted.)
 template <bool kFp8, int kMT>
 struct Stream {
-  static constexpr bool kOnce = kMT == 1;            // else other blocks of query rows may read the keys too
-  static constexpr bool kLayout = kFp8 || kMT == 1;  // swapped, or paired
+  static constexpr bool kOnce = kMT == 1;    // else other blocks of query rows may read the keys too
+  static constexpr bool kLayout = kMT == 1;  // swapped, or paired
   KeyTile<kFp8> k;
   ValueTile<kFp8> v;
   int valid[2];
@@ -828,10 +839,9 @@ __device__ __forceinline__ void append_step(const TreeArgs& a, const Work& w, co
   values<true, kMT>(y, one, lane, s, st);
 }
 
-// Q as the products take it (raw: as it was loaded), a clear state, and this wave's own steps s, s + kW, ... before T.
-template <bool kFp8, int kMode, int kMT, int kW>
-__device__ __forceinline__ void first_steps(const TreeArgs& a, const Work& w, int s, int T, int lane, Query<false, kMT>& raw,
-                                            Query<kFp8, kMT>& q, State<kMT>& st) {
+// raw, as it was loaded, with the sign that the scale asks for.
+template <int kMT>
+__device__ __forceinline__ void turn_signs(Query<false, kMT>& raw) {
   const uint32_t sign = args_again().q_sign;
 #pragma unroll
   for (int t = 0; t < kMT; ++t)
@@ -840,18 +850,6 @@ __device__ __forceinline__ void first_steps(const TreeArgs& a, const Work& w, in
       const uint4 v = __builtin_bit_cast(uint4, raw.v[t][c]);
       raw.v[t][c] = __builtin_bit_cast(bf16x8_t, make_uint4(v.x ^ sign, v.y ^ sign, v.z ^ sign, v.w ^ sign));
     }
-  if constexpr (kMode == kTree) {
-    clear(st);
-    for (; s < T; s += kW) tree_step<kFp8, kMT, kMT == 2 && !kFp8>(w, s - w.Tc, raw, st);
-  }
-  prepare(raw.v, q);
-  if constexpr (kMode != kTree) {
-    __builtin_amdgcn_sched_barrier(0);
-    clear(st);  // (not before: Q's two parts and what they come from fill the registers)
-  }
-  if constexpr (kMode == kAppend) {
-    if (s < T) append_step<kMT>(a, w, q, lane, st);
-  }
 }
 
 // Query rows that the waves merge at once, 34 KB of them.
@@ -1072,7 +1070,7 @@ __device__ __forceinline__ int kth_longest(const TreeArgs& a, int row0, int k, i
 // One workgroup a (row, KV head, block of 16 kMT query rows), its kW waves taking the row's steps in turn; or (kChunked) one of
 // a chunk of a row's steps, which leaves a record for the join kernel unless it is the row's only one.
 template <bool kFp8, int kMode, int kMT, int kW, bool kChunked>
-__global__ __launch_bounds__(64 * kW, kMT == 1 && kFp8 && kMode != kTree ? 3 : 2) void tree_kernel(const TreeArgs args) {
+__global__ __launch_bounds__(64 * kW, kMT == 2 || (kMode == kTree && kChunked) ? 2 : 3) void tree_kernel(const TreeArgs args) {
   __shared__ __align__(16) MergeLds<kW> lds;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Work w;
@@ -1134,10 +1132,38 @@ __global__ __launch_bounds__(64 * kW, kMT == 1 && kFp8 && kMode != kTree ? 3 : 2
     };
     Stream<kFp8, kMT> x;
     Query<kFp8, kMT> q;
-    constexpr bool kEarly = kFp8 || kMT == 1;  // else own steps and a tile do not fit the registers together
-    if constexpr (kEarly) x.load(a, place(0), lane);
-    first_steps<kFp8, kMode, kMT, kW>(a, w, own, s1, lane, raw, q, st);
-    if constexpr (!kEarly) x.load(a, place(0), lane);
+    if constexpr (kMode == kTree) {
+      // A wave that has own steps takes them first.  Chunks, which are few, ask for their keys ahead of them; where the chip is
+      // full the registers that this takes would cost every compute unit its third workgroup (256 rows x 600 tokens x 8 nodes
+      // over the 8-bit pool: 67.0 us with three, 70.7 with two; one row of four nodes: 0.4 us the other way).
+      constexpr bool kEarly = kChunked && (kFp8 || kMT == 1);
+      auto own_steps = [&]() __attribute__((always_inline)) {
+        turn_signs(raw);
+        clear(st);
+        for (int s = own; s < s1; s += kW) tree_step<kFp8, kMT>(w, s - w.Tc, raw, st);
+      };
+      if constexpr (kEarly) {
+        x.load(a, place(0), lane);
+        own_steps();
+      } else if (own < s1) {
+        own_steps();
+        x.load(a, place(0), lane);
+      } else {
+        x.load(a, place(0), lane);
+        turn_signs(raw);
+        clear(st);
+      }
+      prepare(raw.v, q);
+    } else {
+      x.load(a, place(0), lane);
+      turn_signs(raw);
+      prepare(raw.v, q);
+      __builtin_amdgcn_sched_barrier(0);
+      clear(st);  // (not before: Q's two parts and what they come from fill the registers)
+      if constexpr (kMode == kAppend) {
+        if (own < s1) append_step<kMT>(a, w, q, lane, st);
+      }
+    }
     for (int i = 0; i < n; ++i) x.turn(a, place(i + 1), q, lane, st);
   }
   merge_waves<kMT, kW>(w, st, rec, wave, lds);
