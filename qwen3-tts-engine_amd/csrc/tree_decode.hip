@@ -451,13 +451,18 @@ __device__ __forceinline__ void scores(const KeyTile<false>& x, const Query<fals
   }
 }
 
-// The larger of two scores as one instruction: fmaxf quiets each operand first.  (Of a NaN and a number the number, of two NaN
-// +inf: a NaN score makes its row NaN either way.)
-__device__ __forceinline__ float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
+// The larger of two scores, NaN if one is (its row will be NaN either way).  fmaxf would quiet each operand first.
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
-// The scores to probabilities: scaled, masked, exp2 of them minus the running maximum, which with the sum is updated and O
-// rescaled to.
+// The scores to probabilities: scaled, masked, exp2 of them minus a base, which with the sum is updated and O rescaled to.
 // kMasked: seen[t] tells which of the lane's 8 keys (bit 4 u + i) its query row sees; else the subtiles' valid ones.
+//
+// The base need not be the maximum, only near it: it moves when some query row's probabilities have outgrown 2^kAhead, which
+// after a row's first steps hardly happens, while with 16 or 32 query rows some row's maximum grows in almost every step, and
+// rescaling is a sixth to a quarter of a step's vector instructions (6 rows x 63 nodes: 82.7 us with kAhead = 0, 80.2 with 4, 79.3
+// with 6).  O and l hold up to 2^kAhead times as much for it.
+constexpr float kAhead = 4.f;
+
 template <bool kMasked, int kMT>
 __device__ __forceinline__ void softmax(const int (&valid)[2], const uint32_t (&seen)[kMT], float scale,
                                         f32x4_t (&s)[kMT][2], State<kMT>& st) {
@@ -481,13 +486,12 @@ __device__ __forceinline__ void softmax(const int (&valid)[2], const uint32_t (&
     top[t] = larger(larger(larger(s[t][0][0], s[t][0][1]), larger(s[t][0][2], s[t][0][3])),
                     larger(larger(s[t][1][0], s[t][1][1]), larger(s[t][1][2], s[t][1][3])));
     top[t] = max_xor32(max_xor16(top[t]));
-    grown = grown | (top[t] > st.m[t]);
+    grown = grown | ((top[t] - st.m[t]) * scale > kAhead);
   }
-  // O and l are rescaled only when some query row's maximum has grown (a factor of 1 changes nothing).
   if (__builtin_amdgcn_ballot_w64(grown) != 0) {
 #pragma unroll
     for (int t = 0; t < kMT; ++t) {
-      const float m = fmaxf(st.m[t], top[t]);
+      const float m = larger(st.m[t], top[t]);
       const float alpha = fast_exp2((st.m[t] - (m == -INFINITY ? 0.f : m)) * scale);
       st.m[t] = m;
       st.l[t] *= alpha;
@@ -500,15 +504,11 @@ __device__ __forceinline__ void softmax(const int (&valid)[2], const uint32_t (&
 #pragma unroll
   for (int t = 0; t < kMT; ++t) {
     const float base = st.m[t] == -INFINITY ? 0.f : st.m[t] * scale;  // nothing seen so far: every exp2 below is of -inf
-    float sum = 0.f;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[t][u][i] = fast_exp2(__builtin_fmaf(s[t][u][i], scale, -base));
-        sum += s[t][u][i];
-      }
-    st.l[t] += sum;
+      for (int i = 0; i < 4; ++i) s[t][u][i] = fast_exp2(__builtin_fmaf(s[t][u][i], scale, -base));
+    st.l[t] += ((s[t][0][0] + s[t][0][1]) + (s[t][0][2] + s[t][0][3])) + ((s[t][1][0] + s[t][1][1]) + (s[t][1][2] + s[t][1][3]));
   }
 }
 
@@ -1164,7 +1164,8 @@ __global__ __launch_bounds__(64 * kW, kMT == 2 || (kMode == kTree && kChunked) ?
         if (own < s1) append_step<kMT>(a, w, q, lane, st);
       }
     }
-    for (int i = 0; i < n; ++i) x.turn(a, place(i + 1), q, lane, st);
+    const TreeArgs again = at_head(args_again(), w.h);  // (not held in registers, and spilled, since the kernel's start)
+    for (int i = 0; i < n; ++i) x.turn(again, place(i + 1), q, lane, st);
   }
   merge_waves<kMT, kW>(w, st, rec, wave, lds);
 }
