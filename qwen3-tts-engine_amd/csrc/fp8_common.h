@@ -53,6 +53,16 @@ __device__ __forceinline__ uint32_t bf16_amax_pair(const uint32_t (&w)[N]) {
 }
 __device__ __forceinline__ uint32_t halves_max(uint32_t a) { return max(a & 0xffffu, a >> 16); }
 
+// Two dwords of bf16 (4 elements) -> one dword of e4m3 codes, of finite elements up to 448 scale.
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2_t;
+__device__ __forceinline__ uint32_t fp8_finite_codes4(uint32_t w0, uint32_t w1, float scale) {
+  s16x2 r = {0, 0};
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2_t, w0), scale, false);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2_t, w1), scale, true);
+  return __builtin_bit_cast(uint32_t, r);
+}
+
 // Two dwords of bf16 (4 elements) -> one dword of e4m3 codes at the exponent byte s.
 __device__ __forceinline__ uint32_t fp8_codes4(uint32_t w0, uint32_t w1, uint32_t s) {
   const float inv = fp8_inv_scale(s), most = s >= kMaxScaleByte ? 240.f : 448.f;

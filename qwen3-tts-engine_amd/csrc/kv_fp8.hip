@@ -52,13 +52,10 @@ __device__ __forceinline__ void write_row(const uint4 a, const uint4 b, bool liv
   top = dpp_max_u32<kDppXor2>(top);
   top = dpp_max_u32<kDppHalfMirror>(top);
   const uint32_t s = fp8_scale_byte(top);
-  const float inv = fp8_inv_scale(s);
+  const float scale = fp8_scale(s);
   uint32_t c[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = __builtin_amdgcn_cvt_pk_fp8_f32(bf16_lo(w[2 * i]) * inv, bf16_hi(w[2 * i]) * inv, 0, false);
-    c[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(bf16_lo(w[2 * i + 1]) * inv, bf16_hi(w[2 * i + 1]) * inv, r, true);
-  }
+  for (int i = 0; i < 4; ++i) c[i] = fp8_finite_codes4(w[2 * i], w[2 * i + 1], scale);
   if (rare) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) c[i] = fp8_codes4(w[2 * i], w[2 * i + 1], s);

@@ -5,8 +5,13 @@
 // sees those that its mask row allows (decode: N = 1 and no own key, or its own one as the pool will hold it).  With
 // G = Hq / Hkv the M = N G query rows m = (n, g) of a KV head share every key:
 //   s_mj = scale q_m . k_j,   o_m = sum_j exp(s_mj - max_j s_mj) v_j / sum_j exp(s_mj - max_j s_mj);   zeros if nothing is seen.
+// K and V are read once for each block of 16 kMT query rows, so with few query rows HBM bounds it: 768 rows of 512 tokens over
+// the 8-bit pool run at 6.2 TB/s (with 5 % more than the keys for the exponent bytes' lines), 256 rows of 600 tokens and 8 nodes
+// over bf16 at 5.9.  63 nodes are bound by vector instructions (480 TFLOP/s), calls of a few rows by latency: 5 us from start to
+// end of the shortest row, of which the keys' way is 2.5.
 //
-// A step is 32 keys (two 16-token subtiles, each inside one page) by 16 kMT query rows, on one wave, from registers alone:
+// A step is 32 keys (two 16-token subtiles, each inside one page) by 16 kMT query rows, on one wave, from registers alone (kMT is
+// 1 up to 16 query rows, else 2: more do not fit the registers):
 //   S^T = K Q^T   A = 16 keys, B = Q^T.  bf16: v_mfma_f32_16x16x32_bf16; lane l holds key l % 16 and, of each 32 dims, the 8
 //                 that its quarter g = l / 16 takes: any split of the 128 dims over (step, quarter) is right as long as Q has
 //                 the same.  8-bit: one v_mfma_scale_f32_16x16x128_f8f6f4 on the codes as they are stored, K's exponent byte
@@ -44,6 +49,7 @@ enum { kNoKeys = 0, kTree = 1, kAppend = 2 };
 
 typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8_t;
 typedef __attribute__((__vector_size__(4 * sizeof(float)))) float f32x4_t;
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 
@@ -177,7 +183,7 @@ struct Work {
 template <int kMT>
 struct State {
   f32x4_t o[kMT][8];
-  float m[kMT], l[kMT];  // of query row l % 16: maximum of the unscaled scores; sum, of this quarter's keys until the merge
+  float m[kMT], l[kMT];  // of query row l % 16: the exponents' base, unscaled; sum, of this quarter's keys until the merge
 };
 
 __device__ __forceinline__ int row_tokens(int b, int mode) {
@@ -203,12 +209,14 @@ constexpr int kNt = 2;
 // A line is 8 lanes' 16 bytes, but an A operand has a row on 4 lanes only, so loading operand rows as they are takes each line
 // in two halves by two instructions, which the non-temporal policy does not suit (a twentieth of the decode's time).  So two
 // lanes that hold neighbouring rows load from one key at a time:
-//   8-bit codes   load i: half r & 1 of key (r & ~1) + i.  The two lanes then exchange what is the other's (two DPP selects a
-//                 register, before the product).
-//   bf16, kPaired (16 query rows): operand row r of a load holds half (r & 1) of a line of key (r & ~3) + 2 i + ((r >> 1) & 1),
+//   8-bit codes   load i: half r & 1 of key (r & ~1) + i.  The two lanes then exchange what is the other's (a DPP move and a
+//                 select a register, before the product).
+//   bf16, kPaired operand row r of a load holds half (r & 1) of a line of key (r & ~3) + 2 i + ((r >> 1) & 1),
 //                 i the load's pair.  Even rows have to meet Q's dims of the lines' first half, odd rows the second's: two
 //                 products of which each uses half, and the score of a key is the sum of two neighbouring rows, which one lane
-//                 holds.  The lane's four keys stay 4 g .. 4 g + 3.  With more query rows the second product costs too much.
+//                 holds.  The lane's four keys stay 4 g .. 4 g + 3.
+// With 32 query rows, which vector instructions bound, the keys are loaded in rows: the exchange and the second product would cost
+// more than they give.
 //
 // No branches and always the same loads, also for a step that is not there (its page ids are -1): only so does the compiler
 // know how many newer loads may be in flight when older ones are waited for, and not wait for all.
@@ -322,7 +330,6 @@ __device__ __forceinline__ void v_operands(const ValueTile<false>& x, int jj, bf
   a1 = __builtin_bit_cast(bf16x8_t, make_uint4(p1[0], p1[1], p1[2], p1[3]));
 }
 
-
 // Q^T as B operands: bf16 as it is, or, against 8-bit keys, in two e4m3 parts.
 //
 // The matrix instruction takes K's codes and its power-of-two scale (one byte a key) as they are, with Q as hi + lo: of q's 8
@@ -373,26 +380,25 @@ __device__ __forceinline__ void prepare(const bf16x8_t (&q)[kMT][4], Query<true,
     const bool rare = __builtin_amdgcn_ballot_w64(top >= 0x7f00u) != 0;
     if (rare) top = row_max(halves_max(bf16_amax_pair(w)));
     const uint32_t sb = fp8_scale_byte(top);
-    const float inv = fp8_inv_scale(sb);
+    const float scale = fp8_scale(sb);
     x.s[t] = (int)sb;
-    int hi[8];
+    uint32_t hi[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      hi[i] = __builtin_amdgcn_cvt_pk_fp8_f32(bf16_lo(w[2 * i]) * inv, bf16_hi(w[2 * i]) * inv, 0, false);
-      hi[i] = __builtin_amdgcn_cvt_pk_fp8_f32(bf16_lo(w[2 * i + 1]) * inv, bf16_hi(w[2 * i + 1]) * inv, hi[i], true);
-    }
+    for (int i = 0; i < 8; ++i) hi[i] = fp8_finite_codes4(w[2 * i], w[2 * i + 1], scale);
     if (rare) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) hi[i] = (int)fp8_codes4(w[2 * i], w[2 * i + 1], sb);
+      for (int i = 0; i < 8; ++i) hi[i] = fp8_codes4(w[2 * i], w[2 * i + 1], sb);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const auto h0 = __builtin_amdgcn_cvt_pk_f32_fp8(hi[i], false), h1 = __builtin_amdgcn_cvt_pk_f32_fp8(hi[i], true);
-      auto rest = [&](float y, float h) { return __builtin_fmaf(y, inv, -h) * 16.f; };  // at most 256 (at byte 247: 240)
-      int lo = __builtin_amdgcn_cvt_pk_fp8_f32(rest(bf16_lo(w[2 * i]), h0[0]), rest(bf16_hi(w[2 * i]), h0[1]), 0, false);
-      lo = __builtin_amdgcn_cvt_pk_fp8_f32(rest(bf16_lo(w[2 * i + 1]), h1[0]), rest(bf16_hi(w[2 * i + 1]), h1[1]), lo, true);
-      x.hi[t][i] = hi[i];
-      x.lo[t][i] = lo;
+      // what hi leaves, exact in fp32: at most 16 scale (at byte 247: 15 scale), so e4m3 at a 16th of the scale holds it
+      s16x2 lo = {0, 0};
+      const f32x2_t h0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi[i], scale, false);
+      const f32x2_t h1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi[i], scale, true);
+      lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, bf16_lo(w[2 * i]) - h0[0], bf16_hi(w[2 * i]) - h0[1], scale * 0.0625f, false);
+      lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, bf16_lo(w[2 * i + 1]) - h1[0], bf16_hi(w[2 * i + 1]) - h1[1], scale * 0.0625f, true);
+      x.hi[t][i] = (int)hi[i];
+      x.lo[t][i] = __builtin_bit_cast(int, lo);
     }
   }
 }
@@ -1326,7 +1332,7 @@ int run(const char* who, TreeArgs a, int mode, bool fp8, int batch, int hq, size
   a.M = a.nodes * a.group;
   // (in floating point: the products of any strides)
   if (((double)a.num_pages * (double)kv_page + (double)a.page_size * (double)kv_tok) * elem >= 0x1p36 ||
-      (fp8 && (double)a.num_pages * (double)a.ss_p >= 0x1p32))
+      (fp8 && (double)a.num_pages * (double)a.ss_p + a.page_size >= 0x1p32))
     return fail(Q3A_EINVAL, "%s: a cache of 64 GiB or more, or scales of 4 GiB", who);
   const Plan p = plan_of(batch, a.nodes, hq, a.hkv, (int64_t)a.max_pages * a.page_size);
   if (p.bytes > 0 && (a.ws == nullptr || workspace_bytes < p.bytes || ((uintptr_t)a.ws & 15) != 0))
