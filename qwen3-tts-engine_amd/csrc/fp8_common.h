@@ -53,6 +53,18 @@ __device__ __forceinline__ uint32_t bf16_amax_pair(const uint32_t (&w)[N]) {
 }
 __device__ __forceinline__ uint32_t halves_max(uint32_t a) { return max(a & 0xffffu, a >> 16); }
 
+// The same whatever the elements are.
+template <int N>
+__device__ __forceinline__ uint32_t bf16_any_amax_pair(const uint32_t (&w)[N]) {
+  uint32_t a = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) a = pk_max_u16(a, w[i] & 0x7fff7fffu);
+  return a;
+}
+// Rows with infinities and NaN, or close to the largest bf16, are rare: their codes need care (bf16_amax_pair, fp8_codes4).
+// True on all lanes if one's largest magnitude bits tell so.
+__device__ __forceinline__ bool any_rare(uint32_t top) { return __builtin_amdgcn_ballot_w64(top >= 0x7f00u) != 0; }
+
 // Two dwords of bf16 (4 elements) -> one dword of e4m3 codes, of finite elements up to 448 scale.
 typedef short s16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2_t;

@@ -41,12 +41,8 @@ struct WriteArgs {
 
 __device__ __forceinline__ void write_row(const uint4 a, const uint4 b, bool live, uint8_t* dst, uint8_t* dscale, int sub) {
   const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-  uint32_t top = 0;  // of the magnitude bits, whatever they are
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = pk_max_u16(top, w[i] & 0x7fff7fffu);
-  top = halves_max(top);
-  // Infinities, NaN and the largest magnitudes are rare: their codes need care.
-  const bool rare = __builtin_amdgcn_ballot_w64(top >= 0x7f00u) != 0;
+  uint32_t top = halves_max(bf16_any_amax_pair(w));
+  const bool rare = any_rare(top);
   if (rare) top = halves_max(bf16_amax_pair(w));
   top = dpp_max_u32<kDppXor1>(top);
   top = dpp_max_u32<kDppXor2>(top);

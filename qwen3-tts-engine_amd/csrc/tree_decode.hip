@@ -372,12 +372,8 @@ __device__ __forceinline__ void prepare(const bf16x8_t (&q)[kMT][4], Query<true,
       w[4 * c + 2] = e.z;
       w[4 * c + 3] = e.w;
     }
-    uint32_t top = 0;  // of the magnitude bits, whatever they are
-#pragma unroll
-    for (int i = 0; i < 16; ++i) top = pk_max_u16(top, w[i] & 0x7fff7fffu);
-    top = row_max(halves_max(top));
-    // Rows with infinities and NaN, or close to the largest bf16, are rare: their codes need care.
-    const bool rare = __builtin_amdgcn_ballot_w64(top >= 0x7f00u) != 0;
+    uint32_t top = row_max(halves_max(bf16_any_amax_pair(w)));
+    const bool rare = any_rare(top);
     if (rare) top = row_max(halves_max(bf16_amax_pair(w)));
     const uint32_t sb = fp8_scale_byte(top);
     const float scale = fp8_scale(sb);
@@ -729,7 +725,12 @@ __device__ __forceinline__ void append_keys(const TreeArgs& a, const Work& w, bo
   vw[1] = e.y;
   vw[2] = e.z;
   vw[3] = e.w;
-  uint32_t km = halves_max(bf16_amax_pair(kw)), vm = halves_max(bf16_amax_pair(vw));
+  uint32_t km = halves_max(bf16_any_amax_pair(kw)), vm = halves_max(bf16_any_amax_pair(vw));
+  const bool rare = any_rare(max(km, vm));
+  if (rare) {
+    km = halves_max(bf16_amax_pair(kw));
+    vm = halves_max(bf16_amax_pair(vw));
+  }
   km = row_max(km);
   vm = dpp_max_u32<kDppXor1>(vm);
   vm = dpp_max_u32<kDppXor2>(vm);
@@ -744,25 +745,31 @@ __device__ __forceinline__ void append_keys(const TreeArgs& a, const Work& w, bo
 #pragma unroll
     for (int i = 0; i < 4; ++i) y.v[u][i] = make_uint2(0u, 0u);
   }
-  uint4 kc[2];
+  uint32_t kc[8], vc[2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    kc[i] = make_uint4(fp8_codes4(kw[8 * i], kw[8 * i + 1], ks), fp8_codes4(kw[8 * i + 2], kw[8 * i + 3], ks),
-                       fp8_codes4(kw[8 * i + 4], kw[8 * i + 5], ks), fp8_codes4(kw[8 * i + 6], kw[8 * i + 7], ks));
-  const uint2 vc = make_uint2(fp8_codes4(vw[0], vw[1], vs), fp8_codes4(vw[2], vw[3], vs));
+  for (int i = 0; i < 8; ++i) kc[i] = fp8_finite_codes4(kw[2 * i], kw[2 * i + 1], fp8_scale(ks));
+#pragma unroll
+  for (int i = 0; i < 2; ++i) vc[i] = fp8_finite_codes4(vw[2 * i], vw[2 * i + 1], fp8_scale(vs));
+  if (rare) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) kc[i] = fp8_codes4(kw[2 * i], kw[2 * i + 1], ks);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) vc[i] = fp8_codes4(vw[2 * i], vw[2 * i + 1], vs);
+  }
   valid = ok ? 1 : 0;
   if (r == 0) {
-    x.k[0] = __builtin_shufflevector(__builtin_bit_cast(i32x4_t, kc[0]), __builtin_bit_cast(i32x4_t, kc[1]), 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x.k[0][i] = (int)kc[i];
   }
-  if (g == 0) y.v[0][0] = vc;
+  if (g == 0) y.v[0][0] = make_uint2(vc[0], vc[1]);
   if (store && ok) {
     const int64_t at = (int64_t)page * a.sp + (int64_t)off * a.st;
     const int64_t sat = (int64_t)page * a.ss_p + off;
     if (r == 0) {
-      st16(a.kc + at + dim_of<true>(0, g), kc[0]);
-      st16(a.kc + at + dim_of<true>(2, g), kc[1]);
+      st16(a.kc + at + dim_of<true>(0, g), make_uint4(kc[0], kc[1], kc[2], kc[3]));
+      st16(a.kc + at + dim_of<true>(2, g), make_uint4(kc[4], kc[5], kc[6], kc[7]));
     }
-    if (g == 0) *reinterpret_cast<u32x2*>(a.vc + at + 8 * r) = __builtin_bit_cast(u32x2, vc);
+    if (g == 0) *reinterpret_cast<u32x2*>(a.vc + at + 8 * r) = u32x2{vc[0], vc[1]};
     if (lane == 0) {
       a.ks[sat] = (uint8_t)ks;
       a.vs[sat] = (uint8_t)vs;
