@@ -1270,11 +1270,12 @@ Plan plan_of(int batch, int nodes, int hq, int hkv, int64_t capacity) {
   p.mblocks = (M + 16 * tiles - 1) / (16 * tiles);
   p.units = batch;
   // Whole rows take one launch, but the longest row's steps follow each other on one compute unit; chunks cost the join (3.7 us)
-  // and records.  8 heads x 1 row are equal at 512 tokens (8.5 us, 9.7 as chunks; at 1000: 11.9, 9.8), 256 workgroups at about
-  // 1000 (16.0, 19.3; with up to 1700 tokens and 13 nodes: 26.8, 22.5), 512 above 1500 (22.8, 23.4).  Rows that are more than
-  // the chip holds at once balance by themselves.
+  // and records.  Rows of one length, us whole and in chunks: 8 workgroups of 512 tokens 7.6 and 9.0, of 1000 11.0 and 9.1; 64 of
+  // 1000 11.9 and 11.2; 128 of 1000 13.9 and 15.3, of 2000 22.6 and 19.4; 256 of 1000 15.0 and 19.3.  Ragged rows leave whole ones
+  // waiting for the longest: 192 workgroups of up to 1373 tokens 15.8 and 13.9, 256 of up to 1725 (13 nodes) 21.4 and 19.2, but 512
+  // of up to 1500 20.0 and 24.4.  Rows that are more than the chip holds at once balance by themselves.
   const int64_t groups = (int64_t)batch * hkv * p.mblocks;
-  if (batch > 1024 || capacity * num_cus() <= 512 * (num_cus() + groups)) return p;
+  if (batch > 1024 || capacity * num_cus() <= 700 * (num_cus() + groups)) return p;
   const int slots = 2 * num_cus() / (hkv * p.mblocks);  // (one or three a compute unit: within 3 %, either way)
   p.target = std::max({1, slots - batch / 2, slots / 2});
   p.units = p.target + batch;
@@ -1326,6 +1327,7 @@ int run(const char* who, TreeArgs a, int mode, bool fp8, int batch, int hq, size
   if (a.nodes == 1) a.q_sn = a.o_sn = a.kn_sn = a.vn_sn = 0;
   if (a.hkv == 1) a.kn_sh = a.vn_sh = 0;
   if (hq == 1) a.q_sh = a.o_sh = 0;
+  if (a.num_pages == 1) kv_page = a.ss_p = 0;
   if (a.q == nullptr || a.out == nullptr || a.seqlens == nullptr || (a.bt == nullptr && a.max_pages > 0))
     return fail(Q3A_EINVAL, "%s: null pointer", who);
   if (misaligned(a.q, a.q_sb, a.q_sn, a.q_sh) || misaligned(a.out, a.o_sb, a.o_sn, a.o_sh))
