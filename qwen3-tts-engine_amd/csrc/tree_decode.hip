@@ -78,7 +78,7 @@ struct TreeArgs {
   uint32_t per_group;  // m / group = m * per_group >> 20 for m < 4096
   int mblocks;
   int units, target;  // rows, or chunks at most and as many as there should be
-  float per_target;     // 1 / target, a little more
+  float per_target, per_target_one;  // 1 / target, a little more; the same of half as many workgroups
   int xcd_units;
   int order;  // whole rows start in the order of their lengths
   float scale_log2;   // positive
@@ -1010,7 +1010,10 @@ __device__ __forceinline__ uint32_t rounds_of(const TreeArgs& a, int L, int mode
 }
 
 // Chunk `at` of all rows' chunks laid end to end.  64 rows at a time, one a lane; every wave does it.  A chunk has up to `size`
-// rounds: total / target, rounded up, so that a row's 1 + floor(rounds / size) come to target + batch at most.
+// rounds: total / target, rounded up, so that a row's 1 + floor(rounds / size) come to target + batch at most.  The target is two
+// workgroups a compute unit.  One alone has its rounds in 0.6 of the time, and spares the other's start and records, about a round
+// and a half: so it is one where its size is not longer by more than that (8 rows x 4000 tokens 20.4 -> 19.1 us, 1 x 4000 x 64
+// nodes 21.7 -> 17.5; ragged batches mostly need two: 6 long rows x 63 nodes take 79 us with two and 121 with one).
 template <int kW>
 __device__ __forceinline__ Chunk chunk_at(const TreeArgs& a, uint32_t at, int mode) {
   const int lane = lane_now(), batch = a.batch, cap = a.max_pages * a.page_size;
@@ -1025,7 +1028,8 @@ __device__ __forceinline__ Chunk chunk_at(const TreeArgs& a, uint32_t at, int mo
     total += (uint32_t)readlane((int)wave_scan(rounds_of<kW>(a, L, mode)), 63);
   }
   // (The reciprocals are a little large and a little small: neither count may come out too high.)
-  const float size = fmaxf(1.f, floorf((float)total * a.per_target + 0.999f));
+  const float two = fmaxf(1.f, floorf((float)total * a.per_target + 0.999f)), one = floorf((float)total * a.per_target_one + 0.999f);
+  const float size = one <= 1.7f * two + 1.5f ? fmaxf(one, two) : two;
   const float per_size = __builtin_amdgcn_rcpf(size) * 0.999999f;
   uint32_t before = 0;
   for (int b = 0; b < batch; b += 64) {
@@ -1259,7 +1263,7 @@ int tiles_per_wave(int M) { return M <= 16 ? 1 : 2; }
 
 
 struct Plan {
-  int mblocks, units, target;  // target == 0: whole rows
+  int mblocks, units, target, target_one;  // target == 0: whole rows
   size_t rows, bytes;
 };
 
@@ -1276,8 +1280,13 @@ Plan plan_of(int batch, int nodes, int hq, int hkv, int64_t capacity) {
   // of up to 1500 20.0 and 24.4.  Rows that are more than the chip holds at once balance by themselves.
   const int64_t groups = (int64_t)batch * hkv * p.mblocks;
   if (batch > 1024 || capacity * num_cus() <= 700 * (num_cus() + groups)) return p;
-  const int slots = 2 * num_cus() / (hkv * p.mblocks);  // (one or three a compute unit: within 3 %, either way)
-  p.target = std::max({1, slots - batch / 2, slots / 2});
+  // (Three workgroups a compute unit: decode within 3 %, trees of 32 query rows a fifth slower.)
+  auto target = [&](int each) {
+    const int slots = each * num_cus() / (hkv * p.mblocks);
+    return std::max({1, slots - batch / 2, slots / 2});
+  };
+  p.target = target(2);
+  p.target_one = target(1);
   p.units = p.target + batch;
   p.rows = ((size_t)batch * sizeof(Joined) + 15) & ~(size_t)15;
   p.bytes = p.rows + (size_t)p.units * p.mblocks * hkv * 16 * tiles * kRecord * sizeof(float);
@@ -1351,7 +1360,10 @@ int run(const char* who, TreeArgs a, int mode, bool fp8, int batch, int hq, size
   a.mblocks = p.mblocks;
   a.units = p.units;
   a.target = p.target;
-  a.per_target = p.target > 0 ? 1.000001f / (float)p.target : 0.f;
+  if (p.target > 0) {
+    a.per_target = 1.000001f / (float)p.target;
+    a.per_target_one = 1.000001f / (float)p.target_one;
+  }
   a.xcd_units = p.units >= 32;
   a.order = p.target == 0 && (int64_t)batch * a.hkv * p.mblocks > num_cus();
   a.rec = p.target > 0 ? reinterpret_cast<float*>(static_cast<char*>(a.ws) + p.rows) : nullptr;
