@@ -99,4 +99,16 @@ __device__ __forceinline__ uint32_t dpp_max_u32(uint32_t x) {
   return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, false));
 }
 
+// x / d for x < 2^31: with 2^s >= d the multiplier is at most 1 too large, which x carries on by less than 1 / d.
+struct Divisor {
+  uint32_t d, m;
+  int shift;
+};
+__device__ __forceinline__ uint32_t divide(uint32_t x, const Divisor& d) { return (uint32_t)(((uint64_t)x * d.m) >> d.shift); }
+inline Divisor divisor(uint32_t d) {
+  int s = 0;
+  while (((uint64_t)1 << s) < d) ++s;
+  return {d, (uint32_t)(((uint64_t)1 << (31 + s)) / d + 1), 31 + s};
+}
+
 }  // namespace q3a

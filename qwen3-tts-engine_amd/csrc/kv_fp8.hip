@@ -14,18 +14,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kRowsPerBlock = kThreads / 8;
 
-// x / d for x < 2^31: with 2^s >= d the multiplier is at most 1 too large, which x carries on by less than 1 / d.
-struct Divisor {
-  uint32_t d, m;
-  int shift;
-};
-__device__ __forceinline__ uint32_t divide(uint32_t x, const Divisor& d) { return (uint32_t)(((uint64_t)x * d.m) >> d.shift); }
-Divisor divisor(uint32_t d) {
-  int s = 0;
-  while (((uint64_t)1 << s) < d) ++s;
-  return {d, (uint32_t)(((uint64_t)1 << (31 + s)) / d + 1), 31 + s};
-}
-
 struct WriteArgs {
   const uint16_t *k, *v;
   int64_t k_st, k_sh, v_st, v_sh;

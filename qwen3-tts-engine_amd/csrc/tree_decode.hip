@@ -66,6 +66,7 @@ struct TreeArgs {
   uint8_t *ks, *vs;
   int64_t ss_p, ss_h;
   int num_pages, page_size;
+  Divisor per_page;
   const int32_t* seqlens;
   const int32_t* bt;
   int64_t bt_sb;
@@ -75,6 +76,7 @@ struct TreeArgs {
   void* ws;
   float* rec;  // in ws
   int batch, nodes, group, hkv, M;
+  Divisor per_hkv;
   uint32_t per_group;  // m / group = m * per_group >> 20 for m < 4096
   int mblocks;
   int units, target;  // rows, or chunks at most and as many as there should be
@@ -151,24 +153,29 @@ struct Window {
   int valid;         // keys that are seen: 0 past the row's end, and where the table has no page
 };
 
-// Lane l's subtile is half l & 1 of step `step` of row b.  Its table entry (-1 past the table), and, once that has come, its
-// place, given the row's L cached tokens; `on`: there is such a step.
-__device__ __forceinline__ int page_at(int b, int step, int lane) {
+// Lane l's subtile is half l & 1 of step `step` of row b: its first token, that token's place in its page, the table's entry (-1
+// past the table); and, once that has come, where it lies, given the row's L cached tokens.  `on`: there is such a step.
+struct Entry {
+  int tok, off, page;
+};
+__device__ __forceinline__ Entry entry_of(int b, int step, int lane) {
   const TreeArgs& a = args_again();
-  const int pi = (int)((uint32_t)(kStep * step + 16 * (lane & 1)) / (uint32_t)a.page_size);
-  if (a.max_pages == 0) return -1;
+  Entry e = {kStep * step + 16 * (lane & 1), 0, -1};
+  const int pi = (int)divide((uint32_t)e.tok, a.per_page);
+  e.off = e.tok - pi * a.page_size;
+  if (a.max_pages == 0) return e;
   const int page = a.bt[(int64_t)b * a.bt_sb + min(pi, a.max_pages - 1)];
-  return pi < a.max_pages ? page : -1;
+  e.page = pi < a.max_pages ? page : -1;
+  return e;
 }
 template <bool kFp8>
-__device__ __forceinline__ Window window_of(int page, int L, int step, bool on, int lane) {
+__device__ __forceinline__ Window window_of(const Entry& e, int L, bool on) {
   const TreeArgs& a = args_again();
-  const int tok = kStep * step + 16 * (lane & 1), off = (int)((uint32_t)tok % (uint32_t)a.page_size);
   Window w = {0u, 0u, 0};
-  if (on && (unsigned)page < (unsigned)a.num_pages) {
-    w.at = (uint32_t)(((int64_t)page * a.sp + (int64_t)off * a.st) >> 4);
-    if constexpr (kFp8) w.sat = (uint32_t)(page * a.ss_p + off);
-    w.valid = max(0, min(16, L - tok));
+  if (on && (unsigned)e.page < (unsigned)a.num_pages) {
+    w.at = (uint32_t)(((int64_t)e.page * a.sp + (int64_t)e.off * a.st) >> 4);
+    if constexpr (kFp8) w.sat = (uint32_t)(e.page * a.ss_p + e.off);
+    w.valid = max(0, min(16, L - e.tok));
   }
   return w;
 }
@@ -708,7 +715,7 @@ __device__ __forceinline__ void append_keys(const TreeArgs& a, const Work& w, bo
   const TreeArgs& more = args_again();
   const uint16_t* kb = more.kn + (int64_t)w.b * more.kn_sb + (int64_t)w.h * more.kn_sh;
   const uint16_t* vb = more.vn + (int64_t)w.b * more.vn_sb + (int64_t)w.h * more.vn_sh;
-  const int pi = w.L / more.page_size, off = w.L - pi * more.page_size;
+  const int pi = (int)divide((uint32_t)w.L, more.per_page), off = w.L - pi * more.page_size;
   const int page = more.bt[(int64_t)w.b * more.bt_sb + pi];
   const bool ok = (unsigned)page < (unsigned)a.num_pages;
   uint32_t kw[16], vw[4];
@@ -963,16 +970,10 @@ __device__ __forceinline__ TreeArgs at_head(const TreeArgs& a, int h) {
 // turn.  With many units, unit i goes to XCD i % 8 with all its heads, which follow each other there: their exponent bytes
 // share lines, and their rows of a token-major pool share DRAM pages.  With few units the heads go to different XCDs.
 __device__ __forceinline__ void unit_of(const TreeArgs& a, int& h, int& mb, int& unit) {
-  if (a.xcd_units) {
-    const int y = blockIdx.x >> 3;
-    h = y % a.hkv;
-    mb = y / a.hkv;
-    unit = 8 * blockIdx.y + (blockIdx.x & 7);
-  } else {
-    h = blockIdx.x % a.hkv;
-    mb = blockIdx.x / a.hkv;
-    unit = blockIdx.y;
-  }
+  const uint32_t y = a.xcd_units ? blockIdx.x >> 3 : blockIdx.x;
+  mb = (int)divide(y, a.per_hkv);
+  h = (int)y - mb * a.hkv;
+  unit = a.xcd_units ? 8 * blockIdx.y + (blockIdx.x & 7) : blockIdx.y;
 }
 
 // Inclusive sum over the wave's lanes.
@@ -1113,17 +1114,17 @@ __global__ __launch_bounds__(64 * kW, kMT == 2 || (kMode == kTree && kChunked) ?
     if (c.index == 0 && w.h == 0 && w.mb == 0 && threadIdx.x == 0)
       reinterpret_cast<Joined*>(args_again().ws)[w.b] = Joined{unit - c.index, c.count};
     const int s = s0 + wave + kW * (lane >> 1);
-    const int page = page_at(w.b, s, lane);
+    const Entry e = entry_of(w.b, s, lane);
     load_q<kFp8, kMT>(w, raw.v);
-    win = window_of<kFp8>(page, w.L, s, s < min(s1, w.Tc), lane);
+    win = window_of<kFp8>(e, w.L, s < min(s1, w.Tc));
   } else {
     w.b = unit;
     const int row0 = max(0, args.batch - 64 * kW);
     if (args.order && unit >= row0) w.b = kth_longest<kW>(args, row0, unit - row0, wave);
     // The first window's page ids do not wait for the row's length.
-    const int s = wave + kW * (lane >> 1), page = page_at(w.b, s, lane);
+    const Entry e = entry_of(w.b, wave + kW * (lane >> 1), lane);
     load_q<kFp8, kMT>(w, raw.v);
-    win = window_of<kFp8>(page, INT_MAX, s, true, lane);
+    win = window_of<kFp8>(e, INT_MAX, true);
     w.L = __builtin_amdgcn_readfirstlane(row_tokens(w.b, kMode));
     w.Tc = w.L > 0 ? (w.L + kStep - 1) / kStep : 0;
     s1 = steps_of(w.L, kMode);
@@ -1142,8 +1143,8 @@ __global__ __launch_bounds__(64 * kW, kMT == 2 || (kMode == kTree && kChunked) ?
     const int own = first + n * kW;  // and its first own step, taken ahead of them, while they are on their way
     auto place = [&](int j) __attribute__((always_inline)) {
       if ((j & (kWindow - 1)) == 0 && j > 0 && j < n) {
-        const int l = lane_now(), s = first + kW * (j + (l >> 1));
-        win = window_of<kFp8>(page_at(w.b, s, l), w.L, s, j + (l >> 1) < n, l);
+        const int l = lane_now();
+        win = window_of<kFp8>(entry_of(w.b, first + kW * (j + (l >> 1)), l), w.L, j + (l >> 1) < n);
       }
       return place_of<kFp8>(win, j & (kWindow - 1), j < n, w.L - kStep * (first + kW * j));
     };
@@ -1187,72 +1188,69 @@ __global__ __launch_bounds__(64 * kW, kMT == 2 || (kMode == kTree && kChunked) ?
   merge_waves<kMT, kW>(w, st, rec, wave, lds);
 }
 
-// Merges a shared row's records.  16 lanes a query row, 8 dims a lane; the thread groups that the query rows leave share the
-// records.
+// Merges a row's records, for 16 query rows of a head.  16 lanes a query row, 8 dims a lane; the thread groups that the query
+// rows leave share the records.  A chain of two round trips (where the records are, and they), so what can be is worked out ahead
+// of them, without divisions.
 template <int kMT>
 __global__ __launch_bounds__(256) void tree_join_kernel(const TreeArgs a) {
   __shared__ float s_o[16][kD + 4];
   __shared__ float s_m[16], s_l[16];
-  const int h = blockIdx.x % a.hkv, mb = blockIdx.x / a.hkv, b = blockIdx.y;
-  const int tile = 16 * blockIdx.z;  // of the block's query rows
+  const int h = blockIdx.x, b = blockIdx.y, mb = blockIdx.z / kMT, tile = 16 * (blockIdx.z % kMT);
   const Joined d = reinterpret_cast<const Joined*>(a.ws)[b];
-  const int n = d.count;
-  if (n == 1) return;
-  const int rows = min(16, a.M - mb * 16 * kMT - tile);
-  if (rows <= 0) return;
-  const int64_t size = 16 * kMT * kRecord;
+  const int n = d.count, rows = min(16, a.M - mb * 16 * kMT - tile);
+  if (n == 1 || rows <= 0) return;
   const int group = threadIdx.x >> 4, d0 = 8 * (threadIdx.x & 15);
-  const int side = rows > 8 ? 16 : rows > 4 ? 8 : rows > 2 ? 4 : rows;  // query rows at once
-  const int share = 16 / side, mine = group / side;
-  for (int i0 = 0; i0 < rows; i0 += side) {
-    const int i = i0 + group % side;
-    float acc[8] = {}, sum = 0.f, top = -INFINITY;
-    if (i < rows && mine < share) {
+  const int bits = rows > 8 ? 4 : rows > 4 ? 3 : rows > 2 ? 2 : rows - 1;  // 2^bits query rows at once
+  const int share = 16 >> bits, mine = group >> bits, i = group & ((1 << bits) - 1);
+  const int64_t step = (int64_t)a.mblocks * a.hkv * (16 * kMT * kRecord);  // from a chunk's records to the next one's
+  const float* rec = a.rec + d.first * step + ((int64_t)mb * a.hkv + h) * (16 * kMT * kRecord) + (tile + i) * kRecord;
+  const int m = mb * 16 * kMT + tile + i, node = node_of(a, m);
+  uint16_t* out = a.out + b * a.o_sb + node * a.o_sn + (int64_t)(h * a.group + m - node * a.group) * a.o_sh + d0;
+  float acc[8] = {}, sum = 0.f, top = -INFINITY;
+  if (i < rows) {
 #pragma unroll 4
-      for (int c = mine; c < n; c += share) {
-        const float* o = a.rec + (((int64_t)(d.first + c) * a.mblocks + mb) * a.hkv + h) * size + (int64_t)(tile + i) * kRecord;
-        const float2 ml = *reinterpret_cast<const float2*>(o + kD);
-        float e[8];
+    for (int c = mine; c < n; c += share) {
+      const float* o = rec + c * step;
+      const float2 ml = *reinterpret_cast<const float2*>(o + kD);
+      float e[8];
 #pragma unroll
-        for (int k = 0; k < 8; k += 2) {
-          const float2 v = *reinterpret_cast<const float2*>(o + d0 + k);
-          e[k] = v.x;
-          e[k + 1] = v.y;
-        }
-        const float m = fmaxf(top, ml.x), base = m == -INFINITY ? 0.f : m;
-        const float f0 = fast_exp2(top - base), f1 = fast_exp2(ml.x - base);
-        top = m;
-        sum = sum * f0 + ml.y * f1;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) acc[k] = acc[k] * f0 + e[k] * f1;
+      for (int k = 0; k < 8; k += 2) {
+        const float2 v = *reinterpret_cast<const float2*>(o + d0 + k);
+        e[k] = v.x;
+        e[k + 1] = v.y;
       }
+      const float next = fmaxf(top, ml.x), base = next == -INFINITY ? 0.f : next;
+      const float f0 = fast_exp2(top - base), f1 = fast_exp2(ml.x - base);
+      top = next;
+      sum = sum * f0 + ml.y * f1;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) acc[k] = acc[k] * f0 + e[k] * f1;
     }
-    if (share > 1) {  // the same for every thread
-      __syncthreads();
-      if (d0 == 0) {
-        s_m[group] = top;
-        s_l[group] = sum;
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) s_o[group][d0 + k] = acc[k];
-      __syncthreads();
-      if (mine == 0) {
-        float all = -INFINITY;
-        for (int c = 0; c < share; ++c) all = fmaxf(all, s_m[c * side + group]);
-        const float base = all == -INFINITY ? 0.f : all;
-        sum = 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) acc[k] = 0.f;
-        for (int c = 0; c < share; ++c) {
-          const float f = fast_exp2(s_m[c * side + group] - base);
-          sum += f * s_l[c * side + group];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) acc[k] += f * s_o[c * side + group][d0 + k];
-        }
-      }
-    }
-    if (mine == 0 && i < rows) store_out(out_row(b, h, mb * 16 * kMT + tile + i) + d0, acc, sum);
   }
+  if (share > 1) {  // the same for every thread
+    if (d0 == 0) {
+      s_m[group] = top;
+      s_l[group] = sum;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s_o[group][d0 + k] = acc[k];
+    __syncthreads();
+    if (mine == 0) {
+      float all = -INFINITY;
+      for (int c = 0; c < share; ++c) all = fmaxf(all, s_m[(c << bits) + i]);
+      const float base = all == -INFINITY ? 0.f : all;
+      sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) acc[k] = 0.f;
+      for (int c = 0; c < share; ++c) {
+        const float f = fast_exp2(s_m[(c << bits) + i] - base);
+        sum += f * s_l[(c << bits) + i];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] += f * s_o[(c << bits) + i][d0 + k];
+      }
+    }
+  }
+  if (mine == 0 && i < rows) store_out(out, acc, sum);
 }
 
 // ---------------------------------------------------------------------------------------------------- host side
@@ -1305,7 +1303,7 @@ int launch(const TreeArgs& a, const char* who, hipStream_t stream) {
     hipLaunchKernelGGL((tree_kernel<kFp8, kMode, kMT, kWaves, true>), grid, dim3(64 * kWaves), 0, stream, a);
     e = hipGetLastError();
     if (e == hipSuccess) {
-      hipLaunchKernelGGL((tree_join_kernel<kMT>), dim3(heads, (unsigned)a.batch, kMT), dim3(256), 0, stream, a);
+      hipLaunchKernelGGL((tree_join_kernel<kMT>), dim3(a.hkv, (unsigned)a.batch, a.mblocks * kMT), dim3(256), 0, stream, a);
       e = hipGetLastError();
     }
   }
@@ -1357,6 +1355,8 @@ int run(const char* who, TreeArgs a, int mode, bool fp8, int batch, int hq, size
     return fail(Q3A_ESPACE, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", who, workspace_bytes, p.bytes);
   a.batch = batch;
   a.per_group = ((1u << 20) + a.group - 1) / a.group;
+  a.per_page = divisor((uint32_t)a.page_size);
+  a.per_hkv = divisor((uint32_t)a.hkv);
   a.mblocks = p.mblocks;
   a.units = p.units;
   a.target = p.target;
