@@ -1,7 +1,7 @@
 // The 8-bit K/V pool's write and read (gfx950).  The row format is fp8_common.h's.
 //
 // Both are one pass over their bytes, bound by HBM: a write reads 512 and writes 258 bytes a row pair (64 x 1700 tokens of 8
-// heads in 136.7 us, 4.9 TB/s, as fast as a large copy), a read the reverse (32 x 1100 tokens in 47.4 us, 4.6 TB/s).  8 lanes
+// heads in 133.7 us, 5.0 TB/s, as fast as a large copy), a read the reverse (32 x 1100 tokens in 47.7 us, 4.6 TB/s).  8 lanes
 // share a row: 32 B of bf16 and 16 B of codes a lane, so a row of codes is one 128 B line, a row of bf16 two, and the row's
 // maximum is 3 DPP steps.  Non-temporal loads changed nothing, non-temporal stores of what is read took 82 us instead of 47,
 // several rows a lane were 2 to 12 % slower.
