@@ -83,7 +83,7 @@ struct TreeArgs {
   float per_target, per_target_one;  // 1 / target, a little more; the same of half as many workgroups
   int xcd_units;
   int order;  // whole rows start in the order of their lengths
-  float scale_log2;   // positive
+  float scale_log2, ahead;  // positive; kAhead / scale_log2, as far as a score may be added to it
   uint32_t q_sign;    // turns the signs of a pair of bf16, or nothing
 };
 
@@ -466,14 +466,15 @@ __device__ __forceinline__ float larger(float a, float b) { return __builtin_ele
 // The scores to probabilities: scaled, masked, exp2 of them minus a base, which with the sum is updated and O rescaled to.
 // kMasked: seen[t] tells which of the lane's 8 keys (bit 4 u + i) its query row sees; else the subtiles' valid ones.
 //
-// The base need not be the maximum, only near it: it moves when some query row's probabilities have outgrown 2^kAhead, which
-// after a row's first steps hardly happens, while with 16 or 32 query rows some row's maximum grows in almost every step, and
-// rescaling is a sixth to a quarter of a step's vector instructions (6 rows x 63 nodes: 82.7 us with kAhead = 0, 80.2 with 4, 79.3
-// with 6).  O and l hold up to 2^kAhead times as much for it.
+// The base need not be the maximum, only near it and not below: where some query row's scores have outgrown it, it is set to
+// their maximum and 2^kAhead more (a.ahead, in unscaled scores), which after a row's first steps hardly happens again, while with
+// 16 or 32 query rows some row's maximum grows in almost every step, and rescaling is a sixth to a quarter of a step's vector
+// instructions (6 rows x 63 nodes: 82.7 us with kAhead = 0, 80.2 with 4, 79.3 with 6).  No probability passes 1 for it, so that a
+// product with the largest V stays finite.
 constexpr float kAhead = 4.f;
 
 template <bool kMasked, int kMT>
-__device__ __forceinline__ void softmax(const int (&valid)[2], const uint32_t (&seen)[kMT], float scale,
+__device__ __forceinline__ void softmax(const int (&valid)[2], const uint32_t (&seen)[kMT], float scale, float ahead,
                                         f32x4_t (&s)[kMT][2], State<kMT>& st) {
   const bool full = valid[0] == 16 && valid[1] == 16;
   if (kMasked || !full) {
@@ -495,12 +496,12 @@ __device__ __forceinline__ void softmax(const int (&valid)[2], const uint32_t (&
     top[t] = larger(larger(larger(s[t][0][0], s[t][0][1]), larger(s[t][0][2], s[t][0][3])),
                     larger(larger(s[t][1][0], s[t][1][1]), larger(s[t][1][2], s[t][1][3])));
     top[t] = max_xor32(max_xor16(top[t]));
-    grown = grown | ((top[t] - st.m[t]) * scale > kAhead);
+    grown = grown | (top[t] > st.m[t]);
   }
   if (__builtin_amdgcn_ballot_w64(grown) != 0) {
 #pragma unroll
     for (int t = 0; t < kMT; ++t) {
-      const float m = larger(st.m[t], top[t]);
+      const float m = top[t] > st.m[t] ? top[t] + ahead : st.m[t];
       const float alpha = fast_exp2((st.m[t] - (m == -INFINITY ? 0.f : m)) * scale);
       st.m[t] = m;
       st.l[t] *= alpha;
@@ -684,7 +685,7 @@ __device__ __forceinline__ void tree_step(const Work& w, int ts, const Query<fal
   const int any[2] = {16, 16};
   f32x4_t sc[kMT][2];
   scores<false, kMT>(x, q, sc);
-  softmax<true, kMT>(any, seen, a.scale_log2, sc, st);
+  softmax<true, kMT>(any, seen, a.scale_log2, a.ahead, sc, st);
   uint32_t top = 0;
 #pragma unroll
   for (int u = 0; u < 2; ++u)
@@ -835,7 +836,7 @@ struct Stream {
     __builtin_amdgcn_sched_barrier(0);
     load_k<kOnce>(a, next, lane, k);
     __builtin_amdgcn_sched_barrier(0);
-    softmax<false, kMT>(valid, all, a.scale_log2, s, st);
+    softmax<false, kMT>(valid, all, a.scale_log2, a.ahead, s, st);
     values<kFp8, kMT>(v, valid, lane, s, st);
     __builtin_amdgcn_sched_barrier(0);
     load_v<kFp8, kOnce>(a, next, lane, v);
@@ -855,7 +856,7 @@ __device__ __forceinline__ void append_step(const TreeArgs& a, const Work& w, co
   int one[2] = {0, 0};
   append_keys(a, w, w.mb == 0, x, y, one[0]);
   scores<false, kMT>(x, q, s);
-  softmax<false, kMT>(one, all, a.scale_log2, s, st);
+  softmax<false, kMT>(one, all, a.scale_log2, a.ahead, s, st);
   values<true, kMT>(y, one, lane, s, st);
 }
 
@@ -1374,6 +1375,7 @@ int run(const char* who, TreeArgs a, int mode, bool fp8, int batch, int hq, size
   // which masked scores of -inf would be NaN, becomes the smallest there is.
   a.q_sign = softmax_scale < 0.f ? 0x80008000u : 0u;
   a.scale_log2 = softmax_scale == 0.f ? FLT_MIN : fabsf(softmax_scale) * kLog2e;
+  a.ahead = std::min(kAhead / a.scale_log2, 1e30f);
   const hipStream_t s = (hipStream_t)stream;
   if (mode == kNoKeys) return launch<true, kNoKeys, 1>(a, who, s);
   if (mode == kAppend) return launch<true, kAppend, 1>(a, who, s);

@@ -239,3 +239,31 @@ def test_a_row_gets_the_same_bits_whatever_the_batch_holds(cuda_device):
     p = torch.randperm(120, generator=torch.Generator().manual_seed(2))
     b = q3attn.paged_decode_fp8(*args(p))
     assert torch.equal(b, a[p.to(cuda_device)])
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("late", [2.0, 7.0])
+def test_values_near_the_largest_number(cuda_device, fp8, late):
+    """One key of a value near bf16's largest, whose score is over all those before it: its probability's share is a number, and
+    so is everything on the way to it.  (Keys 0 to 31 and 128 to 159 are one wave's steps.)"""
+    page, n, at = 16, 170, 140
+    k, v = torch.zeros((n, 1, D)), torch.zeros((n, 1, D))
+    k[at, 0, 0], v[at, 0, ::2], v[at, 0, 1::2] = 1.0, 3e38, -3e38
+    k, v = (torch.nn.functional.pad(x, (0, 0, 0, 0, 0, 176 - n)).to(torch.bfloat16).to(cuda_device) for x in (k, v))
+    slots = torch.arange(176, device=cuda_device)
+    if fp8:
+        pool = q3attn.fp8_cache(11, page, 1)
+        q3attn.paged_write_fp8(k, v, slots, *pool)
+    else:
+        pool = (k.view(11, page, 1, D), v.view(11, page, 1, D), None, None)
+    table, lens = torch.arange(11, dtype=torch.int32)[None], torch.tensor([n], dtype=torch.int32)
+    q = torch.zeros((1, 1, 2, D), dtype=torch.bfloat16)
+    q[..., 0] = late * 128 ** 0.5
+    own = torch.zeros((1, 1, 1, D), dtype=torch.bfloat16)
+    mask = torch.zeros((1, 1, 1), dtype=torch.bool)
+    want, spread = attention(q, pool_values(pool[0], pool[2]), pool_values(pool[1], pool[3]), lens, table, SCALE, (own, own, mask))
+    assert torch.isfinite(want).all()
+    assert_close(run_tree(cuda_device, pool, table, lens, q, own, own, mask), want, spread)
+    if fp8:
+        out = q3attn.paged_decode_fp8(q[:, 0].to(cuda_device), *pool, lens.to(cuda_device), table.to(cuda_device), SCALE)
+        assert_close(out, want[:, 0], spread[:, 0])
