@@ -645,18 +645,15 @@ __device__ __forceinline__ void tree_step(const Work& w, int ts, const Query<fal
 #pragma unroll
     for (int c = 0; c < 4; ++c) x.k[u][c] = ld16(kb + (int64_t)j * a.kn_sn + dim_of<kFp8>(c, g));
   }
-  auto load_values = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+  for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = kStep * ts + 16 * u + 4 * g + i;
-        const uint4 e = ld16(vb + (int64_t)min(j, a.nodes - 1) * a.vn_sn + 8 * r);
-        const uint32_t keep = j < a.nodes ? ~0u : 0u;
-        y.v[u][i] = make_uint4(e.x & keep, e.y & keep, e.z & keep, e.w & keep);
-      }
-  };
-  load_values();
+    for (int i = 0; i < 4; ++i) {
+      const int j = kStep * ts + 16 * u + 4 * g + i;
+      const uint4 e = ld16(vb + (int64_t)min(j, a.nodes - 1) * a.vn_sn + 8 * r);
+      const uint32_t keep = j < a.nodes ? ~0u : 0u;
+      y.v[u][i] = make_uint4(e.x & keep, e.y & keep, e.z & keep, e.w & keep);
+    }
   uint32_t seen[kMT];
 #pragma unroll
   for (int t = 0; t < kMT; ++t) {
@@ -691,11 +688,10 @@ __device__ __forceinline__ void tree_step(const Work& w, int ts, const Query<fal
   for (int u = 0; u < 2; ++u)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint4 e = y.v[u][i];
-      top = pk_max_u16(top, pk_max_u16(pk_max_u16(e.x & 0x7fff7fffu, e.y & 0x7fff7fffu), pk_max_u16(e.z & 0x7fff7fffu, e.w & 0x7fff7fffu)));
+      const uint32_t w4[4] = {y.v[u][i].x, y.v[u][i].y, y.v[u][i].z, y.v[u][i].w};
+      top = pk_max_u16(top, bf16_any_amax_pair(w4));
     }
-  const bool odd = halves_max(top) >= 0x7f80u;
-  const bool any_odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+  const bool any_odd = __builtin_amdgcn_ballot_w64(halves_max(top) >= 0x7f80u) != 0;
   if (any_odd) {
 #pragma unroll
     for (int u = 0; u < 2; ++u)
