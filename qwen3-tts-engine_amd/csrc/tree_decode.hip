@@ -1280,6 +1280,7 @@ Plan plan_of(int batch, int nodes, int hq, int hkv, int64_t capacity) {
     const int slots = each * num_cus() / (hkv * p.mblocks);
     return std::max({1, slots - batch / 2, slots / 2});
   };
+  if (target(2) < 2) return p;  // a single row's heads and nodes fill the chip, or nearly
   p.target = target(2);
   p.target_one = target(1);
   p.units = p.target + batch;
@@ -1362,7 +1363,7 @@ int run(const char* who, TreeArgs a, int mode, bool fp8, int batch, int hq, size
     a.per_target_one = 1.000001f / (float)p.target_one;
   }
   a.xcd_units = p.units >= 32;
-  a.order = p.target == 0 && (int64_t)batch * a.hkv * p.mblocks > num_cus();
+  a.order = p.target == 0 && batch > 1 && (int64_t)batch * a.hkv * p.mblocks > num_cus();
   a.rec = p.target > 0 ? reinterpret_cast<float*>(static_cast<char*>(a.ws) + p.rows) : nullptr;
   a.sp = kv_page * elem;
   a.st = (int)(kv_tok * elem);

@@ -36,3 +36,8 @@ def test_workspace_is_bounded(batch, heads, tokens):
     """Chunks are as many as the compute units hold, and one a row more: at most 512 (or a row each) of 16 query rows a head."""
     need = _lib.lib().q3a_paged_decode_tree_workspace_bytes(batch, 1, heads, heads, 128, tokens // 16, 16)
     assert need <= 8 * batch + 16 + (512 + batch * heads) * 16 * 130 * 4
+
+
+def test_no_workspace_where_one_rows_query_rows_fill_the_chip():
+    for batch, nodes, hq, hkv in ((1, 256, 1024, 64), (3, 64, 256, 16), (1024, 256, 1024, 64)):
+        assert _lib.lib().q3a_paged_decode_tree_workspace_bytes(batch, nodes, hq, hkv, 128, 1 << 20, 16) == 0

@@ -267,3 +267,15 @@ def test_values_near_the_largest_number(cuda_device, fp8, late):
     if fp8:
         out = q3attn.paged_decode_fp8(q[:, 0].to(cuda_device), *pool, lens.to(cuda_device), table.to(cuda_device), SCALE)
         assert_close(out, want[:, 0], spread[:, 0])
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+def test_long_rows_whose_query_rows_fill_the_chip(cuda_device, fp8):
+    """64 nodes of 256 heads over 16 KV heads: 512 workgroups a row, so its steps stay together however long it is."""
+    pool, table, lens, q, k, v = tree_case(cuda_device, [1500], 64, 16, 16, 16, fp8, True, 30, width=4096)
+    mask = _tree_masks(1, 64, 31)
+    out = run_tree(cuda_device, pool, table, lens, q, k, v, mask)
+    nodes = [0, 31, 63]
+    want, spread = attention(q[:, nodes], pool_values(pool[0], pool[2]), pool_values(pool[1], pool[3]), lens, table, SCALE,
+                             (k, v, mask[:, nodes]))
+    assert_close(out[:, nodes], want, spread)
