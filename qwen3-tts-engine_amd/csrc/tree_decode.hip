@@ -566,9 +566,6 @@ __device__ __forceinline__ void values(const ValueTile<kFp8>& x, const int (&val
   }
 }
 
-__device__ __forceinline__ bool not_finite_pair(uint32_t w) {
-  return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
-}
 // The pair with its halves that are not finite set to zero.
 __device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
   if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
