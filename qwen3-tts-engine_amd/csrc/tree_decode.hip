@@ -21,8 +21,7 @@
 //                 whose P its S^T registers hold, so P needs no lane moves.  Row i of MFMA j stands for dim 8 i + j: the
 //                 lane loads 8 dims in a row of its 8 keys, and the transpose is byte permutes within the lane.
 // Lane l of O^T then holds 32 dims in a row of query row l % 16.  V's scale goes onto P.  Scores, statistics and O are fp32; P
-// is rounded to bf16 for the product (2^-8 of each term at worst, the sum l is of the unrounded ones), as the prefill kernel
-// does.
+// goes into the product as two bf16 numbers, which leave 2^-15 of each term at worst.
 #include <float.h>
 #include <limits.h>
 #include <math.h>
@@ -522,7 +521,14 @@ __device__ __forceinline__ void softmax(const int (&valid)[2], const uint32_t (&
   }
 }
 
-// O^T += V^T P^T.
+// O^T += V^T P^T, with each probability as the sum of two bf16 numbers.
+//
+// One bf16 number holds 8 of its significant bits, and only a row's largest one is a power of two: over eight calls the results were
+// off by 0.0018 to 0.0023 of their norm instead of the 0.0017 that their own rounding to bf16 takes.  Two hold 16 bits (2^-16 of
+// each probability is left) and reach the 0.0017.  The second product takes nothing where HBM is the bound, 3.6 % of 32 rows
+// x 13 nodes (17.9 -> 18.6 us) and 6.7 % of 6 long rows x 63 nodes (73.3 -> 78.2), which vector instructions bound.
+// Over the 8-bit pool the first part is rounded to nearest.  Over bf16, whose V may hold infinities, both parts of a probability
+// over 0 have to be over 0, that no product of 0 and an infinity makes a NaN: the first is cut off from the next smaller number.
 template <bool kFp8, int kMT>
 __device__ __forceinline__ void values(const ValueTile<kFp8>& x, const int (&valid)[2], int lane, const f32x4_t (&p)[kMT][2],
                                        State<kMT>& st) {
@@ -542,17 +548,28 @@ __device__ __forceinline__ void values(const ValueTile<kFp8>& x, const int (&val
 #pragma unroll
       for (int i = 0; i < 4; ++i) f[u][i] = fp8_scale((bytes[u] >> (8 * i)) & 0xffu);
   }
-  bf16x8_t pb[kMT];
+  bf16x8_t hi[kMT], lo[kMT];
 #pragma unroll
   for (int t = 0; t < kMT; ++t) {
-    uint32_t pk[4];
+    uint32_t h[4], r[4];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      auto scaled = [&](int i) { return kFp8 ? p[t][u][i] * f[u][i] : p[t][u][i]; };
-      pk[2 * u] = pack_bf16x2(scaled(0), scaled(1));
-      pk[2 * u + 1] = pack_bf16x2(scaled(2), scaled(3));
-    }
-    pb[t] = __builtin_bit_cast(bf16x8_t, make_uint4(pk[0], pk[1], pk[2], pk[3]));
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        const float a = kFp8 ? p[t][u][i] * f[u][i] : p[t][u][i], b = kFp8 ? p[t][u][i + 1] * f[u][i + 1] : p[t][u][i + 1];
+        const int w = 2 * u + (i >> 1);
+        if constexpr (kFp8) {
+          h[w] = pack_bf16x2(a, b);
+          r[w] = pack_bf16x2(a - bf16_lo(h[w]), b - bf16_hi(h[w]));
+        } else {
+          const uint32_t ah = __builtin_elementwise_sub_sat(__float_as_uint(a), 1u);
+          const uint32_t bh = __builtin_elementwise_sub_sat(__float_as_uint(b), 1u);
+          h[w] = perm_b32(bh, ah, kPermHiHi);
+          r[w] = pack_bf16x2(a - bf16_hi(ah), b - bf16_hi(bh));
+        }
+      }
+    hi[t] = __builtin_bit_cast(bf16x8_t, make_uint4(h[0], h[1], h[2], h[3]));
+    lo[t] = __builtin_bit_cast(bf16x8_t, make_uint4(r[0], r[1], r[2], r[3]));
   }
 #pragma unroll
   for (int jj = 0; jj < 8; jj += 2) {
@@ -560,8 +577,10 @@ __device__ __forceinline__ void values(const ValueTile<kFp8>& x, const int (&val
     v_operands(x, jj, a0, a1);
 #pragma unroll
     for (int t = 0; t < kMT; ++t) {
-      st.o[t][jj] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, pb[t], st.o[t][jj], 0, 0, 0);
-      st.o[t][jj + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, pb[t], st.o[t][jj + 1], 0, 0, 0);
+      st.o[t][jj] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, lo[t], st.o[t][jj], 0, 0, 0);
+      st.o[t][jj + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, lo[t], st.o[t][jj + 1], 0, 0, 0);
+      st.o[t][jj] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, hi[t], st.o[t][jj], 0, 0, 0);
+      st.o[t][jj + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, hi[t], st.o[t][jj + 1], 0, 0, 0);
     }
   }
 }
