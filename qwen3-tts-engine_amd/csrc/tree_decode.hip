@@ -340,8 +340,14 @@ __device__ __forceinline__ void v_operands(const ValueTile<false>& x, int jj, bf
 //
 // The matrix instruction takes K's codes and its power-of-two scale (one byte a key) as they are, with Q as hi + lo: of q's 8
 // significant bits hi = e4m3(q / 2^e) holds the upper 4 and lo = e4m3(16 (q / 2^e - hi)) at 2^(e - 4) the rest.  That is q
-// itself down to 2^-14 of its row's largest element and 2^-22 of that element below, so the scores are those of the bf16 row,
-// and a step's two products (K = 128 each) replace 32 conversions and 8 products in bf16.
+// itself down to 2^(e - 6), where e4m3 stops being a floating-point format, 2^-14 of its row's largest element.  So the scores are
+// those of the bf16 row, and a step's two products (K = 128 each) replace 32 conversions and 8 products in bf16.
+//
+// Smaller elements would be held to 2^-22 of the largest only.  That is nothing beside the largest one's share of a score, unless K is
+// small where q is large: with q = (2^22, 1, ..) and keys (0, k1, ..) k1 would not count.  So where a wave's query rows have
+// such an element, other than 0, its steps take Q in bf16 and convert K (2.4 times the cycles; a quarter of the waves do with 16 rows
+// of normalised queries, half with 32: 32 rows x 13 nodes 18.6 -> 19.2 us, 6 long rows x 63 nodes 79.7 -> 83.6).  Asking whether
+// the parts hold all the same what is smaller but short, which a third of those would pass, took as long or longer.
 template <bool kFp8, int kMT>
 struct Query;
 template <int kMT>
@@ -350,8 +356,9 @@ struct Query<false, kMT> {
 };
 template <int kMT>
 struct Query<true, kMT> {
-  i32x8_t hi[kMT], lo[kMT];
-  int s[kMT];  // the exponent byte of hi; lo's is 4 less
+  i32x8_t hi[kMT], lo[kMT];  // two parts, or the four bf16 operands as they are loaded
+  int s[kMT];                // the exponent byte of hi; lo's is 4 less
+  bool parts;                // the same for the wave
 };
 
 // The largest over the four lanes of a query row (small integers order as floats do).
@@ -367,29 +374,48 @@ __device__ __forceinline__ void prepare(const bf16x8_t (&q)[kMT][4], Query<false
 }
 template <int kMT>
 __device__ __forceinline__ void prepare(const bf16x8_t (&q)[kMT][4], Query<true, kMT>& x) {
+  bool fine = false;  // some element may be too small for the parts
+  uint32_t w[kMT][16], sb[kMT];
+  bool rare[kMT];
 #pragma unroll
   for (int t = 0; t < kMT; ++t) {
-    uint32_t w[16];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const uint4 e = __builtin_bit_cast(uint4, q[t][c]);
-      w[4 * c] = e.x;
-      w[4 * c + 1] = e.y;
-      w[4 * c + 2] = e.z;
-      w[4 * c + 3] = e.w;
+      w[t][4 * c] = e.x;
+      w[t][4 * c + 1] = e.y;
+      w[t][4 * c + 2] = e.z;
+      w[t][4 * c + 3] = e.w;
     }
-    uint32_t top = row_max(halves_max(bf16_any_amax_pair(w)));
-    const bool rare = any_rare(top);
-    if (rare) top = row_max(halves_max(bf16_amax_pair(w)));
-    const uint32_t sb = fp8_scale_byte(top);
-    const float scale = fp8_scale(sb);
-    x.s[t] = (int)sb;
+    uint32_t top = row_max(halves_max(bf16_any_amax_pair(w[t])));
+    rare[t] = any_rare(top);
+    if (rare[t]) top = row_max(halves_max(bf16_amax_pair(w[t])));
+    sb[t] = fp8_scale_byte(top);
+    fine = fine | (bf16_amin_less1(w[t]) < ((sb[t] - 6) << 7) - 1);
+  }
+  x.parts = __builtin_amdgcn_ballot_w64(fine) == 0;
+  if (!x.parts) {
+#pragma unroll
+    for (int t = 0; t < kMT; ++t) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x.hi[t][i] = (int)nan_if_not_finite(w[t][i]);
+        x.lo[t][i] = (int)nan_if_not_finite(w[t][8 + i]);
+      }
+      x.s[t] = 0;
+    }
+    return;
+  }
+#pragma unroll
+  for (int t = 0; t < kMT; ++t) {
+    const float scale = fp8_scale(sb[t]);
+    x.s[t] = (int)sb[t];
     uint32_t hi[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) hi[i] = fp8_finite_codes4(w[2 * i], w[2 * i + 1], scale);
-    if (rare) {
+    for (int i = 0; i < 8; ++i) hi[i] = fp8_finite_codes4(w[t][2 * i], w[t][2 * i + 1], scale);
+    if (rare[t]) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) hi[i] = fp8_codes4(w[2 * i], w[2 * i + 1], sb);
+      for (int i = 0; i < 8; ++i) hi[i] = fp8_codes4(w[t][2 * i], w[t][2 * i + 1], sb[t]);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -397,8 +423,9 @@ __device__ __forceinline__ void prepare(const bf16x8_t (&q)[kMT][4], Query<true,
       s16x2 lo = {0, 0};
       const f32x2_t h0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi[i], scale, false);
       const f32x2_t h1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi[i], scale, true);
-      lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, bf16_lo(w[2 * i]) - h0[0], bf16_hi(w[2 * i]) - h0[1], scale * 0.0625f, false);
-      lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, bf16_lo(w[2 * i + 1]) - h1[0], bf16_hi(w[2 * i + 1]) - h1[1], scale * 0.0625f, true);
+      const uint32_t a = w[t][2 * i], b = w[t][2 * i + 1];
+      lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, bf16_lo(a) - h0[0], bf16_hi(a) - h0[1], scale * 0.0625f, false);
+      lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, bf16_lo(b) - h1[0], bf16_hi(b) - h1[1], scale * 0.0625f, true);
       x.hi[t][i] = (int)hi[i];
       x.lo[t][i] = __builtin_bit_cast(int, lo);
     }
@@ -421,11 +448,28 @@ __device__ __forceinline__ void scores(const KeyTile<true>& x, const Query<true,
         k[i] = odd ? odd_gets : k[i];
       }
     }
+    const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+    if (q.parts) {
 #pragma unroll
-    for (int t = 0; t < kMT; ++t) {
-      const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
-      s[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q.lo[t], zero, 0, 0, 0, (int)x.ks[u], 0, q.s[t] - 4);
-      s[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q.hi[t], s[t][u], 0, 0, 0, (int)x.ks[u], 0, q.s[t]);
+      for (int t = 0; t < kMT; ++t) {
+        s[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q.lo[t], zero, 0, 0, 0, (int)x.ks[u], 0, q.s[t] - 4);
+        s[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q.hi[t], s[t][u], 0, 0, 0, (int)x.ks[u], 0, q.s[t]);
+      }
+    } else {
+      const float f = fp8_scale(x.ks[u]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const uint32_t a = (uint32_t)k[2 * c], b = (uint32_t)k[2 * c + 1];
+        const bf16x8_t kf = __builtin_bit_cast(
+            bf16x8_t, make_uint4(fp8_pair<false>(a, f), fp8_pair<true>(a, f), fp8_pair<false>(b, f), fp8_pair<true>(b, f)));
+#pragma unroll
+        for (int t = 0; t < kMT; ++t) {
+          const i32x8_t& half = c < 2 ? q.hi[t] : q.lo[t];
+          const int i = 4 * (c & 1);
+          const i32x4_t qf = {half[i], half[i + 1], half[i + 2], half[i + 3]};
+          s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, __builtin_bit_cast(bf16x8_t, qf), c == 0 ? zero : s[t][u], 0, 0, 0);
+        }
+      }
     }
   }
 }

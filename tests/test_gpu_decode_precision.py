@@ -107,3 +107,36 @@ def test_infinite_cached_values(cuda_device, nodes):
     assert torch.isnan(out[..., 9]).all()
     rest = [d for d in range(D) if d not in (3, 5, 7, 9)]
     assert torch.isfinite(out[..., rest]).all()
+
+
+@pytest.mark.parametrize("large", [2.0 ** 12, 2.0 ** 17, 2.0 ** 24, 3.0e38])
+@pytest.mark.parametrize("nodes,hkv,group", [(1, 2, 2), (3, 1, 4), (30, 1, 2)])
+def test_small_query_elements_beside_large_ones(cuda_device, nodes, hkv, group, large):
+    """Queries whose first element is far larger than the others, over keys that are 0 there: the others are the score.  Only some
+    heads have it, and one has elements of every size."""
+    g = torch.Generator().manual_seed(nodes)
+    lens = torch.tensor(LENS, dtype=torch.int32)
+    used = sum(-(-n // 16) for n in LENS)
+    kv = torch.randn((2, used * 16, hkv, D), generator=g).to(torch.bfloat16)
+    kv[0, ..., 0] = 0
+    pool = q3attn.fp8_cache(used, 16, hkv, device=cuda_device)
+    q3attn.paged_write_fp8(kv[0].to(cuda_device), kv[1].to(cuda_device), torch.arange(used * 16, device=cuda_device), *pool)
+    table = table_for(LENS, 16, used, -(-max(LENS) // 16), nodes)
+    q = (0.2 * torch.randn((len(LENS), nodes, hkv * group, D), generator=g)).to(torch.bfloat16)
+    q[:, ::2, 0, 0] = large
+    q[1::2, :, -1, 0] = -large
+    q[2, 0, -1] *= torch.exp2(-torch.arange(D) / 4.0).to(torch.bfloat16)
+    k, v = (torch.randn((len(LENS), nodes, hkv, D), generator=g).to(torch.bfloat16) for _ in range(2))
+    k[..., 0] = 0
+    mask = _tree_masks(len(LENS), nodes, nodes)
+    vals = pool_values(pool[0], pool[2]), pool_values(pool[1], pool[3])
+    want, spread = attention(q, *vals, lens, table, SCALE, (k, v, mask))
+    _assert_precise(_tree(cuda_device, pool, table, lens, q, k, v, mask), want, spread)
+    want, spread = attention(q[:, :1], *vals, lens, table, SCALE)
+    args = lens.to(cuda_device), table.to(cuda_device), SCALE
+    _assert_precise(q3attn.paged_decode_fp8(q[:, 0].to(cuda_device), *pool, *args), want[:, 0], spread[:, 0])
+    now = torch.tensor([n - 1 for n in LENS], dtype=torch.int32)    # the last token again, as the step's own
+    last = [int(table[b, (n - 1) // 16]) * 16 + (n - 1) % 16 for b, n in enumerate(LENS)]
+    out = q3attn.paged_decode_fp8_append(q[:, 0].to(cuda_device), kv[0, last].to(cuda_device), kv[1, last].to(cuda_device), *pool,
+                                         now.to(cuda_device), *args[1:])
+    _assert_precise(out, want[:, 0], spread[:, 0])
