@@ -250,20 +250,35 @@ def check(rc: int, what: str) -> None:
         raise Q3AttnError(f"{what} failed ({rc}): {msg}")
 
 
-def torch_ops(*names: str):
-    """The ops ``q3attn::name`` that libq3torch.so registers; without the built libraries, functions that raise."""
-    if os.path.exists(LIB_PATH) and os.path.exists(TORCH_LIB_PATH):
-        lib()
-        torch.ops.load_library(TORCH_LIB_PATH)
-        return [getattr(torch.ops.q3attn, name).default for name in names]
-
-    def missing(*args, **kwargs):
-        raise Q3AttnError(f"q3attn: {LIB_PATH} or {TORCH_LIB_PATH} was not built when q3attn was imported; build them first "
-                          "(python qwen3-tts-engine_amd/build.py or __graft_entry__.build())")
-    return [missing] * len(names)
+def _bind(name: str, fake):
+    lib()
+    if not os.path.exists(TORCH_LIB_PATH):
+        raise Q3AttnError(f"torch ops not found at {TORCH_LIB_PATH}")
+    torch.ops.load_library(TORCH_LIB_PATH)
+    op = getattr(torch.ops.q3attn, name).default
+    torch.library.register_fake(f"q3attn::{name}", fake, allow_override=True)
+    return op
 
 
-def register_fake(op, fn) -> None:
-    """fn as ``op``'s implementation on fake tensors (shapes only), if the op is there."""
-    if isinstance(op, torch._ops.OpOverload):
-        torch.library.register_fake(op._schema.name, fn)
+def torch_op(name: str, fake):
+    """The op ``q3attn::name`` that libq3torch.so registers, with ``fake`` as its implementation on fake tensors (shapes only).
+
+    Nothing else of the package needs that library, which is bound to the torch it was built against.  Where it cannot be loaded
+    (not built yet, built for another torch, beside a libq3attn.so of another ABI), this is a function that tries again when it is
+    called and raises the reason if it still cannot."""
+    unavailable = (OSError, RuntimeError, AttributeError)
+    try:
+        return _bind(name, fake)
+    except unavailable:
+        pass
+    bound = []
+
+    def late(*args, **kwargs):
+        if not bound:
+            try:
+                bound.append(_bind(name, fake))
+            except unavailable as e:
+                raise Q3AttnError(f"q3attn.{name} needs {TORCH_LIB_PATH}, which cannot be loaded: {e}; build it for this torch "
+                                  "(python qwen3-tts-engine_amd/build.py or __graft_entry__.build())") from e
+        return bound[0](*args, **kwargs)
+    return late

@@ -13,12 +13,20 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import register_fake, torch_ops
+from ._lib import torch_op
 
 E4M3 = torch.float8_e4m3fn
 
-_write, _read, _decode, _decode_append = torch_ops("paged_write_fp8", "paged_read_fp8", "paged_decode_fp8",
-                                                   "paged_decode_fp8_append")
+
+def _read_fake(k_cache, v_cache, k_scale, v_scale, slots):
+    shape = (slots.shape[0], k_cache.shape[2], k_cache.shape[3])
+    return (k_cache.new_empty(shape, dtype=torch.bfloat16), k_cache.new_empty(shape, dtype=torch.bfloat16))
+
+
+_write = torch_op("paged_write_fp8", lambda k, v, slots, k_cache, v_cache, k_scale, v_scale: None)
+_read = torch_op("paged_read_fp8", _read_fake)
+_decode = torch_op("paged_decode_fp8", lambda q, *rest: q.new_empty(q.shape))
+_decode_append = torch_op("paged_decode_fp8_append", lambda q, *rest: q.new_empty(q.shape))
 
 
 def fp8_cache(num_pages: int, page_size: int = 16, num_kv_heads: int = 8, head_dim: int = 128, device="cuda"):
@@ -65,14 +73,3 @@ def paged_decode_fp8_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k
     returned, the new one with the value that the pool now holds (``paged_write_fp8`` then ``paged_decode_fp8``).  Rows with
     cache_seqlens < 0, or without room for the new token, give zeros and write nothing."""
     return _decode_append(q, k, v, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_table, softmax_scale)
-
-
-def _read_fake(k_cache, v_cache, k_scale, v_scale, slots):
-    shape = (slots.shape[0], k_cache.shape[2], k_cache.shape[3])
-    return (k_cache.new_empty(shape, dtype=torch.bfloat16), k_cache.new_empty(shape, dtype=torch.bfloat16))
-
-
-register_fake(_write, lambda k, v, slots, k_cache, v_cache, k_scale, v_scale: None)
-register_fake(_read, _read_fake)
-register_fake(_decode, lambda q, *rest: q.new_empty(q.shape))
-register_fake(_decode_append, lambda q, *rest: q.new_empty(q.shape))

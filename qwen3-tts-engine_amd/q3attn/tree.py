@@ -9,9 +9,9 @@ from typing import Optional
 
 import torch
 
-from ._lib import register_fake, torch_ops
+from ._lib import torch_op
 
-(_tree,) = torch_ops("paged_decode_tree")
+_tree = torch_op("paged_decode_tree", lambda q, *rest, **more: torch.empty_like(q, memory_format=torch.contiguous_format))
 
 
 def paged_decode_tree(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tree_mask: Optional[torch.Tensor],
@@ -29,6 +29,3 @@ def paged_decode_tree(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tree_ma
     for the bf16 pool).  The reference decodes one token a row (engine/talker.py:77); with N = 1 and no mask this is its call
     with the new token not yet in the cache."""
     return _tree(q, k, v, tree_mask, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, k_scale, v_scale)
-
-
-register_fake(_tree, lambda q, *rest, **more: torch.empty_like(q, memory_format=torch.contiguous_format))
