@@ -2,8 +2,8 @@
 
 Compiles every ``csrc/*.hip`` with hipcc for gfx950 and links ``q3attn/libq3attn.so`` in-tree, so
 the built library travels with the source tree; ``binding/torch_ops.cpp``, the torch ops that are
-registered from C++, becomes ``q3attn/libq3torch.so`` beside it (host code only).  Object files go to
-``_build/`` (git-ignored).
+registered from C++, becomes ``q3attn/libq3torch.so`` beside it (host code only, by the host compiler against
+torch's headers).  Object files go to ``_build/`` (git-ignored).
 """
 from __future__ import annotations
 
@@ -72,7 +72,10 @@ def _compile(src: str) -> str:
 
 
 def _run(cmd, what: str) -> None:
-    r = subprocess.run(cmd, capture_output=True, text=True)
+    try:
+        r = subprocess.run(cmd, capture_output=True, text=True)
+    except OSError as e:
+        raise RuntimeError(f"{what} failed: {e}") from e
     if r.returncode != 0:
         raise RuntimeError(f"{what} failed:\n{r.stdout}{r.stderr}")
 
@@ -101,7 +104,6 @@ def build(verbose: bool = False) -> str:
     with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as ex:
         binding = ex.submit(_compile_torch_ops)
         objs = list(ex.map(_compile, srcs + [PROBE_SRC]))
-        binding = binding.result()
     for out, parts in ((OUT, objs[:-1]), (PROBE_OUT, objs[-1:])):
         tmp = out + ".tmp"
         soname = ["-Wl,-soname," + os.path.basename(out)]
@@ -109,7 +111,14 @@ def build(verbose: bool = False) -> str:
         os.replace(tmp, out)
         if verbose:
             print(f"built {out}")
-    _link_torch_ops(binding)
+    # Last, since it needs a host compiler and torch's headers and nothing needs it: where it fails, the HIP libraries are there all
+    # the same, and no binding of an earlier build beside them.
+    try:
+        _link_torch_ops(binding.result())
+    except (RuntimeError, ImportError) as e:
+        if os.path.exists(TORCH_OUT):
+            os.remove(TORCH_OUT)
+        raise RuntimeError(f"{OUT} is built, but the torch ops of {TORCH_SRC} are not: {e}") from e
     if verbose:
         print(f"built {TORCH_OUT}")
     return OUT

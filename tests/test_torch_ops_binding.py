@@ -1,5 +1,6 @@
 """CPU tests of how the C++-registered torch ops are found: a libq3torch.so that is missing or cannot be loaded costs its own ops and
-nothing else."""
+nothing else, neither at import nor in the build."""
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -66,3 +67,33 @@ refused('must be on a GPU')
 k, v = call('meta')
 assert k.shape == v.shape == (3, 8, 128) and k.dtype == torch.bfloat16
 """)
+
+
+def _build_module(tmp_path, monkeypatch):
+    """build.py with its outputs under tmp_path, the HIP compiler's part left out."""
+    spec = importlib.util.spec_from_file_location("q3attn_build_under_test", os.path.join(PKG, "build.py"))
+    b = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(b)
+    for name, file in (("OUT", "libq3attn.so"), ("PROBE_OUT", "libq3probe.so"), ("TORCH_OUT", "libq3torch.so"), ("BUILD", "_build")):
+        monkeypatch.setattr(b, name, str(tmp_path / file))
+    monkeypatch.setattr(b, "_compile", lambda src: src + ".o")
+    run = b._run
+
+    def link_only(cmd, what):
+        if what != "link":
+            return run(cmd, what)
+        with open(cmd[-1], "w") as f:
+            f.write("linked")
+
+    monkeypatch.setattr(b, "_run", link_only)
+    return b
+
+
+def test_a_build_without_a_host_compiler_keeps_the_hip_libraries(tmp_path, monkeypatch):
+    b = _build_module(tmp_path, monkeypatch)
+    (tmp_path / "libq3torch.so").write_text("of an earlier build")
+    monkeypatch.setattr(b, "CXX", str(tmp_path / "no-compiler"))
+    with pytest.raises(RuntimeError, match="no-compiler"):
+        b.build()
+    assert (tmp_path / "libq3attn.so").read_text() == (tmp_path / "libq3probe.so").read_text() == "linked"
+    assert not (tmp_path / "libq3torch.so").exists()
