@@ -8,7 +8,10 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <ATen/core/LegacyTypeDispatch.h>
 #include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/VariableTypeUtils.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include <tuple>
@@ -229,6 +232,102 @@ Tensor paged_decode_tree(const Tensor& q, const Tensor& k, const Tensor& v, cons
   return c.out;
 }
 
+// What autograd sees.  None of the ops has a backward: one that is asked for raises, instead of leaving gradients out.  And the ops
+// that write into caches count as in-place operations on them, so that autograd notices a cache that it has saved.
+//
+// (Each form calls the op again below its own dispatch key, as dispatch modes and fake tensors have to see it there.)
+template <class Op>
+auto op_of(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Op>();
+}
+
+void no_backward(const char* name, const Tensor& out, torch::autograd::edge_list&& edges) {
+  torch::autograd::set_history(
+      out, std::shared_ptr<torch::autograd::Node>(new torch::autograd::NotImplemented(name, std::move(edges)), torch::autograd::deleteNode));
+}
+
+Tensor decode_autograd(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs, const Tensor& lens,
+                       const Tensor& bt, double softmax_scale) {
+  static const auto op = op_of<decltype(paged_decode_fp8)>("q3attn::paged_decode_fp8");
+  Tensor out;
+  {
+    const at::AutoDispatchBelowAutograd below;
+    out = op.call(q, kc, vc, ks, vs, lens, bt, softmax_scale);
+  }
+  if (torch::autograd::compute_requires_grad(q, kc, vc))
+    no_backward("q3attn::paged_decode_fp8", out, torch::autograd::collect_next_edges(q, kc, vc));
+  return out;
+}
+
+Tensor decode_append_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& kc, const Tensor& vc, const Tensor& ks,
+                              const Tensor& vs, const Tensor& lens, const Tensor& bt, double softmax_scale) {
+  static const auto op = op_of<decltype(paged_decode_fp8_append)>("q3attn::paged_decode_fp8_append");
+  Tensor out;
+  {
+    const at::AutoDispatchBelowAutograd below;
+    out = op.call(q, k, v, kc, vc, ks, vs, lens, bt, softmax_scale);
+  }
+  if (torch::autograd::compute_requires_grad(q, k, v))
+    no_backward("q3attn::paged_decode_fp8_append", out, torch::autograd::collect_next_edges(q, k, v));
+  return out;
+}
+
+std::tuple<Tensor, Tensor> read_autograd(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs, const Tensor& slots) {
+  static const auto op = op_of<decltype(paged_read_fp8)>("q3attn::paged_read_fp8");
+  std::tuple<Tensor, Tensor> out;
+  {
+    const at::AutoDispatchBelowAutograd below;
+    out = op.call(kc, vc, ks, vs, slots);
+  }
+  if (torch::autograd::compute_requires_grad(kc, vc)) {
+    no_backward("q3attn::paged_read_fp8", std::get<0>(out), torch::autograd::collect_next_edges(kc, vc));
+    no_backward("q3attn::paged_read_fp8", std::get<1>(out), torch::autograd::collect_next_edges(kc, vc));
+  }
+  return out;
+}
+
+Tensor tree_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const optional<Tensor>& tree_mask, const Tensor& kc,
+                     const Tensor& vc, const Tensor& lens, const Tensor& bt, double softmax_scale, const optional<Tensor>& k_scale,
+                     const optional<Tensor>& v_scale) {
+  static const auto op = op_of<decltype(paged_decode_tree)>("q3attn::paged_decode_tree");
+  Tensor out;
+  {
+    const at::AutoDispatchBelowAutograd below;
+    out = op.call(q, k, v, tree_mask, kc, vc, lens, bt, softmax_scale, k_scale, v_scale);
+  }
+  if (torch::autograd::compute_requires_grad(q, k, v, kc, vc))
+    no_backward("q3attn::paged_decode_tree", out, torch::autograd::collect_next_edges(q, k, v, kc, vc));
+  return out;
+}
+
+template <class... T>
+void written(const T&... caches) {
+  for (const Tensor& t : {caches...})
+    if (!t.is_inference()) torch::autograd::increment_version(t);
+}
+
+void write_in_place(const Tensor& k, const Tensor& v, const Tensor& slots, const Tensor& kc, const Tensor& vc, const Tensor& ks,
+                    const Tensor& vs) {
+  static const auto op = op_of<decltype(paged_write_fp8)>("q3attn::paged_write_fp8");
+  {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    op.call(k, v, slots, kc, vc, ks, vs);
+  }
+  written(kc, vc, ks, vs);
+}
+
+Tensor decode_append_in_place(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& kc, const Tensor& vc, const Tensor& ks,
+                              const Tensor& vs, const Tensor& lens, const Tensor& bt, double softmax_scale) {
+  static const auto op = op_of<decltype(paged_decode_fp8_append)>("q3attn::paged_decode_fp8_append");
+  Tensor out;
+  {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    out = op.call(q, k, v, kc, vc, ks, vs, lens, bt, softmax_scale);
+  }
+  written(kc, vc, ks, vs);
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(q3attn, m) {
@@ -250,4 +349,16 @@ TORCH_LIBRARY_IMPL(q3attn, CompositeExplicitAutograd, m) {
   m.impl("paged_decode_fp8", &paged_decode_fp8);
   m.impl("paged_decode_fp8_append", &paged_decode_fp8_append);
   m.impl("paged_decode_tree", &paged_decode_tree);
+}
+
+TORCH_LIBRARY_IMPL(q3attn, Autograd, m) {
+  m.impl("paged_read_fp8", &read_autograd);
+  m.impl("paged_decode_fp8", &decode_autograd);
+  m.impl("paged_decode_fp8_append", &decode_append_autograd);
+  m.impl("paged_decode_tree", &tree_autograd);
+}
+
+TORCH_LIBRARY_IMPL(q3attn, ADInplaceOrView, m) {
+  m.impl("paged_write_fp8", &write_in_place);
+  m.impl("paged_decode_fp8_append", &decode_append_in_place);
 }
