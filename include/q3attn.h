@@ -483,7 +483,9 @@ int q3a_paged_read_fp8(const void* k_cache, const void* v_cache, int64_t kv_stri
  * token must not be read by another row of the same call.
  *
  * workspace: q3a_paged_decode_tree_workspace_bytes(batch, 1, ...) bytes, 16-byte aligned, uninitialised (0: may be NULL);
- * calls that overlap need one each.  batch at most 65,535; a table of at most 2^28 tokens a row; a cache below 64 GiB (pages
+ * calls that overlap need one each.  Ask for every shape that is called, on the device that will run it: the size depends on the
+ * device's compute units, and a larger batch, table or number of nodes may need less (576 rows of a 2,048-token table and 8 KV
+ * heads need none, one such row 4.1 MiB).  batch at most 65,535; a table of at most 2^28 tokens a row; a cache below 64 GiB (pages
  * times page stride), its scales below 4 GiB.
  */
 int q3a_paged_decode_fp8(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k_cache, const void* v_cache,
