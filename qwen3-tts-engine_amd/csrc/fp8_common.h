@@ -127,4 +127,8 @@ inline Divisor divisor(uint32_t d) {
   return {d, (uint32_t)(((uint64_t)1 << (31 + s)) / d + 1), 31 + s};
 }
 
+// A pool's pointers, strides and sizes as every entry point over it needs them (kv_fp8.hip): Q3A_OK, or the error for the caller.
+int check_fp8_pool(const char* who, const void* kc, const void* vc, int64_t sp, int64_t st, int64_t sh, const void* ks,
+                   const void* vs, int64_t ss_p, int64_t ss_h, int num_pages, int page_size, int hkv);
+
 }  // namespace q3a

@@ -33,10 +33,6 @@
 #include "../../include/q3attn.h"
 
 namespace q3a {
-
-int check_fp8_pool(const char* who, const void* kc, const void* vc, int64_t sp, int64_t st, int64_t sh, const void* ks,
-                   const void* vs, int64_t ss_p, int64_t ss_h, int num_pages, int page_size, int hkv);
-
 namespace {
 
 constexpr int kD = kRowDims;
