@@ -5,6 +5,7 @@ import torch
 
 import q3attn
 from fp8_reference import D, E4M3, attention, pool_values, table_for
+from q3attn import _lib
 from test_gpu_decode_tree import _tree_masks
 
 pytestmark = pytest.mark.gpu
@@ -140,3 +141,53 @@ def test_small_query_elements_beside_large_ones(cuda_device, nodes, hkv, group, 
     out = q3attn.paged_decode_fp8_append(q[:, 0].to(cuda_device), kv[0, last].to(cuda_device), kv[1, last].to(cuda_device), *pool,
                                          now.to(cuda_device), *args[1:])
     _assert_precise(out, want[:, 0], spread[:, 0])
+
+
+@pytest.mark.parametrize("nodes,hkv,group", [(1, 2, 2), (3, 1, 4), (30, 1, 2)])
+def test_small_query_elements_in_chunks(cuda_device, nodes, hkv, group):
+    """The same in a table so wide that rows are cut into chunks; a head that is not finite beside it gives NaN, and no other does."""
+    g = torch.Generator().manual_seed(nodes)
+    lens, width = torch.tensor([2500, 3, 0, 1100], dtype=torch.int32), 4096
+    used = 157 + 1 + 69
+    kv = torch.randn((2, used * 16, hkv, D), generator=g).to(torch.bfloat16)
+    kv[0, ..., 0] = 0
+    pool = q3attn.fp8_cache(used, 16, hkv, device=cuda_device)
+    q3attn.paged_write_fp8(kv[0].to(cuda_device), kv[1].to(cuda_device), torch.arange(used * 16, device=cuda_device), *pool)
+    table = table_for(lens.tolist(), 16, used, width, nodes)
+    assert _lib.lib().q3a_paged_decode_tree_workspace_bytes(4, nodes, hkv * group, hkv, D, width, 16) > 0
+    q = (0.2 * torch.randn((4, nodes, hkv * group, D), generator=g)).to(torch.bfloat16)
+    q[:, ::2, 0, 0] = 2.0 ** 20
+    k, v = (torch.randn((4, nodes, hkv, D), generator=g).to(torch.bfloat16) for _ in range(2))
+    k[..., 0] = 0
+    mask = _tree_masks(4, nodes, nodes)
+    bad = q.clone()
+    bad[0, 0, 1, 5], bad[3, -1, -1, 9] = float("inf"), float("nan")
+    vals = pool_values(pool[0], pool[2]), pool_values(pool[1], pool[3])
+    args = lens.to(cuda_device), table.to(cuda_device), SCALE
+    for n, own in ((nodes, (k, v, mask)), (1, None)):
+        want, spread = attention(q[:, :n], *vals, lens, table, SCALE, own)
+        for qq in (q, bad):
+            if own is not None:
+                out = _tree(cuda_device, pool, table, lens, qq, k, v, mask)
+            else:
+                out = q3attn.paged_decode_fp8(qq[:, 0].to(cuda_device), *pool, *args)[:, None]
+            if qq is bad:
+                lost = ~torch.isfinite(qq[:, :n].float()).all(-1)
+                assert torch.isnan(out[lost.to(cuda_device)]).all() and int(lost.sum()) == (2 if n == nodes else 1 + (nodes == 1))
+                out = torch.where(lost[..., None].to(cuda_device), want.to(cuda_device).to(torch.bfloat16), out)
+            _assert_precise(out, want, spread)
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("nodes", [5, 40])
+def test_probabilities_in_chunks(cuda_device, fp8, nodes):
+    g = torch.Generator().manual_seed(nodes)
+    lens = [2500, 3, 0, 1100]
+    pool, table = _pool(lens, 2, fp8, cuda_device, nodes)
+    assert _lib.lib().q3a_paged_decode_tree_workspace_bytes(4, nodes, 4, 2, D, table.shape[1], 16) > 0
+    q = (0.2 * torch.randn((4, nodes, 4, D), generator=g)).to(torch.bfloat16)
+    k, v = (torch.randn((4, nodes, 2, D), generator=g).to(torch.bfloat16) for _ in range(2))
+    mask = _tree_masks(4, nodes, nodes)
+    lens = torch.tensor(lens, dtype=torch.int32)
+    want, spread = attention(q, pool_values(pool[0], pool[2]), pool_values(pool[1], pool[3]), lens, table, SCALE, (k, v, mask))
+    _assert_precise(_tree(cuda_device, pool, table, lens, q, k, v, mask), want, spread)
