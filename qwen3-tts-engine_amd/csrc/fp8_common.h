@@ -61,16 +61,6 @@ __device__ __forceinline__ uint32_t bf16_any_amax_pair(const uint32_t (&w)[N]) {
   for (int i = 0; i < N; ++i) a = pk_max_u16(a, w[i] & 0x7fff7fffu);
   return a;
 }
-// The least magnitude bits of n dwords of bf16 that are not 0, less 1 (0xffff: all are 0).
-template <int N>
-__device__ __forceinline__ uint32_t bf16_amin_less1(const uint32_t (&w)[N]) {
-  u16x2 a = {0xffff, 0xffff};
-  const u16x2 one = {1, 1};
-#pragma unroll
-  for (int i = 0; i < N; ++i) a = __builtin_elementwise_min(a, (u16x2)(__builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu) - one));
-  const uint32_t r = __builtin_bit_cast(uint32_t, a);
-  return min(r & 0xffffu, r >> 16);
-}
 // The pair with NaN in the halves that are not finite.
 __device__ __forceinline__ uint32_t nan_if_not_finite(uint32_t w) {
   if ((w & 0x7f80u) == 0x7f80u) w |= 0x7fu;

@@ -14,9 +14,7 @@
 // 1 up to 16 query rows, else 2: more do not fit the registers):
 //   S^T = K Q^T   A = 16 keys, B = Q^T.  bf16: v_mfma_f32_16x16x32_bf16; lane l holds key l % 16 and, of each 32 dims, the 8
 //                 that its quarter g = l / 16 takes: any split of the 128 dims over (step, quarter) is right as long as Q has
-//                 the same.  8-bit: one v_mfma_scale_f32_16x16x128_f8f6f4 on the codes as they are stored, K's exponent byte
-//                 being its scale operand, against Q in two e4m3 parts (converting K to bf16 first took 444 cycles a step
-//                 instead of 188).
+//                 the same.  8-bit codes are converted on the way, their exponent byte with them.
 //   O^T = V^T P^T A = V^T: lane l holds for dim index l % 16 the 8 keys 4 g .. 4 g + 3 of both subtiles, which are the keys
 //                 whose P its S^T registers hold, so P needs no lane moves.  Row i of MFMA j stands for dim 8 i + j: the
 //                 lane loads 8 dims in a row of its 8 keys, and the transpose is byte permutes within the lane.
@@ -44,7 +42,6 @@ enum { kNoKeys = 0, kTree = 1, kAppend = 2 };
 
 typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8_t;
 typedef __attribute__((__vector_size__(4 * sizeof(float)))) float f32x4_t;
-typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 
@@ -332,105 +329,22 @@ __device__ __forceinline__ void v_operands(const ValueTile<false>& x, int jj, bf
   a1 = __builtin_bit_cast(bf16x8_t, make_uint4(p1[0], p1[1], p1[2], p1[3]));
 }
 
-// Q^T as B operands: bf16 as it is, or, against 8-bit keys, in two e4m3 parts.
-//
-// The matrix instruction takes K's codes and its power-of-two scale (one byte a key) as they are, with Q as hi + lo: of q's 8
-// significant bits hi = e4m3(q / 2^e) holds the upper 4 and lo = e4m3(16 (q / 2^e - hi)) at 2^(e - 4) the rest.  That is q
-// itself down to 2^(e - 6), where e4m3 stops being a floating-point format, 2^-14 of its row's largest element.  So the scores are
-// those of the bf16 row, and a step's two products (K = 128 each) replace 32 conversions and 8 products in bf16.
-//
-// Smaller elements would be held to 2^-22 of the largest only.  That is nothing beside the largest one's share of a score, unless K is
-// small where q is large: with q = (2^22, 1, ..) and keys (0, k1, ..) k1 would not count.  So where a wave's query rows have
-// such an element, other than 0, its steps take Q in bf16 and convert K (2.4 times the cycles; a quarter of the waves do with 16 rows
-// of normalised queries, half with 32: 32 rows x 13 nodes 18.6 -> 19.2 us, 6 long rows x 63 nodes 79.7 -> 83.6).  Asking whether
-// the parts hold all the same what is smaller but short, which a third of those would pass, took as long or longer.
-template <bool kFp8, int kMT>
-struct Query;
+// Q^T as B operands, in bf16.
 template <int kMT>
-struct Query<false, kMT> {
+struct Query {
   bf16x8_t v[kMT][4];
 };
-template <int kMT>
-struct Query<true, kMT> {
-  i32x8_t hi[kMT], lo[kMT];  // two parts, or the four bf16 operands as they are loaded
-  int s[kMT];                // the exponent byte of hi; lo's is 4 less
-  bool parts;                // the same for the wave
-};
-
-// The largest over the four lanes of a query row (small integers order as floats do).
-__device__ __forceinline__ uint32_t row_max(uint32_t x) {
-  return (uint32_t)__float_as_int(max_xor32(max_xor16(__int_as_float((int)x))));
-}
-template <int kMT>
-__device__ __forceinline__ void prepare(const bf16x8_t (&q)[kMT][4], Query<false, kMT>& x) {
-#pragma unroll
-  for (int t = 0; t < kMT; ++t)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) x.v[t][c] = q[t][c];
-}
-template <int kMT>
-__device__ __forceinline__ void prepare(const bf16x8_t (&q)[kMT][4], Query<true, kMT>& x) {
-  bool fine = false;  // some element may be too small for the parts
-  uint32_t w[kMT][16], sb[kMT];
-  bool rare[kMT];
-#pragma unroll
-  for (int t = 0; t < kMT; ++t) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const uint4 e = __builtin_bit_cast(uint4, q[t][c]);
-      w[t][4 * c] = e.x;
-      w[t][4 * c + 1] = e.y;
-      w[t][4 * c + 2] = e.z;
-      w[t][4 * c + 3] = e.w;
-    }
-    uint32_t top = row_max(halves_max(bf16_any_amax_pair(w[t])));
-    rare[t] = any_rare(top);
-    if (rare[t]) top = row_max(halves_max(bf16_amax_pair(w[t])));
-    sb[t] = fp8_scale_byte(top);
-    fine = fine | (bf16_amin_less1(w[t]) < ((sb[t] - 6) << 7) - 1);
-  }
-  x.parts = __builtin_amdgcn_ballot_w64(fine) == 0;
-  if (!x.parts) {
-#pragma unroll
-    for (int t = 0; t < kMT; ++t) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x.hi[t][i] = (int)nan_if_not_finite(w[t][i]);
-        x.lo[t][i] = (int)nan_if_not_finite(w[t][8 + i]);
-      }
-      x.s[t] = 0;
-    }
-    return;
-  }
-#pragma unroll
-  for (int t = 0; t < kMT; ++t) {
-    const float scale = fp8_scale(sb[t]);
-    x.s[t] = (int)sb[t];
-    uint32_t hi[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) hi[i] = fp8_finite_codes4(w[t][2 * i], w[t][2 * i + 1], scale);
-    if (rare[t]) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) hi[i] = fp8_codes4(w[t][2 * i], w[t][2 * i + 1], sb[t]);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      // what hi leaves, exact in fp32: at most 16 scale (at byte 247: 15 scale), so e4m3 at a 16th of the scale holds it
-      s16x2 lo = {0, 0};
-      const f32x2_t h0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi[i], scale, false);
-      const f32x2_t h1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi[i], scale, true);
-      const uint32_t a = w[t][2 * i], b = w[t][2 * i + 1];
-      lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, bf16_lo(a) - h0[0], bf16_hi(a) - h0[1], scale * 0.0625f, false);
-      lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, bf16_lo(b) - h1[0], bf16_hi(b) - h1[1], scale * 0.0625f, true);
-      x.hi[t][i] = (int)hi[i];
-      x.lo[t][i] = __builtin_bit_cast(int, lo);
-    }
-  }
-}
 
 // A step's scores S^T, unscaled.  kSwapped: the keys are as load_k left them.
+//
+// 8-bit keys are converted to bf16, exactly: 16 instructions a subtile, which take the exponent byte along.  So the scores are those of
+// the bf16 row.  (The scaled 8-bit matrix instruction takes the codes as they are, but wants Q in 8 bits too.  Two such numbers an
+// element do not hold what is below 2^-14 of its row's largest element, and scores over keys that are small where that one is were
+// wrong; two products where they do hold a wave's queries, and this where not, took longer than this alone: 83.2 us for 82.0, 6 long
+// rows x 63 nodes, 19.9 for 19.0, 32 rows x 13 nodes, 8.8 for 8.3, one row x 1000.)
 template <bool kSwapped, int kMT>
-__device__ __forceinline__ void scores(const KeyTile<true>& x, const Query<true, kMT>& q, f32x4_t (&s)[kMT][2]) {
+__device__ __forceinline__ void scores(const KeyTile<true>& x, const Query<kMT>& q, f32x4_t (&s)[kMT][2]) {
+  const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     i32x8_t k = x.k[u];
@@ -444,33 +358,20 @@ __device__ __forceinline__ void scores(const KeyTile<true>& x, const Query<true,
         k[i] = odd ? odd_gets : k[i];
       }
     }
-    const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
-    if (q.parts) {
+    const float f = fp8_scale(x.ks[u]);
 #pragma unroll
-      for (int t = 0; t < kMT; ++t) {
-        s[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q.lo[t], zero, 0, 0, 0, (int)x.ks[u], 0, q.s[t] - 4);
-        s[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q.hi[t], s[t][u], 0, 0, 0, (int)x.ks[u], 0, q.s[t]);
-      }
-    } else {
-      const float f = fp8_scale(x.ks[u]);
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t a = (uint32_t)k[2 * c], b = (uint32_t)k[2 * c + 1];
+      const bf16x8_t kf = __builtin_bit_cast(
+          bf16x8_t, make_uint4(fp8_pair<false>(a, f), fp8_pair<true>(a, f), fp8_pair<false>(b, f), fp8_pair<true>(b, f)));
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const uint32_t a = (uint32_t)k[2 * c], b = (uint32_t)k[2 * c + 1];
-        const bf16x8_t kf = __builtin_bit_cast(
-            bf16x8_t, make_uint4(fp8_pair<false>(a, f), fp8_pair<true>(a, f), fp8_pair<false>(b, f), fp8_pair<true>(b, f)));
-#pragma unroll
-        for (int t = 0; t < kMT; ++t) {
-          const i32x8_t& half = c < 2 ? q.hi[t] : q.lo[t];
-          const int i = 4 * (c & 1);
-          const i32x4_t qf = {half[i], half[i + 1], half[i + 2], half[i + 3]};
-          s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, __builtin_bit_cast(bf16x8_t, qf), c == 0 ? zero : s[t][u], 0, 0, 0);
-        }
-      }
+      for (int t = 0; t < kMT; ++t)
+        s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q.v[t][c], c == 0 ? zero : s[t][u], 0, 0, 0);
     }
   }
 }
 template <bool kPaired, int kMT>
-__device__ __forceinline__ void scores(const KeyTile<false>& x, const Query<false, kMT>& q, f32x4_t (&s)[kMT][2]) {
+__device__ __forceinline__ void scores(const KeyTile<false>& x, const Query<kMT>& q, f32x4_t (&s)[kMT][2]) {
   const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -686,7 +587,7 @@ __device__ __forceinline__ void add_not_finite(const uint16_t* vb, int ts, const
 // not finite must not reach the rows that do not see its key (0 * inf in the product): such elements are zeroed in the
 // product and added afterwards for the rows that see them.
 template <bool kFp8, int kMT>
-__device__ __forceinline__ void tree_step(const Work& w, int ts, const Query<false, kMT>& q, State<kMT>& st) {
+__device__ __forceinline__ void tree_step(const Work& w, int ts, const Query<kMT>& q, State<kMT>& st) {
   const int lane = lane_now();
   const int r = lane & 15, g = lane >> 4;
   const TreeArgs& a = args_again();
@@ -759,6 +660,11 @@ __device__ __forceinline__ void tree_step(const Work& w, int ts, const Query<fal
   }
   values<false, kMT>(y, any, lane, sc, st);
   if (any_odd) add_not_finite<kMT>(vb, ts, seen, st);
+}
+
+// The largest over the four lanes that hold a row (small integers order as floats do).
+__device__ __forceinline__ uint32_t row_max(uint32_t x) {
+  return (uint32_t)__float_as_int(max_xor32(max_xor16(__int_as_float((int)x))));
 }
 
 // The append form's new row, quantised as the write kernel does and stored, then attended as a cached subtile of one key.
@@ -881,7 +787,7 @@ struct Stream {
     valid[1] = p.valid[1];
   }
   // Computes the step and loads the next one.
-  __device__ __forceinline__ void turn(const TreeArgs& a, const Place& next, const Query<kFp8, kMT>& q, int lane, State<kMT>& st) {
+  __device__ __forceinline__ void turn(const TreeArgs& a, const Place& next, const Query<kMT>& q, int lane, State<kMT>& st) {
     const uint32_t all[kMT] = {};
     f32x4_t s[kMT][2];
     scores<kLayout, kMT>(k, q, s);
@@ -900,7 +806,7 @@ struct Stream {
 
 // The append form's step: the new row.
 template <int kMT>
-__device__ __forceinline__ void append_step(const TreeArgs& a, const Work& w, const Query<true, kMT>& q, int lane, State<kMT>& st) {
+__device__ __forceinline__ void append_step(const TreeArgs& a, const Work& w, const Query<kMT>& q, int lane, State<kMT>& st) {
   const uint32_t all[kMT] = {};
   f32x4_t s[kMT][2];
   KeyTile<true> x;
@@ -912,17 +818,31 @@ __device__ __forceinline__ void append_step(const TreeArgs& a, const Work& w, co
   values<true, kMT>(y, one, lane, s, st);
 }
 
-// raw, as it was loaded, with the sign that the scale asks for.
+// Q, as it was loaded, with the sign that the scale asks for; an element that is not finite becomes NaN, as its row's result then is
+// (scores of -inf alone would else give zeros).
 template <int kMT>
-__device__ __forceinline__ void turn_signs(Query<false, kMT>& raw) {
+__device__ __forceinline__ void turn_signs(Query<kMT>& q) {
   const uint32_t sign = args_again().q_sign;
+  uint32_t top = 0;
 #pragma unroll
   for (int t = 0; t < kMT; ++t)
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const uint4 v = __builtin_bit_cast(uint4, raw.v[t][c]);
-      raw.v[t][c] = __builtin_bit_cast(bf16x8_t, make_uint4(v.x ^ sign, v.y ^ sign, v.z ^ sign, v.w ^ sign));
+      const uint4 v = __builtin_bit_cast(uint4, q.v[t][c]);
+      const uint32_t w[4] = {v.x ^ sign, v.y ^ sign, v.z ^ sign, v.w ^ sign};
+      top = pk_max_u16(top, bf16_any_amax_pair(w));
+      q.v[t][c] = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
     }
+  if (__builtin_amdgcn_ballot_w64(halves_max(top) >= 0x7f80u) != 0) {
+#pragma unroll
+    for (int t = 0; t < kMT; ++t)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const uint4 v = __builtin_bit_cast(uint4, q.v[t][c]);
+        q.v[t][c] = __builtin_bit_cast(bf16x8_t, make_uint4(nan_if_not_finite(v.x), nan_if_not_finite(v.y), nan_if_not_finite(v.z),
+                                                            nan_if_not_finite(v.w)));
+      }
+  }
 }
 
 // Query rows that the waves merge at once, 34 KB of them.
@@ -1149,7 +1069,7 @@ __global__ __launch_bounds__(64 * kW, kMT == 2 || (kMode == kTree && kChunked) ?
   unit_of(args, w.h, w.mb, unit);
   if (unit >= args.units) return;
   Window win;
-  Query<false, kMT> raw;
+  Query<kMT> q;
   int s0 = 0, s1;  // the chunk's steps
   float* rec = nullptr;
   if constexpr (kChunked) {
@@ -1168,7 +1088,7 @@ __global__ __launch_bounds__(64 * kW, kMT == 2 || (kMode == kTree && kChunked) ?
       reinterpret_cast<Joined*>(args_again().ws)[w.b] = Joined{unit - c.index, c.count};
     const int s = s0 + wave + kW * (lane >> 1);
     const Entry e = entry_of(w.b, s, lane);
-    load_q<kFp8, kMT>(w, raw.v);
+    load_q<kFp8, kMT>(w, q.v);
     win = window_of<kFp8>(e, w.L, s < min(s1, w.Tc));
   } else {
     w.b = unit;
@@ -1176,7 +1096,7 @@ __global__ __launch_bounds__(64 * kW, kMT == 2 || (kMode == kTree && kChunked) ?
     if (args.order && unit >= row0) w.b = kth_longest<kW>(args, row0, unit - row0, wave);
     // The first window's page ids do not wait for the row's length.
     const Entry e = entry_of(w.b, wave + kW * (lane >> 1), lane);
-    load_q<kFp8, kMT>(w, raw.v);
+    load_q<kFp8, kMT>(w, q.v);
     win = window_of<kFp8>(e, INT_MAX, true);
     w.L = __builtin_amdgcn_readfirstlane(row_tokens(w.b, kMode));
     w.Tc = w.L > 0 ? (w.L + kStep - 1) / kStep : 0;
@@ -1202,16 +1122,15 @@ __global__ __launch_bounds__(64 * kW, kMT == 2 || (kMode == kTree && kChunked) ?
       return place_of<kFp8>(win, j & (kWindow - 1), j < n, w.L - kStep * (first + kW * j));
     };
     Stream<kFp8, kMT> x;
-    Query<kFp8, kMT> q;
     if constexpr (kMode == kTree) {
       // A wave that has own steps takes them first.  Chunks, which are few, ask for their keys ahead of them; where the chip is
       // full the registers that this takes would cost every compute unit its third workgroup (256 rows x 600 tokens x 8 nodes
       // over the 8-bit pool: 67.0 us with three, 70.7 with two; one row of four nodes: 0.4 us the other way).
       constexpr bool kEarly = kChunked && (kFp8 || kMT == 1);
       auto own_steps = [&]() __attribute__((always_inline)) {
-        turn_signs(raw);
+        turn_signs(q);
         clear(st);
-        for (int s = own; s < s1; s += kW) tree_step<kFp8, kMT>(w, s - w.Tc, raw, st);
+        for (int s = own; s < s1; s += kW) tree_step<kFp8, kMT>(w, s - w.Tc, q, st);
       };
       if constexpr (kEarly) {
         x.load(a, place(0), lane);
@@ -1221,16 +1140,13 @@ __global__ __launch_bounds__(64 * kW, kMT == 2 || (kMode == kTree && kChunked) ?
         x.load(a, place(0), lane);
       } else {
         x.load(a, place(0), lane);
-        turn_signs(raw);
+        turn_signs(q);
         clear(st);
       }
-      prepare(raw.v, q);
     } else {
       x.load(a, place(0), lane);
-      turn_signs(raw);
-      prepare(raw.v, q);
-      __builtin_amdgcn_sched_barrier(0);
-      clear(st);  // (not before: Q's two parts and what they come from fill the registers)
+      turn_signs(q);
+      clear(st);
       if constexpr (kMode == kAppend) {
         if (own < s1) append_step<kMT>(a, w, q, lane, st);
       }

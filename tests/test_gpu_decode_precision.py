@@ -191,3 +191,25 @@ def test_probabilities_in_chunks(cuda_device, fp8, nodes):
     lens = torch.tensor(lens, dtype=torch.int32)
     want, spread = attention(q, pool_values(pool[0], pool[2]), pool_values(pool[1], pool[3]), lens, table, SCALE, (k, v, mask))
     _assert_precise(_tree(cuda_device, pool, table, lens, q, k, v, mask), want, spread)
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("nodes", [3, 20])
+def test_infinite_queries_give_nan(cuda_device, fp8, nodes):
+    """Also where every score is -inf (exp(-inf - -inf)), over cached and own keys; other heads and nodes as without."""
+    lens = torch.tensor([1, 40, 0], dtype=torch.int32)
+    pool, table = _pool([1, 40, 1], 1, fp8, cuda_device, 5)
+    if not fp8:
+        pool[0].copy_(pool[0].abs())
+    g = torch.Generator().manual_seed(6)
+    q = (0.2 * torch.randn((3, nodes, 2, D), generator=g)).to(torch.bfloat16)
+    k, v = (torch.randn((3, nodes, 1, D), generator=g).to(torch.bfloat16) for _ in range(2))
+    k = k.abs()
+    mask = _tree_masks(3, nodes, nodes)
+    bad = q.clone()
+    for b, n, h, value in ((0, 0, 1, "-inf"), (1, nodes - 1, 0, "-inf"), (2, 1, 0, "-inf"), (2, 2, 1, "inf")):
+        bad[b, n, h, 7] = float(value)
+    lost = torch.isinf(bad).any(-1)
+    out = _tree(cuda_device, pool, table, lens, bad, k, v, mask).cpu()
+    clean = _tree(cuda_device, pool, table, lens, q, k, v, mask).cpu()
+    assert torch.isnan(out[lost]).all() and torch.equal(out[~lost], clean[~lost])
