@@ -6,8 +6,8 @@
 // G = Hq / Hkv the M = N G query rows m = (n, g) of a KV head share every key:
 //   s_mj = scale q_m . k_j,   o_m = sum_j exp(s_mj - max_j s_mj) v_j / sum_j exp(s_mj - max_j s_mj);   zeros if nothing is seen.
 // K and V are read once for each block of 16 kMT query rows, so with few query rows HBM bounds it: 768 rows of 512 tokens over
-// the 8-bit pool run at 6.2 TB/s (with 5 % more than the keys for the exponent bytes' lines), 256 rows of 600 tokens and 8 nodes
-// over bf16 at 5.9.  63 nodes are bound by vector instructions (480 TFLOP/s), calls of a few rows by latency: 5 us from start to
+// the 8-bit pool run at 6.4 TB/s (with 5 % more than the keys for the exponent bytes' lines), 256 rows of 600 tokens and 8 nodes
+// over bf16 at 6.1.  63 nodes are bound by vector instructions (430 TFLOP/s), calls of a few rows by latency: 5 us from start to
 // end of the shortest row, of which the keys' way is 2.5.
 //
 // A step is 32 keys (two 16-token subtiles, each inside one page) by 16 kMT query rows, on one wave, from registers alone (kMT is
@@ -409,7 +409,7 @@ __device__ __forceinline__ float larger(float a, float b) { return __builtin_ele
 // The base need not be the maximum, only near it and not below: where some query row's scores have outgrown it, it is set to
 // their maximum and 2^kAhead more (a.ahead, in unscaled scores), which after a row's first steps hardly happens again, while with
 // 16 or 32 query rows some row's maximum grows in almost every step, and rescaling is a sixth to a quarter of a step's vector
-// instructions (6 rows x 63 nodes: 82.7 us with kAhead = 0, 80.2 with 4, 79.3 with 6).  No probability passes 1 for it, so that a
+// instructions (6 rows x 63 nodes: 89.1 us with kAhead = 0, 85.5 with 4, 84.3 with 6).  No probability passes 1 for it, so that a
 // product with the largest V stays finite.
 constexpr float kAhead = 4.f;
 
@@ -465,9 +465,10 @@ __device__ __forceinline__ void softmax(const int (&valid)[2], const uint32_t (&
 // O^T += V^T P^T, with each probability as the sum of two bf16 numbers.
 //
 // One bf16 number holds 8 of its significant bits, and only a row's largest one is a power of two: over eight calls the results were
-// off by 0.0018 to 0.0023 of their norm instead of the 0.0017 that their own rounding to bf16 takes.  Two hold 16 bits (2^-16 of
-// each probability is left) and reach the 0.0017.  The second product takes nothing where HBM is the bound, 3.6 % of 32 rows
-// x 13 nodes (17.9 -> 18.6 us) and 6.7 % of 6 long rows x 63 nodes (73.3 -> 78.2), which vector instructions bound.
+// off by 0.0018 to 0.0023 of their norm instead of the 0.0017 that their own rounding to bf16 takes.  Two hold 16 bits (2^-15 of
+// each probability is left) and reach the 0.0017.  The second product takes nothing where HBM is the bound (576 rows 96.8 and
+// 97.0 us), a little of 32 rows x 13 nodes (18.2 -> 18.9) and more of 6 long rows x 63 nodes (76.1 -> 85.5), which vector
+// instructions bound.
 // Over the 8-bit pool the first part is rounded to nearest.  Over bf16, whose V may hold infinities, both parts of a probability
 // over 0 have to be over 0, that no product of 0 and an infinity makes a NaN: the first is cut off from the next smaller number.
 template <bool kFp8, int kMT>
@@ -986,8 +987,8 @@ __device__ __forceinline__ uint32_t rounds_of(const TreeArgs& a, int L, int mode
 // Chunk `at` of all rows' chunks laid end to end.  64 rows at a time, one a lane; every wave does it.  A chunk has up to `size`
 // rounds: total / target, rounded up, so that a row's 1 + floor(rounds / size) come to target + batch at most.  The target is two
 // workgroups a compute unit.  One alone has its rounds in 0.6 of the time, and spares the other's start and records, about a round
-// and a half: so it is one where its size is not longer by more than that (8 rows x 4000 tokens 20.4 -> 19.1 us, 1 x 4000 x 64
-// nodes 21.7 -> 17.5; ragged batches mostly need two: 6 long rows x 63 nodes take 79 us with two and 121 with one).
+// and a half: so it is one where its size is not longer by more than that (8 rows x 4000 tokens 19.0 -> 17.7 us, 1 x 4000 x 64
+// nodes 20.4 -> 16.9; ragged batches mostly need two: 6 long rows x 63 nodes take 86 us with two and 135 with one).
 template <int kW>
 __device__ __forceinline__ Chunk chunk_at(const TreeArgs& a, uint32_t at, int mode) {
   const int lane = lane_now(), batch = a.batch, cap = a.max_pages * a.page_size;
@@ -1021,11 +1022,11 @@ __device__ __forceinline__ Chunk chunk_at(const TreeArgs& a, uint32_t at, int mo
 }
 
 // The k-th of the batch's last rows, from row0 on (up to 64 kW), by their lengths, longest first.  Workgroups start in the order
-// of their numbers, and the last to start should be short: 250 rows of 200 to 1200 tokens took 59.4 us as they came, 51.4 so,
-// 256 rows of 8 nodes 122.3 and 115.4 (equal ones 109.8 and 111.7), 576 rows of 100 to 1700 tokens 105.4 and 103.9 (all 576 in
-// order, with four times the rows a wave: 102, but equal rows lost 5 %).  Rows are told apart by eighths of octaves below the
-// table's length, 64 of them, and stand in their own order within one: each wave counts a part of them in LDS, and the wave
-// whose count the k-th falls into finds it.
+// of their numbers, and the last to start should be short: 250 rows of 200 to 1200 tokens took 57.3 us as they came, 48.5 so,
+// 256 rows of 8 nodes 121.3 and 110.7 (equal ones 106.3 and 107.8, over the 8-bit pool 61.8 and 64.4), 576 rows of 100 to 1700
+// tokens 119.4 and 110.0 (all 576 in order, with four times the rows a wave, gained 2 % more, but equal rows lost 5 %).  Rows are
+// told apart by eighths of octaves below the table's length, 64 of them, and stand in their own order within one: each wave counts
+// a part of them in LDS, and the wave whose count the k-th falls into finds it.
 template <int kW>
 __device__ __forceinline__ int kth_longest(const TreeArgs& a, int row0, int k, int wave) {
   __shared__ int s_count[kW][64];
@@ -1125,7 +1126,7 @@ __global__ __launch_bounds__(64 * kW, kMT == 2 || (kMode == kTree && kChunked) ?
     if constexpr (kMode == kTree) {
       // A wave that has own steps takes them first.  Chunks, which are few, ask for their keys ahead of them; where the chip is
       // full the registers that this takes would cost every compute unit its third workgroup (256 rows x 600 tokens x 8 nodes
-      // over the 8-bit pool: 67.0 us with three, 70.7 with two; one row of four nodes: 0.4 us the other way).
+      // over the 8-bit pool: 64.4 us with three, 67.6 with two; one row of four nodes: 0.5 us the other way).
       constexpr bool kEarly = kChunked && (kFp8 || kMT == 1);
       auto own_steps = [&]() __attribute__((always_inline)) {
         turn_signs(q);
@@ -1241,13 +1242,13 @@ Plan plan_of(int batch, int nodes, int hq, int hkv, int64_t capacity) {
   p.mblocks = (M + 16 * tiles - 1) / (16 * tiles);
   p.units = batch;
   // Whole rows take one launch, but the longest row's steps follow each other on one compute unit; chunks cost the join (3.7 us)
-  // and records.  Rows of one length, us whole and in chunks: 8 workgroups of 512 tokens 7.6 and 9.0, of 1000 11.0 and 9.1; 64 of
-  // 1000 11.9 and 11.2; 128 of 1000 13.9 and 15.3, of 2000 22.6 and 19.4; 256 of 1000 15.0 and 19.3.  Ragged rows leave whole ones
-  // waiting for the longest: 192 workgroups of up to 1373 tokens 15.8 and 13.9, 256 of up to 1725 (13 nodes) 21.4 and 19.2, but 512
-  // of up to 1500 20.0 and 24.4.  Rows that are more than the chip holds at once balance by themselves.
+  // and records.  Rows of one length, us whole and in chunks: 8 workgroups of 512 tokens 7.5 and 8.2, of 1000 11.1 and 8.4; 64 of
+  // 1000 11.5 and 11.0; 128 of 1000 12.1 and 12.7, of 2000 20.5 and 18.2; 256 of 1000 13.7 and 18.1.  Ragged rows leave whole ones
+  // waiting for the longest: 192 workgroups of up to 1373 tokens 15.0 and 12.8, 256 of up to 1725 (13 nodes) 23.4 and 19.1, but 512
+  // of up to 1500 18.9 and 23.2.  Rows that are more than the chip holds at once balance by themselves.
   const int64_t groups = (int64_t)batch * hkv * p.mblocks;
   if (batch > 1024 || capacity * num_cus() <= 700 * (num_cus() + groups)) return p;
-  // (Three workgroups a compute unit: decode within 3 %, trees of 32 query rows a fifth slower.)
+  // (Three workgroups a compute unit: decode 3 % slower, trees of 32 query rows 6 to 25 %.)
   auto target = [&](int each) {
     const int slots = each * num_cus() / (hkv * p.mblocks);
     return std::max({1, slots - batch / 2, slots / 2});

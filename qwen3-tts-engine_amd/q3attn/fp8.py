@@ -7,7 +7,8 @@ finite are held as NaN).  A row takes 129 bytes instead of 256.  The scale being
 number, and attention over the pool is attention over the bf16 rows that ``paged_read_fp8`` returns.
 
 The ops are registered from C++ (binding/torch_ops.cpp), where their arguments are checked, enqueue on the tensors' device's
-current stream, allocate only through torch's caching allocator and never synchronise.  GPU only.
+current stream, allocate only through torch's caching allocator and never synchronise.  GPU only.  None has a backward (one that is
+asked for raises), and those that write into caches count as in-place operations on them.
 """
 from __future__ import annotations
 
