@@ -475,7 +475,7 @@ int q3a_paged_read_fp8(const void* k_cache, const void* v_cache, int64_t kv_stri
  * Decode attention over the 8-bit pool: q3a_paged_decode's semantics (rows with ctx <= 0 give zeros, ctx is clamped to
  * max_pages_per_seq * page_size, a page index outside [0, num_pages) contributes no tokens) for any Hq that is a multiple of
  * Hkv, up to 16 query heads to a KV head and 64 KV heads.  q and out [B, Hq, 128] bf16; a query head with an element that is not
- * finite gives NaN.
+ * finite gives NaN where it sees a token.
  *
  * The append form quantises k_new, v_new [B, Hkv, 128] bf16 into position cache_seqlens[b] of row b as
  * q3a_paged_write_fp8 does, and attends over tokens 0 .. cache_seqlens[b], the new one with the value that the pool now holds.
