@@ -31,8 +31,9 @@ extern "C" {
  * q3a_cp_attn_append_rope.  7: the decode path codes below (negative split_tokens).  8: per-frame decode plans
  * (q3a_paged_decode_plan_bytes, q3a_paged_decode_plan, Q3A_DECODE_PLANNED).  9: the 8-bit pool (q3a_paged_write_fp8,
  * q3a_paged_read_fp8, q3a_paged_decode_fp8, q3a_paged_decode_fp8_append) and q3a_paged_decode_tree with its workspace
- * query. */
-#define Q3A_ABI_VERSION 9
+ * query.  10: the 4-bit pool (q3a_paged_write_fp4, q3a_paged_read_fp4, q3a_paged_decode_fp4, q3a_paged_decode_fp4_append) and the
+ * moves of pages and tokens (q3a_paged_copy, q3a_paged_compact). */
+#define Q3A_ABI_VERSION 10
 
 /* Decode decomposition codes, passed as split_tokens to the q3a_paged_decode* entry points (0 lets the library
  * choose, a positive multiple of 16 is a fixed split of that many tokens):
@@ -503,6 +504,95 @@ int q3a_paged_decode_fp8_append(
     int64_t scale_stride_head, int num_pages, int page_size, const int32_t* cache_seqlens, const int32_t* block_table,
     int64_t bt_stride_b, int max_pages_per_seq, void* out, int64_t o_stride_b, int64_t o_stride_h, void* workspace,
     size_t workspace_bytes, int batch, int num_q_heads, int num_kv_heads, int head_dim, float softmax_scale, void* stream);
+
+/*
+ * The 4-bit K/V pool.
+ *
+ *   k_cache, v_cache  [num_pages, page_size, Hkv, 64] bytes of two e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives;
+ *                     dim 2 i in byte i's low half), strides in bytes, dim stride 1, shared by the two pools
+ *   k_scale, v_scale  [num_pages, Hkv, 4, page_size] one exponent byte s per token and block of 32 dims, strides scale_stride_page /
+ *                     scale_stride_head, a block's tokens contiguous and the blocks page_size apart, shared
+ *
+ * An element is code * 2^(s - 127); all 32 of a block with s = 255 are NaN.  A written block gets the smallest power of two
+ * 2^(s-127), s in [2, 252], with max |x_d| <= 7 * 2^(s-127), and codes e2m1(x_d * 2^(127-s)) rounded to nearest even, at most 6 in
+ * magnitude; a block with an element that is not finite gets s = 255 and codes 0.  Every value read back is a bf16 number, so
+ * attention over the pool is attention over the bf16 rows read back.  Bytes 0, 1, 253 and 254 are not written and stand for no value.
+ * Requirements: page_size a multiple of 16 (at most 2^26), caches 16-byte aligned with strides multiples of 16, token stride in
+ * [64, 2^26]; scales 4-byte aligned with strides multiples of 4.  Slots, tokens and limits as for the 8-bit pool's write and read.
+ */
+int q3a_paged_write_fp4(const void* k, int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
+                        int64_t v_stride_h, const int64_t* slots, void* k_cache, void* v_cache, int64_t kv_stride_page,
+                        int64_t kv_stride_tok, int64_t kv_stride_head, void* k_scale, void* v_scale,
+                        int64_t scale_stride_page, int64_t scale_stride_head, int num_pages, int page_size,
+                        int64_t num_tokens, int num_kv_heads, int head_dim, void* stream);
+int q3a_paged_read_fp4(const void* k_cache, const void* v_cache, int64_t kv_stride_page, int64_t kv_stride_tok,
+                       int64_t kv_stride_head, const void* k_scale, const void* v_scale, int64_t scale_stride_page,
+                       int64_t scale_stride_head, int num_pages, int page_size, const int64_t* slots, void* k,
+                       int64_t k_stride_t, int64_t k_stride_h, void* v, int64_t v_stride_t, int64_t v_stride_h,
+                       int64_t num_tokens, int num_kv_heads, int head_dim, void* stream);
+
+/*
+ * Decode attention over the 4-bit pool: everything as for q3a_paged_decode_fp8 and its append form, whose new row is quantised as
+ * q3a_paged_write_fp4 does.  workspace: q3a_paged_decode_tree_workspace_bytes(batch, 1, ...) bytes.
+ */
+int q3a_paged_decode_fp4(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k_cache, const void* v_cache,
+                         int64_t kv_stride_page, int64_t kv_stride_tok, int64_t kv_stride_head, const void* k_scale,
+                         const void* v_scale, int64_t scale_stride_page, int64_t scale_stride_head, int num_pages,
+                         int page_size, const int32_t* cache_seqlens, const int32_t* block_table, int64_t bt_stride_b,
+                         int max_pages_per_seq, void* out, int64_t o_stride_b, int64_t o_stride_h, void* workspace,
+                         size_t workspace_bytes, int batch, int num_q_heads, int num_kv_heads, int head_dim,
+                         float softmax_scale, void* stream);
+int q3a_paged_decode_fp4_append(
+    const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k_new, int64_t kn_stride_b, int64_t kn_stride_h,
+    const void* v_new, int64_t vn_stride_b, int64_t vn_stride_h, void* k_cache, void* v_cache, int64_t kv_stride_page,
+    int64_t kv_stride_tok, int64_t kv_stride_head, void* k_scale, void* v_scale, int64_t scale_stride_page,
+    int64_t scale_stride_head, int num_pages, int page_size, const int32_t* cache_seqlens, const int32_t* block_table,
+    int64_t bt_stride_b, int max_pages_per_seq, void* out, int64_t o_stride_b, int64_t o_stride_h, void* workspace,
+    size_t workspace_bytes, int batch, int num_q_heads, int num_kv_heads, int head_dim, float softmax_scale, void* stream);
+
+/*
+ * Copies whole pages inside caches: page dst[i] becomes what page src[i] is, for each of num_pairs pairs in each of num_caches caches
+ * (a pool's layers, their K and V, and their scales) in as few launches as their addresses take: 128 caches of up to 4 shapes in a row
+ * each.  For forks of a sequence, whose last page each of them goes on writing, for pages that move together, and for a page that is
+ * shared and about to be written.  No counterpart in the reference, whose seats own fixed pages (engine/talker.py:23-31, 42).
+ *
+ *   caches   host array.  A page of a cache is n_1 x n_0 runs of run_bytes, stride_1 and stride_0 apart, and pages are stride_page
+ *            apart, all in bytes and multiples of 4 (of 16 in every cache: faster); num_pages of the cache
+ *   src, dst device int32 [num_pairs]
+ *
+ * A pair with a page outside [0, num_pages) of a cache, or onto itself, is left out there.  A page may be the source of many pairs.
+ * A page that is the destination of two pairs, or of one and the source of another, holds a mix afterwards.  At most 8 GiB a cache
+ * in one call.
+ */
+typedef struct {
+  void* base;
+  int64_t stride_page, stride_1, stride_0, n_1, n_0, run_bytes;
+  int num_pages;
+} q3a_page_cache;
+int q3a_paged_copy(const q3a_page_cache* caches, int num_caches, const int32_t* src, const int32_t* dst, int64_t num_pairs,
+                   void* stream);
+
+/*
+ * Moves the kept tokens of each row to the front of its pages, in order and in place, in every cache of a list: for long streams that
+ * let go of tokens, and for drafted tokens that were written and rejected.  No counterpart in the reference, whose seats only grow.
+ *
+ * Row b holds cache_seqlens[b] tokens (at most max_pages_per_seq * page_size) in the pages of its table.  Token t is kept if
+ * keep[b * keep_stride_b + t] != 0, or t >= keep_width.  The j-th kept token goes to place j; new_seqlens[b] (device, [batch], not
+ * the memory of cache_seqlens) gets their number, or cache_seqlens[b] where that is 0 or less.  What lies behind the last kept token stays as it was.  A token
+ * whose page, or whose place's page, is outside [0, num_pages) is not moved, but counted.  Pages from a row's first gap on must be no
+ * other row's of the call.
+ *
+ *   caches   host array of num_caches device pointers, [num_pages, page_size, Hkv] rows of row_bytes (256, 128 or 64), strides in bytes
+ *            and multiples of 16, shared by all
+ *   scales   scale_blocks > 0: as many device pointers, [num_pages, Hkv, scale_blocks, page_size] bytes, blocks page_size apart
+ *            (128 bytes a row with 1, the 8-bit pool; 64 with 4, the 4-bit pool); else unused
+ * batch and Hkv at most 65,535 and 65,536, a table of at most 2^28 tokens a row.
+ */
+int q3a_paged_compact(void* const* caches, void* const* scales, int num_caches, int row_bytes, int scale_blocks, int64_t stride_page,
+                      int64_t stride_tok, int64_t stride_head, int64_t scale_stride_page, int64_t scale_stride_head, int num_pages,
+                      int page_size, const uint8_t* keep, int64_t keep_stride_b, int keep_width, const int32_t* cache_seqlens,
+                      const int32_t* block_table, int64_t bt_stride_b, int max_pages_per_seq, int32_t* new_seqlens, int batch,
+                      int num_kv_heads, void* stream);
 
 /*
  * Attention for trees of drafted tokens (speculative decoding's check of several candidate continuations in one pass) over

@@ -121,4 +121,8 @@ inline Divisor divisor(uint32_t d) {
 int check_fp8_pool(const char* who, const void* kc, const void* vc, int64_t sp, int64_t st, int64_t sh, const void* ks,
                    const void* vs, int64_t ss_p, int64_t ss_h, int num_pages, int page_size, int hkv);
 
+// Rows k, v [tokens, hkv, 128] of bf16 and their slots, as the pools' writes and reads take them (kv_fp8.hip).
+int check_pool_rows(const char* who, const void* k, const void* v, int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh,
+                    const void* slots, int64_t tokens, int hkv, int head_dim);
+
 }  // namespace q3a

@@ -139,9 +139,8 @@ int check_fp8_pool(const char* who, const void* kc, const void* vc, int64_t sp, 
   return Q3A_OK;
 }
 
-namespace {
-int check_rows(const char* who, const void* k, const void* v, int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh,
-               const void* slots, int64_t tokens, int hkv, int head_dim) {
+int check_pool_rows(const char* who, const void* k, const void* v, int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh,
+                    const void* slots, int64_t tokens, int hkv, int head_dim) {
   if (head_dim != kRowDims) return fail(Q3A_EINVAL, "%s: head_dim %d (only 128)", who, head_dim);
   if (tokens < 0 || hkv < 1 || hkv > 65536 || tokens > ((int64_t)1 << 28) / hkv)  // 8 lanes a row, 8 rows a wave: below 2^32
     return fail(Q3A_EINVAL, "%s: bad token count %lld for %d KV heads (at most 65536 heads and 2^28 rows)", who, (long long)tokens, hkv);
@@ -153,7 +152,6 @@ int check_rows(const char* who, const void* k, const void* v, int64_t k_st, int6
     return fail(Q3A_EINVAL, "%s: rows must be 16-byte aligned with strides multiples of 8 elements", who);
   return Q3A_OK;
 }
-}  // namespace
 }  // namespace q3a
 
 using namespace q3a;
@@ -164,7 +162,7 @@ extern "C" int q3a_paged_write_fp8(const void* k, int64_t k_stride_t, int64_t k_
                                    void* v_scale, int64_t scale_stride_page, int64_t scale_stride_head, int num_pages,
                                    int page_size, int64_t num_tokens, int num_kv_heads, int head_dim, void* stream) {
   const char* who = "q3a_paged_write_fp8";
-  int rc = check_rows(who, k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h, slots, num_tokens, num_kv_heads, head_dim);
+  int rc = check_pool_rows(who, k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h, slots, num_tokens, num_kv_heads, head_dim);
   if (rc != Q3A_OK) return rc;
   rc = check_fp8_pool(who, k_cache, v_cache, kv_stride_page, kv_stride_tok, kv_stride_head, k_scale, v_scale,
                       scale_stride_page, scale_stride_head, num_pages, page_size, num_kv_heads);
@@ -204,7 +202,7 @@ extern "C" int q3a_paged_read_fp8(const void* k_cache, const void* v_cache, int6
                                   int64_t v_stride_t, int64_t v_stride_h, int64_t num_tokens, int num_kv_heads,
                                   int head_dim, void* stream) {
   const char* who = "q3a_paged_read_fp8";
-  int rc = check_rows(who, k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h, slots, num_tokens, num_kv_heads, head_dim);
+  int rc = check_pool_rows(who, k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h, slots, num_tokens, num_kv_heads, head_dim);
   if (rc != Q3A_OK) return rc;
   rc = check_fp8_pool(who, k_cache, v_cache, kv_stride_page, kv_stride_tok, kv_stride_head, k_scale, v_scale,
                       scale_stride_page, scale_stride_head, num_pages, page_size, num_kv_heads);

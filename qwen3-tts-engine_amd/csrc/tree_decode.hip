@@ -27,7 +27,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "fp8_common.h"
+#include "fp4_common.h"
 #include "../../include/q3attn.h"
 
 namespace q3a {
@@ -39,6 +39,7 @@ constexpr int kWindow = 32;     // steps whose page ids a wave holds at once (on
 constexpr int kMergeRow = kD + 4;  // floats per row of the merge buffer (16-byte rows off the bank period)
 constexpr int kRecord = kD + 2;    // floats per query row of a record: o[128], m, l
 enum { kNoKeys = 0, kTree = 1, kAppend = 2 };
+enum { kBf16Pool = 0, kFp8Pool = 1, kFp4Pool = 2 };
 
 typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8_t;
 typedef __attribute__((__vector_size__(4 * sizeof(float)))) float f32x4_t;
@@ -102,32 +103,55 @@ __device__ __forceinline__ const TreeArgs& args_again() {
 }
 
 // The first of the 8 dims that MFMA step c's operand holds in quarter g, and the 16 B piece of the row it lies in.
-template <bool kFp8>
+template <int kPool>
 __device__ __forceinline__ int dim_of(int c, int g) {
-  return kFp8 ? (c >> 1) * 64 + g * 16 + (c & 1) * 8 : c * 32 + g * 8;
+  return kPool == kFp8Pool ? (c >> 1) * 64 + g * 16 + (c & 1) * 8 : kPool == kFp4Pool ? g * 32 + c * 8 : c * 32 + g * 8;
 }
 
-// A step's K and V in registers: the 8-bit pool's codes, or bf16.
-template <bool kFp8>
+// Bytes of a row of K or V in the pool.
+template <int kPool>
+__host__ __device__ constexpr int row_bytes() {
+  return kPool == kBf16Pool ? 2 * kD : kPool == kFp8Pool ? kD : kFp4Row;
+}
+
+// The key of a subtile that operand row 4 g + i stands for, whose scores S^T's register i holds on quarter g.  The 4-bit pool's rows
+// are half a line: there the four quarters' keys at one i are two pairs of neighbours, so that their loads take whole lines.
+template <int kPool>
+__device__ __forceinline__ int key_of(int g, int i) {
+  return kPool == kFp4Pool ? 8 * (g >> 1) + 2 * i + (g & 1) : 4 * g + i;
+}
+
+// A step's K and V in registers: the pool's codes, or bf16.
+template <int kPool>
 struct KeyTile;
 template <>
-struct KeyTile<true> {
+struct KeyTile<kFp4Pool> {
+  uint4 k[2];      // block g of the key of operand row l % 16
+  uint32_t ks[2];  // and its scale byte
+};
+template <>
+struct KeyTile<kFp8Pool> {
   i32x8_t k[2];
   uint32_t ks[2];  // scale byte of key l % 16
 };
 template <>
-struct KeyTile<false> {
+struct KeyTile<kBf16Pool> {
   uint4 k[2][4];
 };
-template <bool kFp8>
+template <int kPool>
 struct ValueTile;
 template <>
-struct ValueTile<true> {
+struct ValueTile<kFp4Pool> {
+  uint32_t v[2][4];  // dims 8 (l % 16) .. + 7 of keys key_of(g, 0 .. 3)
+  uint2 vs[2];       // their block's scale bytes of keys 8 (g / 2) .. + 7
+};
+template <>
+struct ValueTile<kFp8Pool> {
   uint2 v[2][4];
   uint32_t vs[2];  // scale bytes of keys 4 g .. 4 g + 3
 };
 template <>
-struct ValueTile<false> {
+struct ValueTile<kBf16Pool> {
   uint4 v[2][4];
 };
 
@@ -160,13 +184,13 @@ __device__ __forceinline__ Entry entry_of(int b, int step, int lane) {
   e.page = pi < a.max_pages ? page : -1;
   return e;
 }
-template <bool kFp8>
+template <int kPool>
 __device__ __forceinline__ Window window_of(const Entry& e, int L, bool on) {
   const TreeArgs& a = args_again();
   Window w = {0u, 0u, 0};
   if (on && (unsigned)e.page < (unsigned)a.num_pages) {
     w.at = (uint32_t)(((int64_t)e.page * a.sp + (int64_t)e.off * a.st) >> 4);
-    if constexpr (kFp8) w.sat = (uint32_t)(e.page * a.ss_p + e.off);
+    if constexpr (kPool != kBf16Pool) w.sat = (uint32_t)(e.page * a.ss_p + e.off);
     w.valid = max(0, min(16, L - e.tok));
   }
   return w;
@@ -220,13 +244,13 @@ constexpr int kNt = 2;
 // No branches and always the same loads, also for a step that is not there (its page ids are -1): only so does the compiler
 // know how many newer loads may be in flight when older ones are waited for, and not wait for all.
 // `live`: there is such a step; its places are not used else.  tokens: what the row has from the step on.
-template <bool kFp8>
+template <int kPool>
 __device__ __forceinline__ Place place_of(const Window& w, int slot, bool live, int tokens) {
   Place p;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     p.at[u] = (int64_t)(uint32_t)readlane((int)w.at, 2 * slot + u) << 4;
-    if constexpr (kFp8) p.sat[u] = (uint32_t)readlane((int)w.sat, 2 * slot + u);
+    if constexpr (kPool != kBf16Pool) p.sat[u] = (uint32_t)readlane((int)w.sat, 2 * slot + u);
     const int n = readlane(w.valid, 2 * slot + u), left = tokens - 16 * u;
     p.valid[u] = live ? (n < left ? n : left < 0 ? 0 : left) : 0;  // (min as a chain of scalar selects)
   }
@@ -234,33 +258,51 @@ __device__ __forceinline__ Place place_of(const Window& w, int slot, bool live, 
 }
 
 // Descriptors end with the last seen key: what lies past it is not read and comes as zeros.
-template <bool kFp8>
+template <int kPool>
 __device__ __forceinline__ uint32_t extent(const TreeArgs& a, int valid) {
-  return valid > 0 ? (uint32_t)(valid - 1) * (uint32_t)a.st + (kFp8 ? kD : 2 * kD) : 0u;
+  return valid > 0 ? (uint32_t)(valid - 1) * (uint32_t)a.st + row_bytes<kPool>() : 0u;
+}
+// The same of a subtile's scale bytes: of the 4-bit pool's blocks, each has its page's tokens after the last one's.
+template <int kPool>
+__device__ __forceinline__ int scale_extent(const TreeArgs& a, int valid) {
+  return valid > 0 ? (kPool == kFp4Pool ? (kFp4Blocks - 1) * a.page_size : 0) + 16 : 0;
 }
 
 template <bool kOnce>
-__device__ __forceinline__ void load_k(const TreeArgs& a, const Place& p, int lane, KeyTile<true>& x) {
+__device__ __forceinline__ void load_k(const TreeArgs& a, const Place& p, int lane, KeyTile<kFp4Pool>& x) {
+  const int r = lane & 15, g = lane >> 4, key = key_of<kFp4Pool>(r >> 2, r & 3);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const auto rk = make_rsrc(a.kc + p.at[u], extent<kFp4Pool>(a, p.valid[u]));
+    x.k[u] = __builtin_bit_cast(
+        uint4, __builtin_amdgcn_raw_buffer_load_b128(rk, (int)((uint32_t)key * (uint32_t)a.st + 16 * g), 0, kOnce ? kNt : 0));
+    const auto rs = make_rsrc(a.ks + p.sat[u], scale_extent<kFp4Pool>(a, p.valid[u]));
+    x.ks[u] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rs, g * a.page_size + key, 0, 0);
+  }
+}
+
+template <bool kOnce>
+__device__ __forceinline__ void load_k(const TreeArgs& a, const Place& p, int lane, KeyTile<kFp8Pool>& x) {
   const int r = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    const auto rk = make_rsrc(a.kc + p.at[u], extent<true>(a, p.valid[u]));
+    const auto rk = make_rsrc(a.kc + p.at[u], extent<kFp8Pool>(a, p.valid[u]));
     const uint32_t row = kOnce ? (uint32_t)(r & ~1) * (uint32_t)a.st + 64 * (r & 1) + 16 * g : (uint32_t)r * (uint32_t)a.st + 16 * g;
     auto ld = [&](uint32_t o) {
       return __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rk, (int)o, 0, kOnce ? kNt : 0));
     };
     x.k[u] = __builtin_shufflevector(ld(row), ld(row + (kOnce ? (uint32_t)a.st : 64u)), 0, 1, 2, 3, 4, 5, 6, 7);
-    const auto rs = make_rsrc(a.ks + p.sat[u], p.valid[u] > 0 ? 16 : 0);
+    const auto rs = make_rsrc(a.ks + p.sat[u], scale_extent<kFp8Pool>(a, p.valid[u]));
     x.ks[u] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rs, r, 0, 0);
   }
 }
 template <bool kPaired>
-__device__ __forceinline__ void load_k(const TreeArgs& a, const Place& p, int lane, KeyTile<false>& x) {
+__device__ __forceinline__ void load_k(const TreeArgs& a, const Place& p, int lane, KeyTile<kBf16Pool>& x) {
   const int r = lane & 15, g = lane >> 4;
   const uint32_t st = (uint32_t)a.st;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    const auto rk = make_rsrc(a.kc + p.at[u], extent<false>(a, p.valid[u]));
+    const auto rk = make_rsrc(a.kc + p.at[u], extent<kBf16Pool>(a, p.valid[u]));
     if constexpr (kPaired) {
       const uint32_t row = (uint32_t)((r & ~3) + ((r >> 1) & 1)) * st + 64 * (r & 1) + 16 * g;
 #pragma unroll
@@ -274,31 +316,54 @@ __device__ __forceinline__ void load_k(const TreeArgs& a, const Place& p, int la
   }
 }
 
-template <bool kFp8, bool kOnce>
-__device__ __forceinline__ void load_v(const TreeArgs& a, const Place& p, int lane, ValueTile<kFp8>& x) {
+template <int kPool, bool kOnce>
+__device__ __forceinline__ void load_v(const TreeArgs& a, const Place& p, int lane, ValueTile<kPool>& x) {
   const int r = lane & 15, g = lane >> 4;
   const uint32_t st = (uint32_t)a.st;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    const auto rv = make_rsrc(a.vc + p.at[u], extent<kFp8>(a, p.valid[u]));
-    const uint32_t row = (uint32_t)(4 * g) * st + (kFp8 ? 8 : 16) * r;
+    const auto rv = make_rsrc(a.vc + p.at[u], extent<kPool>(a, p.valid[u]));
+    const uint32_t row = (uint32_t)key_of<kPool>(g, 0) * st + row_bytes<kPool>() / 16 * r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if constexpr (kFp8) {
+      if constexpr (kPool == kFp4Pool) {
+        x.v[u][i] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rv, (int)(row + 2 * i * st), 0, kOnce ? kNt : 0);
+      } else if constexpr (kPool == kFp8Pool) {
         x.v[u][i] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rv, (int)(row + i * st), 0, kOnce ? kNt : 0));
       } else {
         x.v[u][i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rv, (int)(row + i * st), 0, kOnce ? kNt : 0));
       }
     }
-    if constexpr (kFp8) {
-      const auto rt = make_rsrc(a.vs + p.sat[u], p.valid[u] > 0 ? 16 : 0);
-      x.vs[u] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rt, 4 * g, 0, 0);
+    if constexpr (kPool != kBf16Pool) {
+      const auto rt = make_rsrc(a.vs + p.sat[u], scale_extent<kPool>(a, p.valid[u]));
+      if constexpr (kPool == kFp4Pool) {
+        x.vs[u] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rt, (r >> 2) * a.page_size + 8 * (g >> 1), 0, 0));
+      } else {
+        x.vs[u] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rt, 4 * g, 0, 0);
+      }
     }
   }
 }
 
 // The A operands of O^T for dims 8 i + j, j = jj and jj + 1 (jj even): the pairs of keys (0, 1), (2, 3) of both subtiles.
-__device__ __forceinline__ void v_operands(const ValueTile<true>& x, int jj, bf16x8_t& a0, bf16x8_t& a1) {
+// (f: the scales of the lane's 8 keys, which the 4-bit pool's V takes along and the 8-bit pool's leaves to P.)
+__device__ __forceinline__ uint32_t fp4_pair_at(uint32_t w, int byte, float f) {
+  return byte == 0 ? fp4_pair<0>(w, f) : byte == 1 ? fp4_pair<1>(w, f) : byte == 2 ? fp4_pair<2>(w, f) : fp4_pair<3>(w, f);
+}
+__device__ __forceinline__ void v_operands(const ValueTile<kFp4Pool>& x, const float (&f)[2][4], int jj, bf16x8_t& a0, bf16x8_t& a1) {
+  uint32_t p0[4], p1[4];
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const uint32_t w0 = fp4_pair_at(x.v[u][2 * p], jj >> 1, f[u][2 * p]), w1 = fp4_pair_at(x.v[u][2 * p + 1], jj >> 1, f[u][2 * p + 1]);
+      p0[2 * u + p] = perm_b32(w1, w0, kPermLoLo);
+      p1[2 * u + p] = perm_b32(w1, w0, kPermHiHi);
+    }
+  a0 = __builtin_bit_cast(bf16x8_t, make_uint4(p0[0], p0[1], p0[2], p0[3]));
+  a1 = __builtin_bit_cast(bf16x8_t, make_uint4(p1[0], p1[1], p1[2], p1[3]));
+}
+__device__ __forceinline__ void v_operands(const ValueTile<kFp8Pool>& x, const float (&)[2][4], int jj, bf16x8_t& a0, bf16x8_t& a1) {
   uint32_t p0[4], p1[4];
 #pragma unroll
   for (int u = 0; u < 2; ++u)
@@ -315,7 +380,7 @@ __device__ __forceinline__ void v_operands(const ValueTile<true>& x, int jj, bf1
   a1 = __builtin_bit_cast(bf16x8_t, make_uint4(p1[0], p1[1], p1[2], p1[3]));
 }
 __device__ __forceinline__ uint32_t word_of(const uint4& w, int i) { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
-__device__ __forceinline__ void v_operands(const ValueTile<false>& x, int jj, bf16x8_t& a0, bf16x8_t& a1) {
+__device__ __forceinline__ void v_operands(const ValueTile<kBf16Pool>& x, const float (&)[2][4], int jj, bf16x8_t& a0, bf16x8_t& a1) {
   uint32_t p0[4], p1[4];
 #pragma unroll
   for (int u = 0; u < 2; ++u)
@@ -343,7 +408,7 @@ struct Query {
 // wrong; two products where they do hold a wave's queries, and this where not, took longer than this alone: 83.2 us for 82.0, 6 long
 // rows x 63 nodes, 19.9 for 19.0, 32 rows x 13 nodes, 8.8 for 8.3, one row x 1000.)
 template <bool kSwapped, int kMT>
-__device__ __forceinline__ void scores(const KeyTile<true>& x, const Query<kMT>& q, f32x4_t (&s)[kMT][2]) {
+__device__ __forceinline__ void scores(const KeyTile<kFp8Pool>& x, const Query<kMT>& q, f32x4_t (&s)[kMT][2]) {
   const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -370,8 +435,26 @@ __device__ __forceinline__ void scores(const KeyTile<true>& x, const Query<kMT>&
     }
   }
 }
+// 4-bit keys likewise: a lane's 32 codes are one block, so the conversion takes its exponent along.
+template <bool kAsLoaded, int kMT>
+__device__ __forceinline__ void scores(const KeyTile<kFp4Pool>& x, const Query<kMT>& q, f32x4_t (&s)[kMT][2]) {
+  const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const float f = fp8_scale(x.ks[u]);
+    const uint32_t k[4] = {x.k[u].x, x.k[u].y, x.k[u].z, x.k[u].w};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const bf16x8_t kf = __builtin_bit_cast(
+          bf16x8_t, make_uint4(fp4_pair<0>(k[c], f), fp4_pair<1>(k[c], f), fp4_pair<2>(k[c], f), fp4_pair<3>(k[c], f)));
+#pragma unroll
+      for (int t = 0; t < kMT; ++t)
+        s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q.v[t][c], c == 0 ? zero : s[t][u], 0, 0, 0);
+    }
+  }
+}
 template <bool kPaired, int kMT>
-__device__ __forceinline__ void scores(const KeyTile<false>& x, const Query<kMT>& q, f32x4_t (&s)[kMT][2]) {
+__device__ __forceinline__ void scores(const KeyTile<kBf16Pool>& x, const Query<kMT>& q, f32x4_t (&s)[kMT][2]) {
   const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -413,7 +496,7 @@ __device__ __forceinline__ float larger(float a, float b) { return __builtin_ele
 // product with the largest V stays finite.
 constexpr float kAhead = 4.f;
 
-template <bool kMasked, int kMT>
+template <int kPool, bool kMasked, int kMT>
 __device__ __forceinline__ void softmax(const int (&valid)[2], const uint32_t (&seen)[kMT], float scale, float ahead,
                                         f32x4_t (&s)[kMT][2], State<kMT>& st) {
   const bool full = valid[0] == 16 && valid[1] == 16;
@@ -425,7 +508,7 @@ __device__ __forceinline__ void softmax(const int (&valid)[2], const uint32_t (&
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const bool ok = kMasked ? ((seen[t] >> (4 * u + i)) & 1) != 0 : 4 * g + i < valid[u];
+          const bool ok = kMasked ? ((seen[t] >> (4 * u + i)) & 1) != 0 : key_of<kPool>(g, i) < valid[u];
           s[t][u][i] = ok ? s[t][u][i] : -INFINITY;
         }
   }
@@ -469,13 +552,30 @@ __device__ __forceinline__ void softmax(const int (&valid)[2], const uint32_t (&
 // each probability is left) and reach the 0.0017.  The second product takes nothing where HBM is the bound (576 rows 96.8 and
 // 97.0 us), a little of 32 rows x 13 nodes (18.2 -> 18.9) and more of 6 long rows x 63 nodes (76.1 -> 85.5), which vector
 // instructions bound.
-// Over the 8-bit pool the first part is rounded to nearest.  Over bf16, whose V may hold infinities, both parts of a probability
+// Over the pools of codes the first part is rounded to nearest.  Over bf16, whose V may hold infinities, both parts of a probability
 // over 0 have to be over 0, that no product of 0 and an infinity makes a NaN: the first is cut off from the next smaller number.
-template <bool kFp8, int kMT>
-__device__ __forceinline__ void values(const ValueTile<kFp8>& x, const int (&valid)[2], int lane, const f32x4_t (&p)[kMT][2],
+template <int kPool, int kMT>
+__device__ __forceinline__ void values(const ValueTile<kPool>& x, const int (&valid)[2], int lane, const f32x4_t (&p)[kMT][2],
                                        State<kMT>& st) {
   const int g = lane >> 4;
   float f[2][4];  // V's scales
+  constexpr bool kFp8 = kPool == kFp8Pool;
+  if constexpr (kPool == kFp4Pool) {
+    uint32_t bytes[2];  // of the lane's keys: every second one of 8
+#pragma unroll
+    for (int u = 0; u < 2; ++u) bytes[u] = perm_b32(x.vs[u].y, x.vs[u].x, (g & 1) != 0 ? 0x07050301u : 0x06040200u);
+    if (valid[0] != 16 || valid[1] != 16) {  // the scale byte of a key that is not seen may be anything
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int left = max(0, min(4, (valid[u] - key_of<kPool>(g, 0) + 1) >> 1));
+        bytes[u] &= (uint32_t)((1ull << (8 * left)) - 1);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[u][i] = fp8_scale((bytes[u] >> (8 * i)) & 0xffu);
+  }
   if constexpr (kFp8) {
     uint32_t bytes[2] = {x.vs[0], x.vs[1]};
     if (valid[0] != 16 || valid[1] != 16) {  // the scale byte of a key that is not seen may be anything
@@ -500,7 +600,7 @@ __device__ __forceinline__ void values(const ValueTile<kFp8>& x, const int (&val
       for (int i = 0; i < 4; i += 2) {
         const float a = kFp8 ? p[t][u][i] * f[u][i] : p[t][u][i], b = kFp8 ? p[t][u][i + 1] * f[u][i + 1] : p[t][u][i + 1];
         const int w = 2 * u + (i >> 1);
-        if constexpr (kFp8) {
+        if constexpr (kPool != kBf16Pool) {
           h[w] = pack_bf16x2(a, b);
           r[w] = pack_bf16x2(a - bf16_lo(h[w]), b - bf16_hi(h[w]));
         } else {
@@ -516,7 +616,7 @@ __device__ __forceinline__ void values(const ValueTile<kFp8>& x, const int (&val
 #pragma unroll
   for (int jj = 0; jj < 8; jj += 2) {
     bf16x8_t a0, a1;
-    v_operands(x, jj, a0, a1);
+    v_operands(x, f, jj, a0, a1);
 #pragma unroll
     for (int t = 0; t < kMT; ++t) {
       st.o[t][jj] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, lo[t], st.o[t][jj], 0, 0, 0);
@@ -544,6 +644,7 @@ __device__ __forceinline__ uint32_t halves_of_kind(uint32_t w, int kind) {
 template <int kMT>
 __device__ __forceinline__ void add_not_finite(const uint16_t* vb, int ts, const uint32_t (&seen)[kMT], State<kMT>& st) {
   const TreeArgs& a = args_again();
+  const float none[2][4] = {};
   bf16x8_t sees[kMT];
 #pragma unroll
   for (int t = 0; t < kMT; ++t) {
@@ -557,7 +658,7 @@ __device__ __forceinline__ void add_not_finite(const uint16_t* vb, int ts, const
   for (int kind = 0; kind < 3; ++kind) {
     const int lane = lane_now();  // (nothing of the elements is computed ahead of the loop)
     const float what = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __builtin_nanf("");
-    ValueTile<false> x;
+    ValueTile<kBf16Pool> x;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -570,7 +671,7 @@ __device__ __forceinline__ void add_not_finite(const uint16_t* vb, int ts, const
 #pragma unroll
     for (int jj = 0; jj < 8; jj += 2) {
       bf16x8_t a[2];
-      v_operands(x, jj, a[0], a[1]);
+      v_operands(x, none, jj, a[0], a[1]);
 #pragma unroll
       for (int t = 0; t < kMT; ++t)
 #pragma unroll
@@ -587,21 +688,21 @@ __device__ __forceinline__ void add_not_finite(const uint16_t* vb, int ts, const
 // The nodes' own keys 32 ts .. + 31, in bf16, with each lane's query rows' view of its 8 keys.  An own V element that is
 // not finite must not reach the rows that do not see its key (0 * inf in the product): such elements are zeroed in the
 // product and added afterwards for the rows that see them.
-template <bool kFp8, int kMT>
+template <int kPool, int kMT>
 __device__ __forceinline__ void tree_step(const Work& w, int ts, const Query<kMT>& q, State<kMT>& st) {
   const int lane = lane_now();
   const int r = lane & 15, g = lane >> 4;
   const TreeArgs& a = args_again();
   const uint16_t* kb = a.kn + (int64_t)w.b * a.kn_sb + (int64_t)w.h * a.kn_sh;
   const uint16_t* vb = a.vn + (int64_t)w.b * a.vn_sb + (int64_t)w.h * a.vn_sh;
-  KeyTile<false> x;
-  ValueTile<false> y;
+  KeyTile<kBf16Pool> x;
+  ValueTile<kBf16Pool> y;
   // Rows past the last node read the last one's, without a branch: no query row sees them, and their V is zeroed.
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int j = min(kStep * ts + 16 * u + r, a.nodes - 1);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) x.k[u][c] = ld16(kb + (int64_t)j * a.kn_sn + dim_of<kFp8>(c, g));
+    for (int c = 0; c < 4; ++c) x.k[u][c] = ld16(kb + (int64_t)j * a.kn_sn + dim_of<kPool>(c, g));
   }
 #pragma unroll
   for (int u = 0; u < 2; ++u)
@@ -640,7 +741,7 @@ __device__ __forceinline__ void tree_step(const Work& w, int ts, const Query<kMT
   const int any[2] = {16, 16};
   f32x4_t sc[kMT][2];
   scores<false, kMT>(x, q, sc);
-  softmax<true, kMT>(any, seen, a.scale_log2, a.ahead, sc, st);
+  softmax<kBf16Pool, true, kMT>(any, seen, a.scale_log2, a.ahead, sc, st);
   uint32_t top = 0;
 #pragma unroll
   for (int u = 0; u < 2; ++u)
@@ -659,7 +760,7 @@ __device__ __forceinline__ void tree_step(const Work& w, int ts, const Query<kMT
         y.v[u][i] = make_uint4(finite_halves(e.x), finite_halves(e.y), finite_halves(e.z), finite_halves(e.w));
       }
   }
-  values<false, kMT>(y, any, lane, sc, st);
+  values<kBf16Pool, kMT>(y, any, lane, sc, st);
   if (any_odd) add_not_finite<kMT>(vb, ts, seen, st);
 }
 
@@ -669,7 +770,8 @@ __device__ __forceinline__ uint32_t row_max(uint32_t x) {
 }
 
 // The append form's new row, quantised as the write kernel does and stored, then attended as a cached subtile of one key.
-__device__ __forceinline__ void append_keys(const TreeArgs& a, const Work& w, bool store, KeyTile<true>& x, ValueTile<true>& y, int& valid) {
+__device__ __forceinline__ void append_keys(const TreeArgs& a, const Work& w, bool store, KeyTile<kFp8Pool>& x,
+                                            ValueTile<kFp8Pool>& y, int& valid) {
   const int lane = lane_now();
   const int r = lane & 15, g = lane >> 4;
   const TreeArgs& more = args_again();
@@ -681,7 +783,7 @@ __device__ __forceinline__ void append_keys(const TreeArgs& a, const Work& w, bo
   uint32_t kw[16], vw[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint4 e = ld16(kb + dim_of<true>(i, g));
+    const uint4 e = ld16(kb + dim_of<kFp8Pool>(i, g));
     kw[4 * i] = e.x;
     kw[4 * i + 1] = e.y;
     kw[4 * i + 2] = e.z;
@@ -733,13 +835,67 @@ __device__ __forceinline__ void append_keys(const TreeArgs& a, const Work& w, bo
     const int64_t at = (int64_t)page * a.sp + (int64_t)off * a.st;
     const int64_t sat = (int64_t)page * a.ss_p + off;
     if (r == 0) {
-      st16(a.kc + at + dim_of<true>(0, g), make_uint4(kc[0], kc[1], kc[2], kc[3]));
-      st16(a.kc + at + dim_of<true>(2, g), make_uint4(kc[4], kc[5], kc[6], kc[7]));
+      st16(a.kc + at + dim_of<kFp8Pool>(0, g), make_uint4(kc[0], kc[1], kc[2], kc[3]));
+      st16(a.kc + at + dim_of<kFp8Pool>(2, g), make_uint4(kc[4], kc[5], kc[6], kc[7]));
     }
     if (g == 0) *reinterpret_cast<u32x2*>(a.vc + at + 8 * r) = u32x2{vc[0], vc[1]};
     if (lane == 0) {
       a.ks[sat] = (uint8_t)ks;
       a.vs[sat] = (uint8_t)vs;
+    }
+  }
+}
+
+// The same into the 4-bit pool.  A lane of quarter g holds K's block g, whole; four lanes share a block of V.
+__device__ __forceinline__ void append_keys(const TreeArgs& a, const Work& w, bool store, KeyTile<kFp4Pool>& x,
+                                            ValueTile<kFp4Pool>& y, int& valid) {
+  const int lane = lane_now();
+  const int r = lane & 15, g = lane >> 4;
+  const TreeArgs& more = args_again();
+  const uint16_t* kb = more.kn + (int64_t)w.b * more.kn_sb + (int64_t)w.h * more.kn_sh;
+  const uint16_t* vb = more.vn + (int64_t)w.b * more.vn_sb + (int64_t)w.h * more.vn_sh;
+  const int pi = (int)divide((uint32_t)w.L, more.per_page), off = w.L - pi * more.page_size;
+  const int page = more.bt[(int64_t)w.b * more.bt_sb + pi];
+  const bool ok = (unsigned)page < (unsigned)a.num_pages;
+  uint32_t kw[16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint4 e = ld16(kb + dim_of<kFp4Pool>(i, g));
+    kw[4 * i] = e.x;
+    kw[4 * i + 1] = e.y;
+    kw[4 * i + 2] = e.z;
+    kw[4 * i + 3] = e.w;
+  }
+  const uint4 e = ld16(vb + 8 * r);
+  const uint32_t vw[4] = {e.x, e.y, e.z, e.w};
+  const uint32_t ks = fp4_scale_byte(halves_max(bf16_any_amax_pair(kw)));
+  const uint32_t vs = fp4_scale_byte(dpp_max_u32<kDppXor2>(dpp_max_u32<kDppXor1>(halves_max(bf16_any_amax_pair(vw)))));
+  uint32_t kc[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) kc[i] = fp4_codes8(kw[4 * i], kw[4 * i + 1], kw[4 * i + 2], kw[4 * i + 3], ks);
+  const uint32_t vc = fp4_codes8(vw[0], vw[1], vw[2], vw[3], vs);
+  const uint4 codes = make_uint4(kc[0], kc[1], kc[2], kc[3]);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    x.ks[u] = ks;
+    y.vs[u] = make_uint2(vs, 0u);
+    x.k[u] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y.v[u][i] = 0u;
+  }
+  valid = ok ? 1 : 0;
+  if (r == 0) x.k[0] = codes;
+  if (g == 0) y.v[0][0] = vc;
+  if (store && ok) {
+    const int64_t at = (int64_t)page * a.sp + (int64_t)off * a.st;
+    const int64_t sat = (int64_t)page * a.ss_p + off;
+    if (r == 0) {
+      st16(a.kc + at + 16 * g, codes);
+      a.ks[sat + g * a.page_size] = (uint8_t)ks;
+    }
+    if (g == 0) {
+      *reinterpret_cast<uint32_t*>(a.vc + at + 4 * r) = vc;
+      if ((r & 3) == 0) a.vs[sat + (r >> 2) * a.page_size] = (uint8_t)vs;
     }
   }
 }
@@ -756,7 +912,7 @@ __device__ __forceinline__ void clear(State<kMT>& st) {
 }
 
 // Q^T of the row's block of query rows as B operands; columns past the last query row have the last one's again.
-template <bool kFp8, int kMT>
+template <int kPool, int kMT>
 __device__ __forceinline__ void load_q(const Work& w, bf16x8_t (&q)[kMT][4]) {
   const int lane = lane_now();
   const TreeArgs& a = args_again();
@@ -767,23 +923,23 @@ __device__ __forceinline__ void load_q(const Work& w, bf16x8_t (&q)[kMT][4]) {
     const int n = node_of(a, m);
     const uint16_t* qp = a.q + (int64_t)w.b * a.q_sb + (int64_t)n * a.q_sn + (int64_t)(w.h * a.group + m - n * a.group) * a.q_sh;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) q[t][c] = __builtin_bit_cast(bf16x8_t, ld16(qp + dim_of<kFp8>(c, g)));
+    for (int c = 0; c < 4; ++c) q[t][c] = __builtin_bit_cast(bf16x8_t, ld16(qp + dim_of<kPool>(c, g)));
   }
 }
 
 // A wave's cached steps in registers: as soon as a step's K has been multiplied, the next step's K is loaded in its place, and
 // its V behind the V product.  (Two steps in registers ahead of the one computed were no faster, where they fitted.)
-template <bool kFp8, int kMT>
+template <int kPool, int kMT>
 struct Stream {
   static constexpr bool kOnce = kMT == 1;    // else other blocks of query rows may read the keys too
   static constexpr bool kLayout = kMT == 1;  // swapped, or paired
-  KeyTile<kFp8> k;
-  ValueTile<kFp8> v;
+  KeyTile<kPool> k;
+  ValueTile<kPool> v;
   int valid[2];
 
   __device__ __forceinline__ void load(const TreeArgs& a, const Place& p, int lane) {
     load_k<kOnce>(a, p, lane, k);
-    load_v<kFp8, kOnce>(a, p, lane, v);
+    load_v<kPool, kOnce>(a, p, lane, v);
     valid[0] = p.valid[0];
     valid[1] = p.valid[1];
   }
@@ -795,10 +951,10 @@ struct Stream {
     __builtin_amdgcn_sched_barrier(0);
     load_k<kOnce>(a, next, lane, k);
     __builtin_amdgcn_sched_barrier(0);
-    softmax<false, kMT>(valid, all, a.scale_log2, a.ahead, s, st);
-    values<kFp8, kMT>(v, valid, lane, s, st);
+    softmax<kPool, false, kMT>(valid, all, a.scale_log2, a.ahead, s, st);
+    values<kPool, kMT>(v, valid, lane, s, st);
     __builtin_amdgcn_sched_barrier(0);
-    load_v<kFp8, kOnce>(a, next, lane, v);
+    load_v<kPool, kOnce>(a, next, lane, v);
     __builtin_amdgcn_sched_barrier(0);
     valid[0] = next.valid[0];
     valid[1] = next.valid[1];
@@ -806,17 +962,17 @@ struct Stream {
 };
 
 // The append form's step: the new row.
-template <int kMT>
+template <int kPool, int kMT>
 __device__ __forceinline__ void append_step(const TreeArgs& a, const Work& w, const Query<kMT>& q, int lane, State<kMT>& st) {
   const uint32_t all[kMT] = {};
   f32x4_t s[kMT][2];
-  KeyTile<true> x;
-  ValueTile<true> y;
+  KeyTile<kPool> x;
+  ValueTile<kPool> y;
   int one[2] = {0, 0};
   append_keys(a, w, w.mb == 0, x, y, one[0]);
   scores<false, kMT>(x, q, s);
-  softmax<false, kMT>(one, all, a.scale_log2, a.ahead, s, st);
-  values<true, kMT>(y, one, lane, s, st);
+  softmax<kPool, false, kMT>(one, all, a.scale_log2, a.ahead, s, st);
+  values<kPool, kMT>(y, one, lane, s, st);
 }
 
 // Q, as it was loaded, with the sign that the scale asks for; an element that is not finite becomes NaN, as its row's result then is
@@ -1061,7 +1217,7 @@ __device__ __forceinline__ int kth_longest(const TreeArgs& a, int row0, int k, i
 
 // One workgroup a (row, KV head, block of 16 kMT query rows), its kW waves taking the row's steps in turn; or (kChunked) one of
 // a chunk of a row's steps, which leaves a record for the join kernel unless it is the row's only one.
-template <bool kFp8, int kMode, int kMT, int kW, bool kChunked>
+template <int kPool, int kMode, int kMT, int kW, bool kChunked>
 __global__ __launch_bounds__(64 * kW, kMT == 2 || (kMode == kTree && kChunked) ? 2 : 3) void tree_kernel(const TreeArgs args) {
   __shared__ __align__(16) MergeLds<kW> lds;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1089,16 +1245,16 @@ __global__ __launch_bounds__(64 * kW, kMT == 2 || (kMode == kTree && kChunked) ?
       reinterpret_cast<Joined*>(args_again().ws)[w.b] = Joined{unit - c.index, c.count};
     const int s = s0 + wave + kW * (lane >> 1);
     const Entry e = entry_of(w.b, s, lane);
-    load_q<kFp8, kMT>(w, q.v);
-    win = window_of<kFp8>(e, w.L, s < min(s1, w.Tc));
+    load_q<kPool, kMT>(w, q.v);
+    win = window_of<kPool>(e, w.L, s < min(s1, w.Tc));
   } else {
     w.b = unit;
     const int row0 = max(0, args.batch - 64 * kW);
     if (args.order && unit >= row0) w.b = kth_longest<kW>(args, row0, unit - row0, wave);
     // The first window's page ids do not wait for the row's length.
     const Entry e = entry_of(w.b, wave + kW * (lane >> 1), lane);
-    load_q<kFp8, kMT>(w, q.v);
-    win = window_of<kFp8>(e, INT_MAX, true);
+    load_q<kPool, kMT>(w, q.v);
+    win = window_of<kPool>(e, INT_MAX, true);
     w.L = __builtin_amdgcn_readfirstlane(row_tokens(w.b, kMode));
     w.Tc = w.L > 0 ? (w.L + kStep - 1) / kStep : 0;
     s1 = steps_of(w.L, kMode);
@@ -1118,20 +1274,20 @@ __global__ __launch_bounds__(64 * kW, kMT == 2 || (kMode == kTree && kChunked) ?
     auto place = [&](int j) __attribute__((always_inline)) {
       if ((j & (kWindow - 1)) == 0 && j > 0 && j < n) {
         const int l = lane_now();
-        win = window_of<kFp8>(entry_of(w.b, first + kW * (j + (l >> 1)), l), w.L, j + (l >> 1) < n);
+        win = window_of<kPool>(entry_of(w.b, first + kW * (j + (l >> 1)), l), w.L, j + (l >> 1) < n);
       }
-      return place_of<kFp8>(win, j & (kWindow - 1), j < n, w.L - kStep * (first + kW * j));
+      return place_of<kPool>(win, j & (kWindow - 1), j < n, w.L - kStep * (first + kW * j));
     };
-    Stream<kFp8, kMT> x;
+    Stream<kPool, kMT> x;
     if constexpr (kMode == kTree) {
       // A wave that has own steps takes them first.  Chunks, which are few, ask for their keys ahead of them; where the chip is
       // full the registers that this takes would cost every compute unit its third workgroup (256 rows x 600 tokens x 8 nodes
       // over the 8-bit pool: 64.4 us with three, 67.6 with two; one row of four nodes: 0.5 us the other way).
-      constexpr bool kEarly = kChunked && (kFp8 || kMT == 1);
+      constexpr bool kEarly = kChunked && (kPool != kBf16Pool || kMT == 1);
       auto own_steps = [&]() __attribute__((always_inline)) {
         turn_signs(q);
         clear(st);
-        for (int s = own; s < s1; s += kW) tree_step<kFp8, kMT>(w, s - w.Tc, q, st);
+        for (int s = own; s < s1; s += kW) tree_step<kPool, kMT>(w, s - w.Tc, q, st);
       };
       if constexpr (kEarly) {
         x.load(a, place(0), lane);
@@ -1149,7 +1305,7 @@ __global__ __launch_bounds__(64 * kW, kMT == 2 || (kMode == kTree && kChunked) ?
       turn_signs(q);
       clear(st);
       if constexpr (kMode == kAppend) {
-        if (own < s1) append_step<kMT>(a, w, q, lane, st);
+        if (own < s1) append_step<kPool, kMT>(a, w, q, lane, st);
       }
     }
     const TreeArgs again = at_head(args_again(), w.h);  // (not held in registers, and spilled, since the kernel's start)
@@ -1262,16 +1418,16 @@ Plan plan_of(int batch, int nodes, int hq, int hkv, int64_t capacity) {
   return p;
 }
 
-template <bool kFp8, int kMode, int kMT>
+template <int kPool, int kMode, int kMT>
 int launch(const TreeArgs& a, const char* who, hipStream_t stream) {
   hipError_t e;
   const unsigned heads = (unsigned)(a.hkv * a.mblocks), units = (unsigned)a.units;
   const dim3 grid = a.xcd_units ? dim3(8 * heads, (units + 7) / 8) : dim3(heads, units);
   if (a.target == 0) {
-    hipLaunchKernelGGL((tree_kernel<kFp8, kMode, kMT, kWaves, false>), grid, dim3(64 * kWaves), 0, stream, a);
+    hipLaunchKernelGGL((tree_kernel<kPool, kMode, kMT, kWaves, false>), grid, dim3(64 * kWaves), 0, stream, a);
     e = hipGetLastError();
   } else {
-    hipLaunchKernelGGL((tree_kernel<kFp8, kMode, kMT, kWaves, true>), grid, dim3(64 * kWaves), 0, stream, a);
+    hipLaunchKernelGGL((tree_kernel<kPool, kMode, kMT, kWaves, true>), grid, dim3(64 * kWaves), 0, stream, a);
     e = hipGetLastError();
     if (e == hipSuccess) {
       hipLaunchKernelGGL((tree_join_kernel<kMT>), dim3(a.hkv, (unsigned)a.batch, a.mblocks * kMT), dim3(256), 0, stream, a);
@@ -1297,9 +1453,9 @@ int check_shape(const char* who, int batch, int nodes, int hq, int hkv, int head
 bool misaligned(const void* p, int64_t a, int64_t b, int64_t c) { return ((uintptr_t)p & 15) != 0 || ((a | b | c) & 7) != 0; }
 
 // Fills what every form shares and launches; `mode` as the enum.
-int run(const char* who, TreeArgs a, int mode, bool fp8, int batch, int hq, size_t workspace_bytes, int64_t kv_page, int64_t kv_tok,
+int run(const char* who, TreeArgs a, int mode, int pool, int batch, int hq, size_t workspace_bytes, int64_t kv_page, int64_t kv_tok,
         int64_t kv_head, float softmax_scale, void* stream) {
-  const int elem = fp8 ? 1 : 2;
+  const int elem = pool == kBf16Pool ? 2 : 1;  // of the pool's strides
   // the stride of a dimension of one element may be anything
   if (batch == 1) a.q_sb = a.o_sb = a.kn_sb = a.vn_sb = 0;
   if (a.nodes == 1) a.q_sn = a.o_sn = a.kn_sn = a.vn_sn = 0;
@@ -1319,7 +1475,7 @@ int run(const char* who, TreeArgs a, int mode, bool fp8, int batch, int hq, size
   a.M = a.nodes * a.group;
   // (in floating point: the products of any strides)
   if (((double)a.num_pages * (double)kv_page + (double)a.page_size * (double)kv_tok) * elem >= 0x1p36 ||
-      (fp8 && (double)a.num_pages * (double)a.ss_p + a.page_size >= 0x1p32))
+      (pool != kBf16Pool && (double)a.num_pages * (double)a.ss_p + a.page_size >= 0x1p32))
     return fail(Q3A_EINVAL, "%s: a cache of 64 GiB or more, or scales of 4 GiB", who);
   const Plan p = plan_of(batch, a.nodes, hq, a.hkv, (int64_t)a.max_pages * a.page_size);
   if (p.bytes > 0 && (a.ws == nullptr || workspace_bytes < p.bytes || ((uintptr_t)a.ws & 15) != 0))
@@ -1347,11 +1503,11 @@ int run(const char* who, TreeArgs a, int mode, bool fp8, int batch, int hq, size
   a.scale_log2 = softmax_scale == 0.f ? FLT_MIN : fabsf(softmax_scale) * kLog2e;
   a.ahead = std::min(kAhead / a.scale_log2, 1e30f);
   const hipStream_t s = (hipStream_t)stream;
-  if (mode == kNoKeys) return launch<true, kNoKeys, 1>(a, who, s);
-  if (mode == kAppend) return launch<true, kAppend, 1>(a, who, s);
+  if (mode == kNoKeys) return pool == kFp4Pool ? launch<kFp4Pool, kNoKeys, 1>(a, who, s) : launch<kFp8Pool, kNoKeys, 1>(a, who, s);
+  if (mode == kAppend) return pool == kFp4Pool ? launch<kFp4Pool, kAppend, 1>(a, who, s) : launch<kFp8Pool, kAppend, 1>(a, who, s);
   switch (tiles_per_wave(a.M)) {
-    case 1: return fp8 ? launch<true, kTree, 1>(a, who, s) : launch<false, kTree, 1>(a, who, s);
-    default: return fp8 ? launch<true, kTree, 2>(a, who, s) : launch<false, kTree, 2>(a, who, s);
+    case 1: return pool == kFp8Pool ? launch<kFp8Pool, kTree, 1>(a, who, s) : launch<kBf16Pool, kTree, 1>(a, who, s);
+    default: return pool == kFp8Pool ? launch<kFp8Pool, kTree, 2>(a, who, s) : launch<kBf16Pool, kTree, 2>(a, who, s);
   }
 }
 
@@ -1403,7 +1559,7 @@ extern "C" int q3a_paged_decode_fp8(const void* q, int64_t q_stride_b, int64_t q
   a.ws = workspace;
   a.nodes = 1;
   a.hkv = num_kv_heads;
-  return run(who, a, kNoKeys, true, batch, num_q_heads, workspace_bytes, kv_stride_page, kv_stride_tok, kv_stride_head,
+  return run(who, a, kNoKeys, kFp8Pool, batch, num_q_heads, workspace_bytes, kv_stride_page, kv_stride_tok, kv_stride_head,
              softmax_scale, stream);
 }
 
@@ -1448,7 +1604,91 @@ extern "C" int q3a_paged_decode_fp8_append(
   a.ws = workspace;
   a.nodes = 1;
   a.hkv = num_kv_heads;
-  return run(who, a, kAppend, true, batch, num_q_heads, workspace_bytes, kv_stride_page, kv_stride_tok, kv_stride_head,
+  return run(who, a, kAppend, kFp8Pool, batch, num_q_heads, workspace_bytes, kv_stride_page, kv_stride_tok, kv_stride_head,
+             softmax_scale, stream);
+}
+
+extern "C" int q3a_paged_decode_fp4(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k_cache,
+                                    const void* v_cache, int64_t kv_stride_page, int64_t kv_stride_tok, int64_t kv_stride_head,
+                                    const void* k_scale, const void* v_scale, int64_t scale_stride_page,
+                                    int64_t scale_stride_head, int num_pages, int page_size, const int32_t* cache_seqlens,
+                                    const int32_t* block_table, int64_t bt_stride_b, int max_pages_per_seq, void* out,
+                                    int64_t o_stride_b, int64_t o_stride_h, void* workspace, size_t workspace_bytes, int batch,
+                                    int num_q_heads, int num_kv_heads, int head_dim, float softmax_scale, void* stream) {
+  const char* who = "q3a_paged_decode_fp4";
+  int rc = check_shape(who, batch, 1, num_q_heads, num_kv_heads, head_dim, max_pages_per_seq, page_size);
+  if (rc != Q3A_OK) return rc;
+  rc = check_fp4_pool(who, k_cache, v_cache, kv_stride_page, kv_stride_tok, kv_stride_head, k_scale, v_scale,
+                      scale_stride_page, scale_stride_head, num_pages, page_size, num_kv_heads);
+  if (rc != Q3A_OK || batch == 0) return rc;
+  TreeArgs a = {};
+  a.q = (const uint16_t*)q;
+  a.q_sb = q_stride_b;
+  a.q_sh = q_stride_h;
+  a.kc = (uint8_t*)const_cast<void*>(k_cache);
+  a.vc = (uint8_t*)const_cast<void*>(v_cache);
+  a.ks = (uint8_t*)const_cast<void*>(k_scale);
+  a.vs = (uint8_t*)const_cast<void*>(v_scale);
+  a.ss_p = scale_stride_page;
+  a.ss_h = scale_stride_head;
+  a.num_pages = num_pages;
+  a.page_size = page_size;
+  a.seqlens = cache_seqlens;
+  a.bt = block_table;
+  a.bt_sb = bt_stride_b;
+  a.max_pages = max_pages_per_seq;
+  a.out = (uint16_t*)out;
+  a.o_sb = o_stride_b;
+  a.o_sh = o_stride_h;
+  a.ws = workspace;
+  a.nodes = 1;
+  a.hkv = num_kv_heads;
+  return run(who, a, kNoKeys, kFp4Pool, batch, num_q_heads, workspace_bytes, kv_stride_page, kv_stride_tok, kv_stride_head,
+             softmax_scale, stream);
+}
+
+extern "C" int q3a_paged_decode_fp4_append(
+    const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k_new, int64_t kn_stride_b, int64_t kn_stride_h,
+    const void* v_new, int64_t vn_stride_b, int64_t vn_stride_h, void* k_cache, void* v_cache, int64_t kv_stride_page,
+    int64_t kv_stride_tok, int64_t kv_stride_head, void* k_scale, void* v_scale, int64_t scale_stride_page,
+    int64_t scale_stride_head, int num_pages, int page_size, const int32_t* cache_seqlens, const int32_t* block_table,
+    int64_t bt_stride_b, int max_pages_per_seq, void* out, int64_t o_stride_b, int64_t o_stride_h, void* workspace,
+    size_t workspace_bytes, int batch, int num_q_heads, int num_kv_heads, int head_dim, float softmax_scale, void* stream) {
+  const char* who = "q3a_paged_decode_fp4_append";
+  int rc = check_shape(who, batch, 1, num_q_heads, num_kv_heads, head_dim, max_pages_per_seq, page_size);
+  if (rc != Q3A_OK) return rc;
+  rc = check_fp4_pool(who, k_cache, v_cache, kv_stride_page, kv_stride_tok, kv_stride_head, k_scale, v_scale,
+                      scale_stride_page, scale_stride_head, num_pages, page_size, num_kv_heads);
+  if (rc != Q3A_OK || batch == 0) return rc;
+  TreeArgs a = {};
+  a.q = (const uint16_t*)q;
+  a.q_sb = q_stride_b;
+  a.q_sh = q_stride_h;
+  a.kn = (const uint16_t*)k_new;
+  a.kn_sb = kn_stride_b;
+  a.kn_sh = kn_stride_h;
+  a.vn = (const uint16_t*)v_new;
+  a.vn_sb = vn_stride_b;
+  a.vn_sh = vn_stride_h;
+  a.kc = (uint8_t*)k_cache;
+  a.vc = (uint8_t*)v_cache;
+  a.ks = (uint8_t*)k_scale;
+  a.vs = (uint8_t*)v_scale;
+  a.ss_p = scale_stride_page;
+  a.ss_h = scale_stride_head;
+  a.num_pages = num_pages;
+  a.page_size = page_size;
+  a.seqlens = cache_seqlens;
+  a.bt = block_table;
+  a.bt_sb = bt_stride_b;
+  a.max_pages = max_pages_per_seq;
+  a.out = (uint16_t*)out;
+  a.o_sb = o_stride_b;
+  a.o_sh = o_stride_h;
+  a.ws = workspace;
+  a.nodes = 1;
+  a.hkv = num_kv_heads;
+  return run(who, a, kAppend, kFp4Pool, batch, num_q_heads, workspace_bytes, kv_stride_page, kv_stride_tok, kv_stride_head,
              softmax_scale, stream);
 }
 
@@ -1512,6 +1752,6 @@ extern "C" int q3a_paged_decode_tree(
   a.ws = workspace;
   a.nodes = num_nodes;
   a.hkv = num_kv_heads;
-  return run(who, a, kTree, fp8, batch, num_q_heads, workspace_bytes, kv_stride_page, kv_stride_tok, kv_stride_head,
+  return run(who, a, kTree, fp8 ? kFp8Pool : kBf16Pool, batch, num_q_heads, workspace_bytes, kv_stride_page, kv_stride_tok, kv_stride_head,
              softmax_scale, stream);
 }

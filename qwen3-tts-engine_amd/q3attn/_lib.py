@@ -15,7 +15,7 @@ import torch  # noqa: F401  (must precede the library load, see above)
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libq3attn.so")
 # The torch ops that are registered from C++ (they link libq3attn.so).
 TORCH_LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libq3torch.so")
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 _c_i64 = ctypes.c_int64
 _c_int = ctypes.c_int
@@ -210,6 +210,27 @@ SIGNATURES = {
         _c_int, _c_int, _c_vp, _c_vp, _c_i64, _c_int,          # num_pages, page_size, seqlens, block_table, stride, max pages
         _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_size,         # out, strides (row, node, head), workspace, bytes
         _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_vp,  # batch, nodes, Hq, Hkv, D, softmax_scale, stream
+    ]),
+}
+
+# The 4-bit pool's calls are the 8-bit one's.
+SIGNATURES |= {name.replace("fp8", "fp4"): sig for name, sig in SIGNATURES.items() if "fp8" in name}
+
+
+class PageCache(ctypes.Structure):
+    """q3a_page_cache (include/q3attn.h)."""
+    _fields_ = [("base", _c_vp)] + [(n, _c_i64) for n in ("stride_page", "stride_1", "stride_0", "n_1", "n_0", "run_bytes")] + \
+        [("num_pages", _c_int)]
+
+
+SIGNATURES |= {
+    "q3a_paged_copy": (_c_int, [ctypes.POINTER(PageCache), _c_int, _c_vp, _c_vp, _c_i64, _c_vp]),  # caches, how many, src, dst, pairs, stream
+    "q3a_paged_compact": (_c_int, [
+        ctypes.POINTER(_c_vp), ctypes.POINTER(_c_vp), _c_int, _c_int, _c_int,  # caches, scales, how many, row bytes, scale blocks
+        _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,                # cache strides (page, tok, head), scale strides (page, head)
+        _c_int, _c_int, _c_vp, _c_i64, _c_int,                 # num_pages, page_size, keep, stride, width
+        _c_vp, _c_vp, _c_i64, _c_int, _c_vp,                   # seqlens, block_table, stride, max pages, new seqlens
+        _c_int, _c_int, _c_vp,                                 # batch, Hkv, stream
     ]),
 }
 
