@@ -11,7 +11,9 @@
 
 namespace q3a {
 
-enum { kNoKeys = 0, kTree = 1, kAppend = 2 };
+// Own keys of a row: none, the tree's nodes, the step's new row behind the cached ones, or that row as one of them (its place in the pool is
+// read, whatever it holds, and replaced in registers).
+enum { kNoKeys = 0, kTree = 1, kAppend = 2, kAppendKey = 3 };
 enum { kBf16Pool = 0, kFp8Pool = 1, kFp4Pool = 2 };
 
 
@@ -42,7 +44,8 @@ struct TreeArgs {
   uint16_t* out;
   int64_t o_sb, o_sn, o_sh;
   void* ws;
-  float* rec;  // in ws
+  float* rec;    // in ws
+  int rec_rows;  // query rows of a record, of one head
   int batch, nodes, group, hkv, M;
   Divisor per_hkv;
   uint32_t per_group;  // m / group = m * per_group >> 20 for m < 4096
@@ -125,6 +128,7 @@ __device__ __forceinline__ int row_tokens(int b, int mode) {
   const int n = a.seqlens[b];
   const int cap = a.max_pages * a.page_size;
   if (mode == kAppend) return n < cap ? n : -1;  // no room for the new row: skipped
+  if (mode == kAppendKey) return n >= 0 && n < cap ? n + 1 : -1;
   return min(n, cap);
 }
 
@@ -227,7 +231,7 @@ __device__ __forceinline__ Chunk chunk_at(const TreeArgs& a, uint32_t at, int mo
   const int lane = lane_now(), batch = a.batch, cap = a.max_pages * a.page_size;
   auto tokens = [&](int b) {  // row_tokens
     const int n = b < batch ? a.seqlens[b] : -1;
-    return mode == kAppend ? (n < cap ? n : -1) : min(n, cap);
+    return mode == kAppend ? (n < cap ? n : -1) : mode == kAppendKey ? (n >= 0 && n < cap ? n + 1 : -1) : min(n, cap);
   };
   uint32_t total = 0;  // below 2^32: 1024 rows of 2^21
   int L = -1;

@@ -35,42 +35,75 @@ typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ int key_of(int g, int i) { return 8 * (g >> 1) + 2 * i + (g & 1); }
 
+// Global loads of a scalar base and a lane's offset.  (The offset is made new for each: widened to 64 bits once, ahead of the loop, it would
+// take two registers and two additions a load.)
+typedef const __attribute__((address_space(1))) uint8_t* gptr;
+template <class T>
+__device__ __forceinline__ T load_at(gptr base, uint32_t off) {
+  asm volatile("" : "+v"(off));
+  return *(const __attribute__((address_space(1))) T*)(base + off);
+}
+// Codes.  kOnce: a head's tokens are neighbours in memory, so that a load takes whole lines which no other workgroup reads: non-temporal
+// (128 rows x 4000 tokens 86.5 us, 98.8 without).  Else two heads share a line, and one's load leaves it for the other's (125.2 us, 141.0
+// with).
+template <bool kOnce, class T>
+__device__ __forceinline__ T load_codes(gptr base, uint32_t off) {
+  asm volatile("" : "+v"(off));
+  const auto p = (const __attribute__((address_space(1))) T*)(base + off);
+  return kOnce ? __builtin_nontemporal_load(p) : *p;
+}
+
+// The pool at one KV head.
+struct Pool {
+  gptr kc, vc, ks, vs;
+  int st, page_size;
+};
+__device__ __forceinline__ Pool pool_of(const TreeArgs& a, int h) {
+  return {(gptr)a.kc + (int64_t)h * a.sh, (gptr)a.vc + (int64_t)h * a.sh, (gptr)a.ks + (int64_t)h * a.ss_h, (gptr)a.vs + (int64_t)h * a.ss_h,
+          a.st, a.page_size};
+}
+
+// Where a step lies, the same on every lane.
+struct Place {
+  int64_t at[kSub];      // byte offset of a subtile's first key,
+  uint32_t sat[kSub];    // and of its first exponent byte
+  int full;              // all keys are seen, else
+  int valid[kSub];       // so many of each subtile
+};
+
+// The lane's offsets in a subtile: of its key's block and of its four keys' dims, and of their exponent bytes.  All 16 keys of a subtile
+// are loaded whatever part of them is seen (a page is a multiple of 16), and the pool's first ones where the table has no page: any codes
+// are finite, and meet probabilities of 0.
+struct Offsets {
+  uint32_t k, ks, v[4], vs;
+};
+__device__ __forceinline__ Offsets offsets_of(const Pool& a, int lane) {
+  const int r = lane & 15, g = lane >> 4;
+  Offsets o;
+  o.k = (uint32_t)(r * a.st + 16 * g);
+  o.ks = (uint32_t)(g * a.page_size + (r & ~3));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o.v[i] = (uint32_t)(key_of(g, i) * a.st + 4 * r);
+  o.vs = (uint32_t)((r >> 2) * a.page_size + 8 * (g >> 1));
+  return o;
+}
+
 struct Tile {
   uint4 k[kSub];            // block g of key l % 16
-  uint32_t ks[kSub];        // its exponent byte
+  uint32_t ks[kSub];        // its exponent byte, with its neighbours' of the aligned four
   uint32_t v[kSub][4];      // dims 8 (l % 16) .. + 7 of keys key_of(g, 0 .. 3)
   uint2 vs[kSub];           // their block's exponent bytes of keys 8 (g / 2) .. + 7
-  int valid[kSub];          // keys that are seen
 
-  __device__ __forceinline__ static __amdgpu_buffer_rsrc_t codes(const TreeArgs& a, const uint8_t* base, int valid) {
-    // Descriptors end with the last seen key: what lies past it is not read and comes as zeros.
-    return make_rsrc(base, valid > 0 ? (uint32_t)(valid - 1) * (uint32_t)a.st + kFp4Row : 0u);
+  template <bool kOnce>
+  __device__ __forceinline__ void load_k(const Pool& a, const Place& p, int u, const Offsets& o) {
+    k[u] = __builtin_bit_cast(uint4, load_codes<kOnce, u32x4>(a.kc + p.at[u], o.k));
+    ks[u] = load_at<uint32_t>(a.ks + p.sat[u], o.ks);
   }
-  __device__ __forceinline__ static __amdgpu_buffer_rsrc_t exps(const TreeArgs& a, const uint8_t* base, int valid) {
-    return make_rsrc(base, valid > 0 ? (kFp4Blocks - 1) * a.page_size + 16 : 0);
-  }
-  __device__ __forceinline__ void load_k(const TreeArgs& a, const int64_t (&at)[kSub], const uint32_t (&sat)[kSub],
-                                         const int (&seen)[kSub], int lane) {
-    const int r = lane & 15, g = lane >> 4;
+  template <bool kOnce>
+  __device__ __forceinline__ void load_v(const Pool& a, const Place& p, int u, const Offsets& o) {
 #pragma unroll
-    for (int u = 0; u < kSub; ++u) {
-      k[u] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(codes(a, a.kc + at[u], seen[u]), r * a.st + 16 * g, 0, kNt));
-      ks[u] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(exps(a, a.ks + sat[u], seen[u]), g * a.page_size + r, 0, 0);
-    }
-  }
-  __device__ __forceinline__ void load_v(const TreeArgs& a, const int64_t (&at)[kSub], const uint32_t (&sat)[kSub],
-                                         const int (&seen)[kSub], int lane) {
-    const int r = lane & 15, g = lane >> 4;
-#pragma unroll
-    for (int u = 0; u < kSub; ++u) {
-      const auto rv = codes(a, a.vc + at[u], seen[u]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v[u][i] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rv, key_of(g, i) * a.st + 4 * r, 0, kNt);
-      vs[u] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(exps(a, a.vs + sat[u], seen[u]),
-                                                                             (r >> 2) * a.page_size + 8 * (g >> 1), 0, 0));
-      valid[u] = seen[u];
-    }
+    for (int i = 0; i < 4; ++i) v[u][i] = load_codes<kOnce, uint32_t>(a.vc + p.at[u], o.v[i]);
+    vs[u] = __builtin_bit_cast(uint2, load_at<u32x2>(a.vs + p.sat[u], o.vs));
   }
 };
 
@@ -90,18 +123,21 @@ struct Lds {
   uint8_t qs[16 * kT][4];
   alignas(16) uint8_t p[kW][2 * kRows][kPRow];
   float m[kW][kRows], l[kW][kRows];
+  alignas(16) uint8_t own[2][kFp4Row];                         // the append form's new row, of one wave: codes of K and V,
+  uint8_t own_s[2][kFp4Blocks];                                // and their exponent bytes
+  int plain;
 };
 
 // Splits Q.  A bf16 number has 8 significant bits, e4m3 4 of them between 2^-6 and 2^8 (and multiples of 2^-9 below).  In a block whose
 // largest element lies in [2^7, 2^8) after its scaling, elements of at least 2^-6 are the sum of their upper 4 bits (part 0) and the
 // lower 4, which times 2^4 are e4m3 numbers too (part 1); those 2^14 times smaller are in parts 2 and 3 likewise.  Elements that are
 // smaller still by 2^28 and more than the largest one have no part (`plain`: one in 10^8 of normal ones).  So the parts hold Q exactly.
-// Each of the workgroup's first four waves makes one part of all rows; every wave looks at all elements.
+// Each of the workgroup's first four waves makes one part of all rows.
 template <int kT, int kW>
-__device__ __forceinline__ void prepare_q(const Work& w, const uint4 (&x)[kT], int wave, Lds<kT, kW>& lds, Query<kT>& q) {
+__device__ __forceinline__ void prepare_q(uint32_t sign, const uint4 (&x)[kT], int wave, Lds<kT, kW>& lds, Query<kT>& q) {
   const int lane = lane_now(), part = wave & 3;
-  const uint32_t sign = args_again().q_sign;
   uint32_t bad = 0;
+  if (wave < 4) {
 #pragma unroll
   for (int t = 0; t < kT; ++t) {
     const uint32_t e[4] = {x[t].x ^ sign, x[t].y ^ sign, x[t].z ^ sign, x[t].w ^ sign};
@@ -126,14 +162,15 @@ __device__ __forceinline__ void prepare_q(const Work& w, const uint4 (&x)[kT], i
       if (i & 1) c[i >> 1] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c[i >> 1], f[0], f[1], scale, true);
       else c[i >> 1] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c[i >> 1], f[0], f[1], scale, false);
     }
-    if (wave < 4) {
-      const int row = 16 * t + 4 * (lane >> 4) + part, seg = lane & 15;
-      *reinterpret_cast<u32x2*>(&lds.q[row][8 * seg]) = u32x2{__builtin_bit_cast(uint32_t, c[0]), __builtin_bit_cast(uint32_t, c[1])};
-      if ((seg & 3) == 0) lds.qs[row][seg >> 2] = (uint8_t)field;
-    }
+    const int row = 16 * t + 4 * (lane >> 4) + part, seg = lane & 15;
+    *reinterpret_cast<u32x2*>(&lds.q[row][8 * seg]) = u32x2{__builtin_bit_cast(uint32_t, c[0]), __builtin_bit_cast(uint32_t, c[1])};
+    if ((seg & 3) == 0) lds.qs[row][seg >> 2] = (uint8_t)field;
   }
-  q.plain = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
+  const bool any = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
+  if (wave == 0 && lane == 0) lds.plain = any ? 1 : 0;
+  }
   __syncthreads();
+  q.plain = __builtin_amdgcn_readfirstlane(lds.plain) != 0;
   const int r = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int t = 0; t < kT; ++t) {
@@ -145,35 +182,35 @@ __device__ __forceinline__ void prepare_q(const Work& w, const uint4 (&x)[kT], i
 }
 
 // The row of Q that a lane's head is: the last one again past it.
-__device__ __forceinline__ const uint16_t* q_row(const Work& w, int head) {
-  const TreeArgs& a = args_again();
-  return a.q + (int64_t)w.b * a.q_sb + (int64_t)(w.h * a.group + min(head, a.group - 1)) * a.q_sh;
+__device__ __forceinline__ const uint16_t* q_row(const TreeArgs& a, int b, int h, int head) {
+  return a.q + (int64_t)b * a.q_sb + (int64_t)(h * a.group + min(head, a.group - 1)) * a.q_sh;
 }
 
+// The parts' sum.
 __device__ __forceinline__ float sum_parts(const f32x4_t d) { return (d[0] + d[1]) + (d[2] + d[3]); }
 
-// A subtile's scores where Q has no parts: codes converted to bf16, Q read again, in the rows of part 0.  (A loop, to be short.)
+// A subtile's scores where Q has no parts: codes converted to bf16, Q read again, in the rows of part 0.  (Piece by piece, to hold few
+// registers: what the loop has in flight stays in its own.)
 template <int kT>
-__device__ __forceinline__ void plain_scores(const Work& w, uint4 k, uint32_t ks, f32x4_t (&d)[kT]) {
-  const int lane = lane_now(), r = lane & 15, g = lane >> 4;
-  const uint32_t sign = args_again().q_sign;
+__device__ __forceinline__ void plain_scores(const Work& w, const uint4& k, uint32_t ks, f32x4_t (&d)[kT]) {
+  const uint32_t k4[4] = {k.x, k.y, k.z, k.w};
   const float f = fp8_scale(ks);
 #pragma unroll
-  for (int t = 0; t < kT; ++t) d[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-  for (int c = 0; c < 4; ++c) {
-    const bf16x8_t kf =
-        __builtin_bit_cast(bf16x8_t, make_uint4(fp4_pair<0>(k.x, f), fp4_pair<1>(k.x, f), fp4_pair<2>(k.x, f), fp4_pair<3>(k.x, f)));
-    k = make_uint4(k.y, k.z, k.w, 0u);
+  for (int c = 0; c < 4; ++c)
 #pragma unroll
     for (int t = 0; t < kT; ++t) {
-      uint4 x = ld16(q_row(w, 4 * t + (r >> 2)) + 32 * g + 8 * c);
+      const int lane = lane_now(), r = lane & 15, g = lane >> 4;
+      const uint32_t sign = args_again().q_sign;
+      uint4 x = ld16(q_row(args_again(), w.b, w.h, 4 * t + (r >> 2)) + 32 * g + 8 * c);
       x = make_uint4(nan_if_not_finite(x.x ^ sign), nan_if_not_finite(x.y ^ sign), nan_if_not_finite(x.z ^ sign),
                      nan_if_not_finite(x.w ^ sign));
       if ((r & 3) != 0) x = make_uint4(0u, 0u, 0u, 0u);
-      d[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x), kf, d[t], 0, 0, 0);
+      const bf16x8_t kf = __builtin_bit_cast(
+          bf16x8_t, make_uint4(fp4_pair<0>(k4[c], f), fp4_pair<1>(k4[c], f), fp4_pair<2>(k4[c], f), fp4_pair<3>(k4[c], f)));
+      const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+      d[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x), kf, c == 0 ? zero : d[t], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
     }
-  }
 }
 
 template <int kT>
@@ -182,26 +219,41 @@ struct State {
   float m[kT], l[kT];      // of head 4 t + g: the exponents' base, unscaled; sum, of this lane's keys until the merge
 };
 
-// A subtile's scores.
+// A step's scores.
 //
 // The compiler counts the passes of the scaled instruction as if both operands had 4 bits: 8 wait states ahead of the result's first use
 // instead of the 12 that an 8-bit operand takes, and the register that was read first then held something else.  So the wait is ours: 16
 // states behind the last product, ahead of any use.
 template <int kT>
-__device__ __forceinline__ void scores(const Work& w, const uint4& codes, uint32_t ks, const Query<kT>& q, float (&s)[kT]) {
-  f32x4_t d[kT];
-  if (q.plain) {
-    plain_scores<kT>(w, codes, ks, d);
-  } else {
-    const i32x8_t k = {(int)codes.x, (int)codes.y, (int)codes.z, (int)codes.w, 0, 0, 0, 0};
+__device__ __forceinline__ void scores(const Work& w, const uint4 (&codes)[kSub], const uint32_t (&four)[kSub], const Query<kT>& q, int lane,
+                                       float (&s)[kT][kSub]) {
+  uint32_t ks[kSub];  // the exponent byte lowest: only that counts
 #pragma unroll
-    for (int t = 0; t < kT; ++t)
-      d[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(q.v[t], k, f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 4, 0, (int)q.s[t], 0, (int)ks);
-    if constexpr (kT == 1) asm volatile("s_nop 15" : "+v"(d[0]));
-    else asm volatile("s_nop 15" : "+v"(d[0]), "+v"(d[1]));
+  for (int u = 0; u < kSub; ++u) ks[u] = four[u] >> (8 * (lane & 3));
+  if (__builtin_expect(q.plain, 0)) {
+#pragma unroll
+    for (int u = 0; u < kSub; ++u) {
+      f32x4_t d[kT];
+      plain_scores<kT>(w, codes[u], ks[u] & 0xffu, d);
+#pragma unroll
+      for (int t = 0; t < kT; ++t) s[t][u] = sum_parts(d[t]);
+    }
+    return;
   }
+  constexpr int kAtOnce = kT == 1 ? 2 : 1;  // (as registers allow)
 #pragma unroll
-  for (int t = 0; t < kT; ++t) s[t] = sum_parts(d[t]);
+  for (int u0 = 0; u0 < kSub; u0 += kAtOnce) {
+    f32x4_t d[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int u = kT == 1 ? u0 + e : u0, t = kT == 1 ? 0 : e;
+      const i32x8_t k = {(int)codes[u].x, (int)codes[u].y, (int)codes[u].z, (int)codes[u].w, 0, 0, 0, 0};
+      d[e] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(q.v[t], k, f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 4, 0, (int)q.s[t], 0, (int)ks[u]);
+    }
+    asm volatile("s_nop 15" : "+v"(d[0]), "+v"(d[1]));
+#pragma unroll
+    for (int e = 0; e < 2; ++e) s[kT == 1 ? 0 : e][kT == 1 ? u0 + e : u0] = sum_parts(d[e]);
+  }
 }
 
 template <int kCtrl>
@@ -209,13 +261,13 @@ __device__ __forceinline__ float dpp_max(float x) { return fmaxf(x, dpp_f32<kCtr
 
 // The scores to probabilities, in s; the base (as tree_decode.hip's softmax has it) and the sum are updated and O rescaled.
 template <int kT>
-__device__ __forceinline__ void softmax(const int (&valid)[kSub], float scale, float ahead, float (&s)[kT][kSub], State<kT>& st) {
-  if (((valid[0] & valid[1] & valid[2] & valid[3]) & 16) == 0) {
+__device__ __forceinline__ void softmax(const Place& at, float scale, float ahead, float (&s)[kT][kSub], State<kT>& st) {
+  if (__builtin_expect(at.full == 0, 0)) {
     const int r = lane_now() & 15;
 #pragma unroll
     for (int t = 0; t < kT; ++t)
 #pragma unroll
-      for (int u = 0; u < kSub; ++u) s[t][u] = r < valid[u] ? s[t][u] : -INFINITY;
+      for (int u = 0; u < kSub; ++u) s[t][u] = r < at.valid[u] ? s[t][u] : -INFINITY;
   }
   float top[kT];
   bool grown = false;
@@ -251,20 +303,26 @@ __device__ __forceinline__ uint32_t pair_at(uint32_t w, int byte, float f) {
   return byte == 0 ? fp4_pair<0>(w, f) : byte == 1 ? fp4_pair<1>(w, f) : byte == 2 ? fp4_pair<2>(w, f) : fp4_pair<3>(w, f);
 }
 
+// Between a wave's writes to its LDS and its reads of them by other lanes.  A wave's LDS operations run in order: only the compiler has to
+// keep them so.
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
 // The probabilities as two bf16 numbers into the wave's LDS, a row each.  A row has its 64 keys as the operands want them: of a quarter's
-// 16 keys (32 bytes) each i's four subtiles, so that a lane's four probabilities are neighbours.
+// 16 keys (32 bytes) each i's first two subtiles, then each i's other two.
 template <int kT>
 __device__ __forceinline__ void store_p(const float (&p)[kT][kSub], int lane, uint8_t (*lds)[kPRow]) {
   const int r = lane & 15, g = lane >> 4;
-  const int i = (r >> 1) & 3, quarter = 2 * (r >> 3) + (r & 1), pos = 32 * quarter + 8 * i;
+  const int i = (r >> 1) & 3, quarter = 2 * (r >> 3) + (r & 1), pos = 32 * quarter + 4 * i;
 #pragma unroll
   for (int t = 0; t < kT; ++t) {
-    const u32x2 hi = {pack_bf16x2(p[t][0], p[t][1]), pack_bf16x2(p[t][2], p[t][3])};
-    const u32x2 lo = {pack_bf16x2(p[t][0] - bf16_lo(hi.x), p[t][1] - bf16_hi(hi.x)),
-                      pack_bf16x2(p[t][2] - bf16_lo(hi.y), p[t][3] - bf16_hi(hi.y))};
-    *reinterpret_cast<u32x2*>(&lds[8 * t + 2 * g][pos]) = hi;
-    *reinterpret_cast<u32x2*>(&lds[8 * t + 2 * g + 1][pos]) = lo;
+#pragma unroll
+    for (int u = 0; u < kSub; u += 2) {
+      const uint32_t hi = pack_bf16x2(p[t][u], p[t][u + 1]);
+      *reinterpret_cast<uint32_t*>(&lds[8 * t + 2 * g][pos + 8 * u]) = hi;
+      *reinterpret_cast<uint32_t*>(&lds[8 * t + 2 * g + 1][pos + 8 * u]) = pack_bf16x2(p[t][u] - bf16_lo(hi), p[t][u + 1] - bf16_hi(hi));
+    }
   }
+  in_order();
 }
 
 // Operands of P: lane l has row l % 16 = 4 head + 2 number + dim, whose pairs are (p, 0) or (0, p).
@@ -275,44 +333,44 @@ __device__ __forceinline__ Pairs pairs_of(int lane) {
   return (lane & 1) != 0 ? Pairs{{0x01000c0cu, 0x03020c0cu}} : Pairs{{0x0c0c0100u, 0x0c0c0302u}};
 }
 
-// O += P V.
-template <int kT>
-__device__ __forceinline__ void values(const Tile& x, const float (&p)[kT][kSub], int lane, uint8_t (*lds)[kPRow], State<kT>& st) {
+// O += P V, `then` behind each subtile's.
+template <int kT, class Then>
+__device__ __forceinline__ void values(const Tile& x, const Place& at, const float (&p)[kT][kSub], int lane, uint8_t (*lds)[kPRow],
+                                       State<kT>& st, Then&& then) {
   const int r = lane & 15, g = lane >> 4;
   store_p<kT>(p, lane, lds);
   uint2 vs[kSub];
 #pragma unroll
   for (int u = 0; u < kSub; ++u) vs[u] = x.vs[u];
-  if (((x.valid[0] & x.valid[1] & x.valid[2] & x.valid[3]) & 16) == 0) {  // the exponent byte of a key that is not seen may be anything
+  if (__builtin_expect(at.full == 0, 0)) {  // the exponent byte of a key that is not seen may be anything
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
-      const int left = max(0, min(8, x.valid[u] - 8 * (g >> 1)));
-      vs[u].x &= (uint32_t)((1ull << (8 * min(left, 4))) - 1);
-      vs[u].y &= (uint32_t)((1ull << (8 * max(left - 4, 0))) - 1);
+      // (on the scalar unit, for the tokens 0 .. 7 and 8 .. 15)
+      const uint64_t lo = at.valid[u] >= 8 ? ~0ull : (1ull << (8 * at.valid[u])) - 1;
+      const uint64_t hi = at.valid[u] >= 16 ? ~0ull : (1ull << (8 * max(0, at.valid[u] - 8))) - 1;
+      vs[u].x &= (g & 2) != 0 ? (uint32_t)hi : (uint32_t)lo;
+      vs[u].y &= (g & 2) != 0 ? (uint32_t)(hi >> 32) : (uint32_t)(lo >> 32);
     }
   }
   // The lane's keys are every second one of 8: bytes 0 and 2, or 1 and 3, of both dwords.  Only the exponent's bits of a scale count (all
   // 256 of them were compared with other bits and signs around them), so a byte is brought there by one shift.
   const int left = (g & 1) != 0 ? 15 : 23, around = (g & 1) != 0 ? 1 : 25;
   const Pairs pairs = pairs_of(lane);
-  uint32_t w[kT][8];
-#pragma unroll
-  for (int t = 0; t < kT; ++t) {
-    const uint8_t* row = lds[8 * t + (r >> 1)] + 32 * g;
-    const uint4 a = ld16(row), b = ld16(row + 16);
-    w[t][0] = a.x, w[t][1] = a.y, w[t][2] = a.z, w[t][3] = a.w, w[t][4] = b.x, w[t][5] = b.y, w[t][6] = b.z, w[t][7] = b.w;
-  }
+  uint4 two[kT];  // P of two subtiles
 #pragma unroll
   for (int u = 0; u < kSub; ++u) {
+    if ((u & 1) == 0) {
+#pragma unroll
+      for (int t = 0; t < kT; ++t) two[t] = ld16(lds[8 * t + (r >> 1)] + 32 * g + 8 * u);
+    }
     const float f[4] = {__uint_as_float(vs[u].x << left), __uint_as_float(__builtin_amdgcn_alignbit(vs[u].x, vs[u].x, around)),
                         __uint_as_float(vs[u].y << left), __uint_as_float(__builtin_amdgcn_alignbit(vs[u].y, vs[u].y, around))};
     bf16x8_t a[kT];
 #pragma unroll
     for (int t = 0; t < kT; ++t) {
-      uint32_t e[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) e[i] = perm_b32(0u, w[t][2 * i + (u >> 1)], pairs.of[u & 1]);
-      a[t] = __builtin_bit_cast(bf16x8_t, make_uint4(e[0], e[1], e[2], e[3]));
+      const uint32_t by = pairs.of[u & 1];
+      a[t] = __builtin_bit_cast(bf16x8_t, make_uint4(perm_b32(0u, two[t].x, by), perm_b32(0u, two[t].y, by), perm_b32(0u, two[t].z, by),
+                                                     perm_b32(0u, two[t].w, by)));
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -321,70 +379,68 @@ __device__ __forceinline__ void values(const Tile& x, const float (&p)[kT][kSub]
 #pragma unroll
       for (int t = 0; t < kT; ++t) st.o[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[t], b, st.o[t][j], 0, 0, 0);
     }
+    then(u);
   }
 }
 
-// The append form's new row, quantised as the write kernel does and stored, and attended: key 0 of a step, whose other keys take no
-// registers.
-template <int kT>
-__device__ __forceinline__ void append_step(const TreeArgs& a, const Work& w, const Query<kT>& q, uint8_t (*lds)[kPRow], State<kT>& st) {
+// The append form's new row, quantised as the write kernel does, into LDS: lane l has 8 dims from 8 (l % 16) of K (l & 16: of V).
+template <int kT, int kW>
+__device__ __forceinline__ void quantise_own(const uint4& x, Lds<kT, kW>& lds) {
+  const int lane = lane_now() & 31, r = lane & 15;  // (lanes from 32 on write the same again)
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  const uint32_t s = fp4_scale_byte(dpp_max_u32<kDppXor2>(dpp_max_u32<kDppXor1>(halves_max(bf16_any_amax_pair(w)))));
+  *reinterpret_cast<uint32_t*>(&lds.own[lane >> 4][4 * r]) = fp4_codes8(w[0], w[1], w[2], w[3], s);
+  lds.own_s[lane >> 4][r >> 2] = (uint8_t)s;
+  in_order();
+}
+// And into the pool, if `page` is one of it.
+template <int kT, int kW>
+__device__ __forceinline__ void store_own(int h, int page, int off, const Lds<kT, kW>& lds) {
+  const TreeArgs& a = args_again();
+  const int lane = lane_now(), r = lane & 15, v = (lane >> 4) & 1;
+  if (lane < 32 && (unsigned)page < (unsigned)a.num_pages) {
+    const int64_t at = (int64_t)page * a.sp + (int64_t)h * a.sh + (int64_t)off * a.st + 4 * r;
+    const int64_t sat = (int64_t)page * a.ss_p + (int64_t)h * a.ss_h + off + (r >> 2) * a.page_size;
+    *reinterpret_cast<uint32_t*>((v ? a.vc : a.kc) + at) = *reinterpret_cast<const uint32_t*>(&lds.own[v][4 * r]);
+    if ((r & 3) == 0) (v ? a.vs : a.ks)[sat] = lds.own_s[v][r >> 2];
+  }
+}
+
+// The new row in a step's registers: key `at` of it, the same on every lane.  (The empty statements keep the branches on it apart: else they
+// become an index into registers.)
+template <int kT, int kW>
+__device__ __forceinline__ void own_key(Tile& x, int at, const Lds<kT, kW>& lds) {
   const int lane = lane_now(), r = lane & 15, g = lane >> 4;
-  const TreeArgs& more = args_again();
-  const uint16_t* kb = more.kn + (int64_t)w.b * more.kn_sb + (int64_t)w.h * more.kn_sh;
-  const uint16_t* vb = more.vn + (int64_t)w.b * more.vn_sb + (int64_t)w.h * more.vn_sh;
-  const int pi = (int)divide((uint32_t)w.L, more.per_page), off = w.L - pi * more.page_size;
-  const int page = more.bt[(int64_t)w.b * more.bt_sb + pi];
-  if ((unsigned)page >= (unsigned)a.num_pages) return;
-  uint32_t kw[16];
+  const uint4 c = ld16(&lds.own[0][16 * g]);
+  const uint32_t s = (uint32_t)lds.own_s[0][g] << (8 * (lane & 3));
+  const bool here = r == (at & 15);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint4 e = ld16(kb + 32 * g + 8 * i);
-    kw[4 * i] = e.x;
-    kw[4 * i + 1] = e.y;
-    kw[4 * i + 2] = e.z;
-    kw[4 * i + 3] = e.w;
-  }
-  const uint4 e = ld16(vb + 8 * r);
-  const uint32_t vw[4] = {e.x, e.y, e.z, e.w};
-  const uint32_t ks = fp4_scale_byte(halves_max(bf16_any_amax_pair(kw)));
-  const uint32_t vs = fp4_scale_byte(dpp_max_u32<kDppXor2>(dpp_max_u32<kDppXor1>(halves_max(bf16_any_amax_pair(vw)))));
-  uint32_t kc[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) kc[i] = fp4_codes8(kw[4 * i], kw[4 * i + 1], kw[4 * i + 2], kw[4 * i + 3], ks);
-  const uint32_t vc = fp4_codes8(vw[0], vw[1], vw[2], vw[3], vs);
-  const uint4 codes = make_uint4(kc[0], kc[1], kc[2], kc[3]);
-  {
-    const int64_t at = (int64_t)page * a.sp + (int64_t)off * a.st;
-    const int64_t sat = (int64_t)page * a.ss_p + off;
-    if (r == 0) {
-      st16(a.kc + at + 16 * g, codes);
-      a.ks[sat + g * a.page_size] = (uint8_t)ks;
+  for (int u = 0; u < kSub; ++u)
+    if (u == at >> 4) {
+      asm volatile("" : "+v"(x.ks[u]));
+      x.k[u] = make_uint4(here ? c.x : x.k[u].x, here ? c.y : x.k[u].y, here ? c.z : x.k[u].z, here ? c.w : x.k[u].w);
+      x.ks[u] = here ? s : x.ks[u];
     }
-    if (g == 0) {
-      *reinterpret_cast<uint32_t*>(a.vc + at + 4 * r) = vc;
-      if ((r & 3) == 0) a.vs[sat + (r >> 2) * a.page_size] = (uint8_t)vs;
+}
+template <int kT, int kW>
+__device__ __forceinline__ void own_value(Tile& x, int at, const Lds<kT, kW>& lds) {
+  const int lane = lane_now(), r = lane & 15, g = lane >> 4;
+  const uint32_t c = *reinterpret_cast<const uint32_t*>(&lds.own[1][4 * r]), shift = 8 * (at & 3);
+  const uint32_t s = (uint32_t)lds.own_s[1][r >> 2] << shift, others = ~(0xffu << shift);
+  const int key = at & 15;
+  const bool here = g == 2 * (key >> 3) + (key & 1), half = (g >> 1) == key >> 3;
+#pragma unroll
+  for (int u = 0; u < kSub; ++u)
+    if (u == at >> 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i == ((key >> 1) & 3)) {
+          asm volatile("" : "+v"(x.v[u][i]));
+          x.v[u][i] = here ? c : x.v[u][i];
+        }
+      if ((key & 4) == 0) x.vs[u].x = half ? (x.vs[u].x & others) | s : x.vs[u].x;
+      else x.vs[u].y = half ? (x.vs[u].y & others) | s : x.vs[u].y;
     }
-  }
-  float s[kT][kSub];
-  float same[kT];  // of every key alike
-  scores<kT>(w, codes, ks, q, same);
-#pragma unroll
-  for (int t = 0; t < kT; ++t) s[t][0] = same[t], s[t][1] = s[t][2] = s[t][3] = -INFINITY;
-  const int valid[kSub] = {1, 0, 0, 0};
-  softmax<kT>(valid, a.scale_log2, a.ahead, s, st);
-  store_p<kT>(s, lane, lds);
-  const Pairs pairs = pairs_of(lane);
-  const float f = fp8_scale(vs);
-#pragma unroll
-  for (int t = 0; t < kT; ++t) {
-    const uint32_t p = *reinterpret_cast<const uint32_t*>(lds[8 * t + (r >> 1)] + 32 * g);
-    const bf16x8_t pa = __builtin_bit_cast(bf16x8_t, make_uint4(perm_b32(0u, p, pairs.of[0]), 0u, 0u, 0u));
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bf16x8_t v = __builtin_bit_cast(bf16x8_t, make_uint4(g == 0 ? pair_at(vc, j, f) : 0u, 0u, 0u, 0u));
-      st.o[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa, v, st.o[t][j], 0, 0, 0);
-    }
-  }
 }
 
 // Merges the waves' states into the output (rec == nullptr) or a record of (o[128], m, l) floats a query head.
@@ -410,33 +466,45 @@ __device__ __forceinline__ void merge_waves(const Work& w, const State<kT>& st, 
                                                         st.o[t][j + 1][0] + st.o[t][j + 1][2], st.o[t][j + 1][1] + st.o[t][j + 1][3]};
   }
   __syncthreads();
-  const int row = thread >> 4, d0 = 8 * (thread & 15);
+  constexpr int kDims = kT == 2 && kW == 4 ? 4 : 2;  // a thread
+  const int row = thread / (kD / kDims), d0 = kDims * (thread % (kD / kDims));
   if (row >= args_again().M) return;  // at most 4 kT rows
   float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < kW; ++i) top = fmaxf(top, lds.m[i][row]);
   const float base = top == -INFINITY ? 0.f : top;
-  float acc[8] = {}, sum = 0.f;
+  float acc[kDims] = {}, sum = 0.f;
 #pragma unroll
   for (int i = 0; i < kW; ++i) {
     const float f = fast_exp2(lds.m[i][row] - base);
     sum += f * lds.l[i][row];
 #pragma unroll
-    for (int d = 0; d < 8; ++d) acc[d] += f * so[i][row][d0 + d];
+    for (int d = 0; d < kDims; ++d) acc[d] += f * so[i][row][d0 + d];
   }
   if (rec == nullptr) {
-    store_out(out_row(w.b, w.h, row) + d0, acc, sum);
+    uint16_t* op = out_row(w.b, w.h, row) + d0;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int d = 0; d < kDims; d += 2) *reinterpret_cast<uint32_t*>(op + d) = pack_bf16x2(acc[d] * inv, acc[d + 1] * inv);
   } else {
     float* o = rec + row * kRecord;
     if (d0 == 0) *reinterpret_cast<float2*>(o + kD) = make_float2(top, sum);
 #pragma unroll
-    for (int d = 0; d < 8; d += 2) *reinterpret_cast<float2*>(o + d0 + d) = make_float2(acc[d], acc[d + 1]);
+    for (int d = 0; d < kDims; d += 2) *reinterpret_cast<float2*>(o + d0 + d) = make_float2(acc[d], acc[d + 1]);
   }
 }
 
+// The pool places of a wave's next kWindow steps, one subtile a lane (4 slot + u), worked out by the lanes at once.
+struct Window4 {
+  uint32_t at, sat;   // offset of the first key in 16 bytes, and of its exponent byte
+  int tok, valid;     // its token; the keys that are seen
+  bool page;          // the table has a page for it
+  uint64_t whole;     // lanes with all 16 keys
+};
+
 // One workgroup a (row, KV head), its kW waves taking the row's steps in turn; or (kChunked) one of a chunk of a row's steps, which
 // leaves a record for the join unless it is the row's only one.
-template <int kMode, int kT, int kW, bool kChunked>
+template <int kMode, int kT, int kW, bool kChunked, bool kOnce>
 __global__ __launch_bounds__(64 * kW, kT == 1 ? 4 : 3) void fp4_decode_kernel(const TreeArgs args) {
   __shared__ Lds<kT, kW> lds;
   __shared__ __align__(16) float s_o[kW][4 * kT][kD + 4];
@@ -445,72 +513,115 @@ __global__ __launch_bounds__(64 * kW, kT == 1 ? 4 : 3) void fp4_decode_kernel(co
   int unit;
   unit_of(args, w.h, w.mb, unit);
   if (unit >= args.units) return;
-  Window win;
-  uint4 raw[kT];
+  uint4 raw[kT], own;
   auto load_q = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < kT; ++t) raw[t] = ld16(q_row(w, 4 * t + (lane >> 4)) + 8 * (lane & 15));
+    for (int t = 0; t < kT; ++t) raw[t] = ld16(q_row(args, w.b, w.h, 4 * t + (lane >> 4)) + 8 * (lane & 15));
   };
-  int s0 = 0, s1;  // the chunk's steps
+  Window4 win;
+  int id, off;   // on the way: the lane's table entry, and its token's place in the page
+  auto look_up = [&](const TreeArgs& a, int step) __attribute__((always_inline)) {
+    win.tok = kStep * step + 16 * (lane_now() & (kSub - 1));
+    const int pi = (int)divide((uint32_t)win.tok, a.per_page);
+    off = win.tok - pi * a.page_size;
+    id = -1;
+    if (pi < a.max_pages) id = a.bt[(int64_t)w.b * a.bt_sb + pi];
+  };
+  auto find = [&](const TreeArgs& a) __attribute__((always_inline)) {
+    win.page = (unsigned)id < (unsigned)a.num_pages;
+    const int page = win.page ? id : 0, in = win.page ? off : 0;
+    win.at = (uint32_t)(((int64_t)page * a.sp + (int64_t)in * a.st) >> 4);
+    win.sat = (uint32_t)(page * a.ss_p + in);
+  };
+  auto see = [&](int limit) __attribute__((always_inline)) {
+    win.valid = win.page ? max(0, min(16, limit - win.tok)) : 0;
+    win.whole = __builtin_amdgcn_ballot_w64(win.valid == 16);
+  };
+  int s0 = 0, s1;  // the chunk's steps: of whole rows all Tc
   float* rec = nullptr;
   if constexpr (kChunked) {
     const Chunk c = chunk_at<kStep * kW>(args, (uint32_t)unit, kMode);
     if (c.row < 0) return;
     w.b = c.row;
     w.L = c.L;
-    const int T = steps_of<kStep>(w.L, kMode);
     w.Tc = w.L > 0 ? (w.L + kStep - 1) / kStep : 0;
     const int steps = (int)((rounds_of<kStep * kW>(args, w.L, kMode) + c.count - 1) / c.count) * kW;
     s0 = min(w.Tc, c.index * steps);
-    s1 = c.index == c.count - 1 ? T : min(w.Tc, s0 + steps);  // the last one has the own step
-    if (c.count > 1) rec = args_again().rec + ((int64_t)unit * args_again().hkv + w.h) * (int64_t)(16 * kRecord);
-    if (c.index == 0 && w.h == 0 && threadIdx.x == 0) reinterpret_cast<Joined*>(args_again().ws)[w.b] = Joined{unit - c.index, c.count};
-    const int s = s0 + wave + kW * (lane >> 2);
-    const Entry e = entry_of<kSub>(w.b, s, lane);
+    s1 = min(w.Tc, s0 + steps);
+    look_up(args, s0 + wave + kW * (lane >> 2));
     load_q();
-    win = window_of<kFp4Pool>(e, w.L, s < min(s1, w.Tc));
+    if (c.count > 1) rec = args.rec + ((int64_t)unit * args.hkv + w.h) * (int64_t)(args.rec_rows * kRecord);
+    if (c.index == 0 && w.h == 0 && threadIdx.x == 0) reinterpret_cast<Joined*>(args.ws)[w.b] = Joined{unit - c.index, c.count};
+    find(args);
   } else {
     w.b = unit;
-    const int row0 = max(0, args.batch - 64 * kW);
-    if (args.order && unit >= row0) w.b = kth_longest<kW>(args, row0, unit - row0, wave);
+    if constexpr (kW == 4) {
+      const int row0 = max(0, args.batch - 64 * kW);
+      if (args.order && unit >= row0) w.b = kth_longest<kW>(args, row0, unit - row0, wave);
+    }
+    const int tokens = args.seqlens[w.b], cap = args.max_pages * args.page_size;
     // The first window's page ids do not wait for the row's length.
-    const Entry e = entry_of<kSub>(w.b, wave + kW * (lane >> 2), lane);
+    look_up(args, wave + kW * (lane >> 2));
     load_q();
-    win = window_of<kFp4Pool>(e, INT_MAX, true);
-    w.L = __builtin_amdgcn_readfirstlane(row_tokens(w.b, kMode));
+    find(args);
+    w.L = __builtin_amdgcn_readfirstlane(kMode == kAppendKey ? (tokens >= 0 && tokens < cap ? tokens + 1 : -1) : min(tokens, cap));
     w.Tc = w.L > 0 ? (w.L + kStep - 1) / kStep : 0;
-    s1 = steps_of<kStep>(w.L, kMode);
+    s1 = w.Tc;
   }
-  const TreeArgs a = at_head(args, w.h);
   if (s1 == 0 && rec == nullptr) {
     zero_rows(w.b, w.h, w.mb, 16);
     return;
   }
-  const int first = s0 + wave;
-  const int n = max(0, (min(s1, w.Tc) - first + kW - 1) / kW);  // this wave's cached steps: first, first + kW, ...
-  int64_t at[kSub];
-  uint32_t sat[kSub];
-  int seen[kSub];
+  const int first = s0 + wave, limit = min(w.L, kStep * s1);
+  const int n = max(0, (s1 - first + kW - 1) / kW);  // this wave's steps: first, first + kW, ...
+  see(limit);
+  // The append form's new row is key w.L - 1, in the last of all steps: the wave that has that one quantises it.
+  const bool has_own = kMode == kAppendKey && n > 0 && first + kW * (n - 1) == w.Tc - 1;
+  const int own_at = has_own ? w.L - 1 - kStep * (w.Tc - 1) : -1;
+  int own_page = -1, own_off = 0;
+  if (has_own) {
+    const int pi = (int)divide((uint32_t)(w.L - 1), args.per_page);
+    own_off = w.L - 1 - pi * args.page_size;
+    own = ld16((lane & 16) != 0 ? args.vn + (int64_t)w.b * args.vn_sb + (int64_t)w.h * args.vn_sh + 8 * (lane & 15)
+                                : args.kn + (int64_t)w.b * args.kn_sb + (int64_t)w.h * args.kn_sh + 8 * (lane & 15));
+    own_page = args.bt[(int64_t)w.b * args.bt_sb + pi];
+  }
   auto place = [&](int j) __attribute__((always_inline)) {
-    if ((j & (kWindow - 1)) == 0 && j > 0 && j < n) {
-      const int l = lane_now();
-      win = window_of<kFp4Pool>(entry_of<kSub>(w.b, first + kW * (j + (l >> 2)), l), w.L, j + (l >> 2) < n);
+    if ((j & (kWindow - 1)) == 0 && j > 0) {
+      const TreeArgs& a = args_again();
+      look_up(a, first + kW * (j + (lane_now() >> 2)));
+      find(a);
+      see(limit);
     }
-    const int slot = kSub * (j & (kWindow - 1)), tokens = w.L - kStep * (first + kW * j);
+    const int slot = kSub * (j & (kWindow - 1));
+    Place p;
+    p.full = ((win.whole >> slot) & 15) == 15 ? 1 : 0;
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
-      at[u] = (int64_t)(uint32_t)readlane((int)win.at, slot + u) << 4;
-      sat[u] = (uint32_t)readlane((int)win.sat, slot + u);
-      const int k = readlane(win.valid, slot + u), left = tokens - 16 * u;
-      seen[u] = j < n ? (k < left ? k : left < 0 ? 0 : left) : 0;  // (min as a chain of scalar selects)
+      p.at[u] = (int64_t)(uint32_t)readlane((int)win.at, slot + u) << 4;
+      p.sat[u] = (uint32_t)readlane((int)win.sat, slot + u);
+      p.valid[u] = 16;
     }
+    if (__builtin_expect(p.full == 0, 0)) {
+#pragma unroll
+      for (int u = 0; u < kSub; ++u) p.valid[u] = readlane(win.valid, slot + u);
+    }
+    return p;
   };
-  Tile x;
-  place(0);
-  x.load_k(a, at, sat, seen, lane);
-  x.load_v(a, at, sat, seen, lane);
+  const Pool pool = pool_of(args, w.h);
+  const Offsets offsets = offsets_of(pool, lane);
+  Tile x;  // (loaded without a branch, also by a wave without steps: only so can what was asked for before be waited for alone)
+  Place at = place(0);
+#pragma unroll
+  for (int u = 0; u < kSub; ++u) x.load_k<kOnce>(pool, at, u, offsets);
+#pragma unroll
+  for (int u = 0; u < kSub; ++u) x.load_v<kOnce>(pool, at, u, offsets);
   Query<kT> q;
-  prepare_q<kT, kW>(w, raw, wave, lds, q);
+  prepare_q<kT, kW>(args.q_sign, raw, wave, lds, q);
+  if (has_own) {
+    quantise_own<kT, kW>(own, lds);
+    store_own<kT, kW>(w.h, own_page, own_off, lds);  // (early: a workgroup lasts until its stores are done)
+  }
   State<kT> st;
 #pragma unroll
   for (int t = 0; t < kT; ++t) {
@@ -521,46 +632,61 @@ __global__ __launch_bounds__(64 * kW, kT == 1 ? 4 : 3) void fp4_decode_kernel(co
   for (int t = 0; t < kT; ++t)
 #pragma unroll
     for (int j = 0; j < 4; ++j) st.o[t][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  if constexpr (kMode == kAppend) {
-    if (first + n * kW == s1 - 1) append_step<kT>(a, w, q, lds.p[wave], st);  // the row's own step is this wave's
-  }
-  const TreeArgs again = at_head(args_again(), w.h);  // (not held in registers, and spilled, since the kernel's start)
-  for (int i = 0; i < n; ++i) {
+  const float scale = args.scale_log2, ahead = args.ahead;
+  auto step = [&](int i, auto more) __attribute__((always_inline)) {
+    Place next = at;
+    if constexpr (decltype(more)::value) next = place(i + 1);
     float s[kT][kSub];
-    place(i + 1);
+    if (kMode == kAppendKey && !decltype(more)::value && has_own) own_key<kT, kW>(x, own_at, lds);
+    scores<kT>(w, x.k, x.ks, q, lane, s);
+    if constexpr (decltype(more)::value) {
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int u = 0; u < kSub; ++u) {
-      float one[kT];
-      scores<kT>(w, x.k[u], x.ks[u], q, one);
-#pragma unroll
-      for (int t = 0; t < kT; ++t) s[t][u] = one[t];
+      for (int u = 0; u < kSub; ++u) x.load_k<kOnce>(pool, next, u, offsets);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_sched_barrier(0);
-    x.load_k(again, at, sat, seen, lane);
-    __builtin_amdgcn_sched_barrier(0);
-    softmax<kT>(x.valid, again.scale_log2, again.ahead, s, st);
-    values<kT>(x, s, lane, lds.p[wave], st);
-    __builtin_amdgcn_sched_barrier(0);
-    x.load_v(again, at, sat, seen, lane);
-    __builtin_amdgcn_sched_barrier(0);
-  }
+    softmax<kT>(at, scale, ahead, s, st);
+    if (kMode == kAppendKey && !decltype(more)::value && has_own) own_value<kT, kW>(x, own_at, lds);
+    values<kT>(x, at, s, lane, lds.p[wave], st, [&](int u) __attribute__((always_inline)) {
+      if constexpr (decltype(more)::value) {
+        __builtin_amdgcn_sched_barrier(0);
+        x.load_v<kOnce>(pool, next, u, offsets);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    });
+    at = next;
+  };
+  // The last step by itself: with branches around the loads the compiler would not know how many of them are newer than those that it
+  // waits for, and wait for all.
+  for (int i = 0; i < n - 1; ++i) step(i, std::true_type{});
+  if (n > 0) step(n - 1, std::false_type{});
   merge_waves<kT, kW>(w, st, rec, wave, s_o, lds);
 }
 
+template <int kMode, int kT, int kW, bool kChunked>
+void launch(const TreeArgs& a, dim3 grid, hipStream_t stream) {
+  if (a.st == kFp4Row) hipLaunchKernelGGL((fp4_decode_kernel<kMode, kT, kW, kChunked, true>), grid, dim3(64 * kW), 0, stream, a);
+  else hipLaunchKernelGGL((fp4_decode_kernel<kMode, kT, kW, kChunked, false>), grid, dim3(64 * kW), 0, stream, a);
+}
+// Four waves a workgroup; eight for chunks of 5 to 8 query heads, whose registers leave room for 12 waves on a compute unit: one workgroup
+// of eight does as much as three of four with a third of the records (5 rows of 20000 to 65000 tokens 23.0 us; two of four 26.4, three 24.0).
+// Whole rows lose by more: what a wave does once for its row is as long as two steps (576 rows 52 us with four, 61 with eight).
 template <int kMode, int kT>
 void launch(const TreeArgs& a, dim3 grid, hipStream_t stream) {
-  if (a.target == 0) hipLaunchKernelGGL((fp4_decode_kernel<kMode, kT, 4, false>), grid, dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL((fp4_decode_kernel<kMode, kT, 4, true>), grid, dim3(256), 0, stream, a);
+  if (a.target == 0) launch<kMode, kT, 4, false>(a, grid, stream);
+  else launch<kMode, kT, kT == 1 ? 4 : 8, true>(a, grid, stream);
 }
 
 }  // namespace
 
-hipError_t launch_fp4_decode(const TreeArgs& a, int mode, dim3 grid, hipStream_t stream) {
+hipError_t launch_fp4_decode(const TreeArgs& args, int mode, dim3 grid, hipStream_t stream) {
+  TreeArgs a = args;
+  if (a.num_pages == 0) a.max_pages = 0;  // no row has a token: the kernel loads some page's codes for every step
   if (a.group <= 4) {
-    if (mode == kAppend) launch<kAppend, 1>(a, grid, stream);
+    if (mode == kAppend) launch<kAppendKey, 1>(a, grid, stream);
     else launch<kNoKeys, 1>(a, grid, stream);
   } else {
-    if (mode == kAppend) launch<kAppend, 2>(a, grid, stream);
+    if (mode == kAppend) launch<kAppendKey, 2>(a, grid, stream);
     else launch<kNoKeys, 2>(a, grid, stream);
   }
   return hipGetLastError();

@@ -965,7 +965,7 @@ __global__ __launch_bounds__(64 * kW, kMT == 2 || (kMode == kTree && kChunked) ?
     s0 = min(w.Tc, c.index * steps);
     s1 = c.index == c.count - 1 ? T : min(w.Tc, s0 + steps);  // the last one has the own steps
     if (c.count > 1)
-      rec = args_again().rec + (((int64_t)unit * args_again().mblocks + w.mb) * args_again().hkv + w.h) * (int64_t)(16 * kMT * kRecord);
+      rec = args_again().rec + (((int64_t)unit * args_again().mblocks + w.mb) * args_again().hkv + w.h) * (int64_t)(args_again().rec_rows * kRecord);
     if (c.index == 0 && w.h == 0 && w.mb == 0 && threadIdx.x == 0)
       reinterpret_cast<Joined*>(args_again().ws)[w.b] = Joined{unit - c.index, c.count};
     const int s = s0 + wave + kW * (lane >> 1);
@@ -1053,8 +1053,8 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const TreeArgs a) {
   const int group = threadIdx.x >> 4, d0 = 8 * (threadIdx.x & 15);
   const int bits = rows > 8 ? 4 : rows > 4 ? 3 : rows > 2 ? 2 : rows - 1;  // 2^bits query rows at once
   const int share = 16 >> bits, mine = group >> bits, i = group & ((1 << bits) - 1);
-  const int64_t step = (int64_t)a.mblocks * a.hkv * (16 * kMT * kRecord);  // from a chunk's records to the next one's
-  const float* rec = a.rec + d.first * step + ((int64_t)mb * a.hkv + h) * (16 * kMT * kRecord) + (tile + i) * kRecord;
+  const int64_t step = (int64_t)a.mblocks * a.hkv * (a.rec_rows * kRecord);  // from a chunk's records to the next one's
+  const float* rec = a.rec + d.first * step + ((int64_t)mb * a.hkv + h) * (a.rec_rows * kRecord) + (tile + i) * kRecord;
   const int m = mb * 16 * kMT + tile + i, node = node_of(a, m);
   uint16_t* out = a.out + b * a.o_sb + node * a.o_sn + (int64_t)(h * a.group + m - node * a.group) * a.o_sh + d0;
   float acc[8] = {}, sum = 0.f, top = -INFINITY;
@@ -1113,11 +1113,12 @@ int tiles_per_wave(int M) { return M <= 16 ? 1 : 2; }
 
 struct Plan {
   int mblocks, units, target, target_one;  // target == 0: whole rows
+  int rec_rows;
   size_t rows, bytes;
 };
 
-// From the shape alone: the lengths are on the device.
-Plan plan_of(int batch, int nodes, int hq, int hkv, int64_t capacity) {
+// From the shape alone: the lengths are on the device.  fp4: the 4-bit pool's own kernels (fp4_decode.hip).
+Plan plan_of(int batch, int nodes, int hq, int hkv, int64_t capacity, bool fp4 = false) {
   Plan p = {};
   const int M = nodes * (hq / hkv), tiles = tiles_per_wave(M);
   p.mblocks = (M + 16 * tiles - 1) / (16 * tiles);
@@ -1135,11 +1136,15 @@ Plan plan_of(int batch, int nodes, int hq, int hkv, int64_t capacity) {
     return std::max({1, slots - batch / 2, slots / 2});
   };
   if (target(2) < 2) return p;  // a single row's heads and nodes fill the chip, or nearly
-  p.target = target(2);
-  p.target_one = target(1);
+  // (Over 4 bits with up to 4 query heads to a KV head, whose workgroups are shorter, twice as many: 24 rows of 100 to 1500 tokens 8.4
+  // and 9.5 us, one row and long ones alike.  Their records are half as large, so that the workspace asked for is enough.)
+  const int each = fp4 && hq / hkv <= 4 ? 4 : 2;
+  p.target = target(each);
+  p.target_one = target(each / 2);
   p.units = p.target + batch;
+  p.rec_rows = fp4 ? 8 : 16 * tiles;
   p.rows = ((size_t)batch * sizeof(Joined) + 15) & ~(size_t)15;
-  p.bytes = p.rows + (size_t)p.units * p.mblocks * hkv * 16 * tiles * kRecord * sizeof(float);
+  p.bytes = p.rows + (size_t)p.units * p.mblocks * hkv * p.rec_rows * kRecord * sizeof(float);
   return p;
 }
 
@@ -1204,7 +1209,7 @@ int run(const char* who, TreeArgs a, int mode, int pool, int batch, int hq, size
   if (((double)a.num_pages * (double)kv_page + (double)a.page_size * (double)kv_tok) * elem >= 0x1p36 ||
       (pool != kBf16Pool && (double)a.num_pages * (double)a.ss_p + a.page_size >= 0x1p32))
     return fail(Q3A_EINVAL, "%s: a cache of 64 GiB or more, or scales of 4 GiB", who);
-  const Plan p = plan_of(batch, a.nodes, hq, a.hkv, (int64_t)a.max_pages * a.page_size);
+  const Plan p = plan_of(batch, a.nodes, hq, a.hkv, (int64_t)a.max_pages * a.page_size, pool == kFp4Pool && a.group <= 8);
   if (p.bytes > 0 && (a.ws == nullptr || workspace_bytes < p.bytes || ((uintptr_t)a.ws & 15) != 0))
     return fail(Q3A_ESPACE, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", who, workspace_bytes, p.bytes);
   a.batch = batch;
@@ -1220,6 +1225,7 @@ int run(const char* who, TreeArgs a, int mode, int pool, int batch, int hq, size
   }
   a.xcd_units = p.units >= 32;
   a.order = p.target == 0 && batch > 1 && (int64_t)batch * a.hkv * p.mblocks > num_cus();
+  a.rec_rows = p.rec_rows;
   a.rec = p.target > 0 ? reinterpret_cast<float*>(static_cast<char*>(a.ws) + p.rows) : nullptr;
   a.sp = kv_page * elem;
   a.st = (int)(kv_tok * elem);
