@@ -114,3 +114,26 @@ def test_pool_without_pages(cuda_device):
     lens, table = torch.tensor([5, 0, 70], dtype=torch.int32, device=dev), torch.full((3, 6), 2, dtype=torch.int32, device=dev)
     with pytest.raises(RuntimeError, match="null pool"):
         q3attn.paged_decode_fp4(q, *pool, lens, table, 0.1)
+
+
+@pytest.mark.parametrize("group", [2, 7])
+def test_chunks_captured_on_two_streams(cuda_device, group):
+    """Chunks and their join in two graphs that share their memory, replayed in turn and with eager calls on another stream between."""
+    cases = [_case(cuda_device, lens, 16, 8, group, True, 31 + group) for lens in ([2600], [40, 3100, 7])]
+    calls = [(q.to(cuda_device), *pool, lens.to(cuda_device), table.to(cuda_device), 0.1) for pool, table, lens, q in cases]
+    eager = [q3attn.paged_decode_fp4(*c).clone() for c in calls]
+    graphs, outs, pool = [], [], None
+    for c in calls:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            outs.append(q3attn.paged_decode_fp4(*c))
+        pool = graph.pool()
+        graphs.append(graph)
+    side = torch.cuda.Stream()
+    for _ in range(4):
+        for graph, out, want, call in zip(graphs, outs, eager, calls):
+            graph.replay()
+            with torch.cuda.stream(side):
+                beside = q3attn.paged_decode_fp4(*call)
+            torch.cuda.synchronize()
+            assert torch.equal(out, want) and torch.equal(beside, want)
