@@ -1213,9 +1213,13 @@ int run(const char* who, TreeArgs a, int mode, int pool, int batch, int hq, size
   if (((double)a.num_pages * (double)kv_page + (double)a.page_size * (double)kv_tok) * elem >= 0x1p36 ||
       (pool != kBf16Pool && (double)a.num_pages * (double)a.ss_p + a.page_size >= 0x1p32))
     return fail(Q3A_EINVAL, "%s: a cache of 64 GiB or more, or scales of 4 GiB", who);
-  const Plan p = plan_of(batch, a.nodes, hq, a.hkv, (int64_t)a.max_pages * a.page_size, pool == kFp4Pool && a.group <= 8);
-  if (p.bytes > 0 && (a.ws == nullptr || workspace_bytes < p.bytes || ((uintptr_t)a.ws & 15) != 0))
-    return fail(Q3A_ESPACE, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", who, workspace_bytes, p.bytes);
+  const int64_t capacity = (int64_t)a.max_pages * a.page_size;
+  const bool fp4 = pool == kFp4Pool && a.group <= 8;
+  const Plan p = plan_of(batch, a.nodes, hq, a.hkv, capacity, fp4);
+  // (What is asked for is what the workspace query says, which knows no pool.)
+  const size_t need = p.bytes == 0 ? 0 : std::max(p.bytes, plan_of(batch, a.nodes, hq, a.hkv, capacity).bytes);
+  if (need > 0 && (a.ws == nullptr || workspace_bytes < need || ((uintptr_t)a.ws & 15) != 0))
+    return fail(Q3A_ESPACE, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", who, workspace_bytes, need);
   a.batch = batch;
   a.per_group = ((1u << 20) + a.group - 1) / a.group;
   a.per_page = divisor((uint32_t)a.page_size);
