@@ -3,7 +3,9 @@
 //
 // At 136 bytes a token and KV head the pool's keys pass at four times the rate of bf16 ones, and what bounds the general kernel over
 // them is vector instructions: 16 query rows' worth of softmax for 2, and a conversion for every pair of codes.  Here a wave's step is
-// 64 keys (four 16-token subtiles u, each inside one page), and:
+// 64 keys (four 16-token subtiles u, each inside one page), 160 vector instructions for up to 4 heads.  HBM bounds long rows (128 x 4000
+// tokens 6.4 TB/s, 576 of 64 to 1800 5.6), few rows the chain of a row's start, its longest wave's steps (0.7 us each) and the merge: 5.6 us
+// for one of 64 tokens, 7.2 for one of 900.  With:
 //   S = Q K^T     the scaled matrix instruction takes K's codes and exponent bytes as they are stored: v_mfma_scale_f32_16x16x128,
 //                 B = 16 keys: lane l holds block g = l / 16 (32 dims) of key l % 16.  It wants 8 bits or fewer of Q too, so Q is
 //                 split, exactly, into four e4m3 parts with exponents of their own for each block (prepare_q), and the 16 rows of A
@@ -139,35 +141,35 @@ __device__ __forceinline__ void prepare_q(uint32_t sign, const uint4 (&x)[kT], i
   uint32_t bad = 0;
   if (wave < 4) {
 #pragma unroll
-  for (int t = 0; t < kT; ++t) {
-    const uint32_t e[4] = {x[t].x ^ sign, x[t].y ^ sign, x[t].z ^ sign, x[t].w ^ sign};
-    uint32_t top = dpp_max_u32<kDppXor2>(dpp_max_u32<kDppXor1>(halves_max(bf16_any_amax_pair(e))));  // of the block's four lanes
-    const int x7 = (int)(top >> 7);
-    const uint32_t least = (uint32_t)max(0, x7 - 27) << 7, large = (uint32_t)max(0, x7 - 13) << 7;
-    bad |= (top >= 0x7f80u || (top != 0 && x7 < 28)) ? 1u : 0u;
-    const uint32_t field = top == 0 ? 127u : (uint32_t)(x7 - 7 - (part == 0 ? 0 : part == 1 ? 4 : part == 2 ? 14 : 18));
-    const float scale = __uint_as_float((field & 0xffu) << 23);
-    s16x2 c[2] = {{0, 0}, {0, 0}};
+    for (int t = 0; t < kT; ++t) {
+      const uint32_t e[4] = {x[t].x ^ sign, x[t].y ^ sign, x[t].z ^ sign, x[t].w ^ sign};
+      uint32_t top = dpp_max_u32<kDppXor2>(dpp_max_u32<kDppXor1>(halves_max(bf16_any_amax_pair(e))));  // of the block's four lanes
+      const int x7 = (int)(top >> 7);
+      const uint32_t least = (uint32_t)max(0, x7 - 27) << 7, large = (uint32_t)max(0, x7 - 13) << 7;
+      bad |= (top >= 0x7f80u || (top != 0 && x7 < 28)) ? 1u : 0u;
+      const uint32_t field = top == 0 ? 127u : (uint32_t)(x7 - 7 - (part == 0 ? 0 : part == 1 ? 4 : part == 2 ? 14 : 18));
+      const float scale = __uint_as_float((field & 0xffu) << 23);
+      s16x2 c[2] = {{0, 0}, {0, 0}};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float f[2];
+      for (int i = 0; i < 4; ++i) {
+        float f[2];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const uint32_t b = k == 0 ? e[i] & 0xffffu : e[i] >> 16, mag = b & 0x7fffu;
-        bad |= (mag != 0 && mag < least) ? 1u : 0u;
-        const bool here = (mag >= large) == (part < 2);
-        const float whole = __uint_as_float(b << 16), upper = __uint_as_float((b & 0xfff0u) << 16);
-        f[k] = here ? ((part & 1) != 0 ? whole - upper : upper) : 0.f;
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t b = k == 0 ? e[i] & 0xffffu : e[i] >> 16, mag = b & 0x7fffu;
+          bad |= (mag != 0 && mag < least) ? 1u : 0u;
+          const bool here = (mag >= large) == (part < 2);
+          const float whole = __uint_as_float(b << 16), upper = __uint_as_float((b & 0xfff0u) << 16);
+          f[k] = here ? ((part & 1) != 0 ? whole - upper : upper) : 0.f;
+        }
+        if (i & 1) c[i >> 1] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c[i >> 1], f[0], f[1], scale, true);
+        else c[i >> 1] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c[i >> 1], f[0], f[1], scale, false);
       }
-      if (i & 1) c[i >> 1] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c[i >> 1], f[0], f[1], scale, true);
-      else c[i >> 1] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c[i >> 1], f[0], f[1], scale, false);
+      const int row = 16 * t + 4 * (lane >> 4) + part, seg = lane & 15;
+      *reinterpret_cast<u32x2*>(&lds.q[row][8 * seg]) = u32x2{__builtin_bit_cast(uint32_t, c[0]), __builtin_bit_cast(uint32_t, c[1])};
+      if ((seg & 3) == 0) lds.qs[row][seg >> 2] = (uint8_t)field;
     }
-    const int row = 16 * t + 4 * (lane >> 4) + part, seg = lane & 15;
-    *reinterpret_cast<u32x2*>(&lds.q[row][8 * seg]) = u32x2{__builtin_bit_cast(uint32_t, c[0]), __builtin_bit_cast(uint32_t, c[1])};
-    if ((seg & 3) == 0) lds.qs[row][seg >> 2] = (uint8_t)field;
-  }
-  const bool any = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
-  if (wave == 0 && lane == 0) lds.plain = any ? 1 : 0;
+    const bool any = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
+    if (wave == 0 && lane == 0) lds.plain = any ? 1 : 0;
   }
   __syncthreads();
   q.plain = __builtin_amdgcn_readfirstlane(lds.plain) != 0;
