@@ -672,14 +672,14 @@ void launch(const TreeArgs& a, dim3 grid, hipStream_t stream) {
 }
 // Four waves a workgroup.  Eight for chunks of 5 to 8 query heads, whose registers leave room for 12 waves on a compute unit: one workgroup
 // of eight does as much as three of four with a third of the records (5 rows of 20000 to 65000 tokens 23.0 us; two of four 26.4, three 24.0).
-// Eight also for whole rows that leave half of the compute units idle, or that leave none a second workgroup where that many would not
-// fit (1 row x 1500 tokens 9.9 us, with four 11.0; of 8 heads 11.9 and 13.6, 32 rows x 2000 of 8 heads 16.6 and 17.9).  More rows lose by
-// it, for what a wave does once for its row is as long as two steps: 576 rows 52 us with four, 61 with eight.
+// Eight also for whole rows that leave each compute unit one workgroup at most (1 row x 1500 tokens 9.9 us, with four 11.0; 24 rows x 1500
+// 11.5 and 12.6, of 188 to 1500 10.4 and 12.0; 32 x 2000 15.2 and 15.1; of 8 query heads a KV head 1 x 1500 11.9 and 13.6, 32 x 2000 16.6
+// and 17.9).  More rows lose by it, for what a wave does once for its row is as long as two steps: 576 rows 52 us with four, 61 with eight.
 template <int kMode, int kT>
 void launch(const TreeArgs& a, dim3 grid, hipStream_t stream) {
   const int groups = a.batch * a.hkv;
   if (a.target > 0) launch<kMode, kT, kT == 1 ? 4 : 8, true>(a, grid, stream);
-  else if (groups <= (kT == 1 ? num_cus() / 2 : num_cus())) launch<kMode, kT, 8, false>(a, grid, stream);
+  else if (groups <= num_cus()) launch<kMode, kT, 8, false>(a, grid, stream);
   else launch<kMode, kT, 4, false>(a, grid, stream);
 }
 
