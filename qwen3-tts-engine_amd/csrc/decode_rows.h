@@ -16,7 +16,6 @@ namespace q3a {
 enum { kNoKeys = 0, kTree = 1, kAppend = 2, kAppendKey = 3 };
 enum { kBf16Pool = 0, kFp8Pool = 1, kFp4Pool = 2 };
 
-
 constexpr int kD = kRowDims;
 constexpr int kRecord = kD + 2;    // floats per query row of a record: o[128], m, l
 
@@ -128,7 +127,6 @@ __device__ __forceinline__ int row_tokens(int b, int mode) {
   const int n = a.seqlens[b];
   const int cap = a.max_pages * a.page_size;
   if (mode == kAppend) return n < cap ? n : -1;  // no room for the new row: skipped
-  if (mode == kAppendKey) return n >= 0 && n < cap ? n + 1 : -1;
   return min(n, cap);
 }
 

@@ -1110,7 +1110,6 @@ constexpr int kWaves = 4;
 
 int tiles_per_wave(int M) { return M <= 16 ? 1 : 2; }
 
-
 struct Plan {
   int mblocks, units, target, target_one;  // target == 0: whole rows
   int rec_rows;
