@@ -302,8 +302,15 @@ void paged_copy(at::TensorList caches, const Tensor& src, const Tensor& dst) {
   check_pages(who, "dst", d, dst);
   TORCH_CHECK(src.size(0) == dst.size(0), who, ": ", src.size(0), " source pages for ", dst.size(0));
   c10::SmallVector<q3a_page_cache, 64> list;
+  const Tensor* last = nullptr;  // (layers are alike: their shape is worked out once)
+  q3a_page_cache c = {};
   for (const Tensor& t : caches) {
-    const q3a_page_cache c = page_cache(who, d, t);
+    if (last != nullptr && t.device() == d && t.element_size() == last->element_size() && t.sizes() == last->sizes() &&
+        t.strides() == last->strides())
+      c.base = t.data_ptr();
+    else
+      c = page_cache(who, d, t);
+    last = &t;
     if (t.numel() > 0) list.push_back(c);
   }
   if (list.empty()) return;
@@ -440,8 +447,8 @@ Tensor tree_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const op
 
 template <class... T>
 void written(const T&... caches) {
-  for (const Tensor& t : {caches...})
-    if (!t.is_inference()) torch::autograd::increment_version(t);
+  for (const Tensor* t : {&caches...})
+    if (!t->is_inference()) torch::autograd::increment_version(*t);
 }
 
 template <int kBits>
