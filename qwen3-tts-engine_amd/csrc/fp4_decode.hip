@@ -221,11 +221,24 @@ struct State {
   float m[kT], l[kT];      // of head 4 t + g: the exponents' base, unscaled; sum, of this lane's keys until the merge
 };
 
-// A step's scores.
+// Two products of Q's parts and 16 keys' codes (u0, u1: exponent bytes), and the wait for them.
 //
 // The compiler counts the passes of the scaled instruction as if both operands had 4 bits: 8 wait states ahead of the result's first use
-// instead of the 12 that an 8-bit operand takes, and the register that was read first then held something else.  So the wait is ours: 16
-// states behind the last product, ahead of any use.
+// instead of the 12 that an 8-bit operand takes, and the register that was read first then held something else.  So the wait is ours, 16
+// states behind the second product, in one statement with them: nothing that the compiler adds, a copy or a move to another register, can
+// come between.  (The 2 states ahead are what operands want that a vector instruction wrote last.)
+__device__ __forceinline__ void two_products(const i32x8_t& q0, uint32_t s0, const i32x8_t& q1, uint32_t s1, const uint4& k0, uint32_t u0,
+                                             const uint4& k1, uint32_t u1, f32x4_t& d0, f32x4_t& d1) {
+  asm volatile(
+      "s_nop 1\n\t"
+      "v_mfma_scale_f32_16x16x128_f8f6f4 %0, %2, %4, 0, %6, %8 op_sel_hi:[0,0,0] blgp:4\n\t"
+      "v_mfma_scale_f32_16x16x128_f8f6f4 %1, %3, %5, 0, %7, %9 op_sel_hi:[0,0,0] blgp:4\n\t"
+      "s_nop 15"
+      : "=&v"(d0), "=&v"(d1)
+      : "v"(q0), "v"(q1), "v"(__builtin_bit_cast(i32x4_t, k0)), "v"(__builtin_bit_cast(i32x4_t, k1)), "v"(s0), "v"(s1), "v"(u0), "v"(u1));
+}
+
+// A step's scores.
 template <int kT>
 __device__ __forceinline__ void scores(const Work& w, const uint4 (&codes)[kSub], const uint32_t (&four)[kSub], const Query<kT>& q, int lane,
                                        float (&s)[kT][kSub]) {
@@ -246,13 +259,9 @@ __device__ __forceinline__ void scores(const Work& w, const uint4 (&codes)[kSub]
 #pragma unroll
   for (int u0 = 0; u0 < kSub; u0 += kAtOnce) {
     f32x4_t d[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int u = kT == 1 ? u0 + e : u0, t = kT == 1 ? 0 : e;
-      const i32x8_t k = {(int)codes[u].x, (int)codes[u].y, (int)codes[u].z, (int)codes[u].w, 0, 0, 0, 0};
-      d[e] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(q.v[t], k, f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 4, 0, (int)q.s[t], 0, (int)ks[u]);
-    }
-    asm volatile("s_nop 15" : "+v"(d[0]), "+v"(d[1]));
+    constexpr int t1 = kT - 1;
+    const int u1 = u0 + kAtOnce - 1;
+    two_products(q.v[0], q.s[0], q.v[t1], q.s[t1], codes[u0], ks[u0], codes[u1], ks[u1], d[0], d[1]);
 #pragma unroll
     for (int e = 0; e < 2; ++e) s[kT == 1 ? 0 : e][kT == 1 ? u0 + e : u0] = sum_parts(d[e]);
   }
