@@ -18,7 +18,9 @@ returned when it is released, so memory follows the live contexts instead of ``n
   that the reference copies into every seat, engine/arrivals.py:118-145), ``unshare`` gives a seat pages of its own again before
   tokens in them are rewritten, and a page is free when its last seat lets go of it.  ``truncate`` frees the pages behind a row's
   end, ``defragment`` moves the used pages together.  Where contents have to follow, these return the page pairs for
-  ``q3attn.paged_copy``.
+  ``q3attn.paged_copy``.  The pool holds neither side of a pair until then: a source page may be free already, and the next call may
+  hand it out.  So each call's pairs are copied by a ``paged_copy`` of their own (pairs of two calls may chain, one's destination the
+  other's source, which one copy does not follow), on the stream that decodes, and before the pool's next call.
 
 The pool tensors themselves (``[num_pages, page_size, kv_heads, head_dim]`` per layer) are the caller's; this class
 only decides which page ids hold which seat's tokens.
@@ -159,7 +161,9 @@ class PagePool:
         """Give each of ``seats``, which hold nothing yet, the first ``length`` positions of seat ``src``: its full pages, shared, and a
         page of their own for the tokens of a last, partly filled one, which they go on writing.  Returns (src, dst), int32 [pairs]
         on the pool's device: the pages that ``q3attn.paged_copy`` has to copy in every cache (none if ``length`` ends with a page).
-        All-or-nothing: raises PoolExhausted (changing nothing) when the free list cannot cover them."""
+        The copy has to be enqueued before the pool's next call (which may hand out the source page, if its seat is released), before
+        the source page is written again and before anything reads the forks; pairs of several calls are not to be joined into one
+        copy.  All-or-nothing: raises PoolExhausted (changing nothing) when the free list cannot cover them."""
         src, seats, length = self._seat(src), [self._seat(s) for s in np.atleast_1d(seats)], int(length)
         if not 0 <= length <= self.capacity(src):
             raise ValueError(f"seat {src} holds {self.capacity(src)} positions, not {length}")
@@ -187,8 +191,8 @@ class PagePool:
 
     def unshare(self, seats, first=0):
         """Give each seat pages of its own from the one that holds position ``first`` on (a number, or one a seat), in place of those
-        that it shares: before tokens in them are rewritten (``paged_compact``).  Returns the pairs to copy, and raises PoolExhausted,
-        as ``fork``."""
+        that it shares: before tokens in them are rewritten (``paged_compact``).  Returns the pairs to copy, under the same conditions,
+        and raises PoolExhausted, as ``fork``."""
         seats = [self._seat(s) for s in np.atleast_1d(seats)]
         firsts = [max(0, int(n)) // self.page_size for n in np.broadcast_to(first, (len(seats),))]
         if len(set(seats)) != len(seats):
@@ -211,8 +215,8 @@ class PagePool:
         return self._pairs([p for _, _, p in todo], dst)
 
     def defragment(self):
-        """Move the used pages to the lowest ids, so that the pool's end is free.  Returns the pairs to copy: the copy has to run before
-        anything reads the pages by the new table, or is written to a page that ``grow`` hands out afterwards."""
+        """Move the used pages to the lowest ids, so that the pool's end is free.  Returns the pairs to copy, under the same conditions as
+        ``fork``'s: their sources are free afterwards."""
         used = sorted(p for p in range(self.num_pages) if self._refs[p] > 0)
         src = [p for p in used if p > len(used)]              # page 0 is the scratch page
         dst = sorted(p for p in self._free if p <= len(used))
