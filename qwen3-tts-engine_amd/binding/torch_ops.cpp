@@ -499,13 +499,18 @@ Tensor compact_in_place(at::TensorList caches, const Tensor& keep, const Tensor&
 
 // The moves take bf16 caches, whose elements may have a history.  What they write over no longer follows from it, so the cache's history
 // becomes a node that raises; a leaf is refused, as by torch's own in-place operations.
-void check_moved(at::TensorList caches) {
-  if (!at::GradMode::is_enabled()) return;
+// Whether a cache has a history that the move ends.
+bool check_moved(at::TensorList caches) {
+  if (!at::GradMode::is_enabled()) return false;
+  bool any = false;
   for (const Tensor& t : caches)
-    if (t.requires_grad()) torch::autograd::check_inplace(t, true);
+    if (t.requires_grad()) {
+      torch::autograd::check_inplace(t, true);
+      any = true;
+    }
+  return any;
 }
 void moved(const char* name, at::TensorList caches) {
-  if (!at::GradMode::is_enabled()) return;
   for (const Tensor& t : caches)
     if (t.requires_grad())
       torch::autograd::rebase_history(
@@ -515,15 +520,15 @@ void moved(const char* name, at::TensorList caches) {
 
 // (Straight to the in-place forms: another way through the dispatcher with lists of 56 caches takes 0.3 us.)
 void copy_autograd(at::TensorList caches, const Tensor& src, const Tensor& dst) {
-  check_moved(caches);
+  const bool any = check_moved(caches);
   copy_in_place(caches, src, dst);
-  moved("q3attn::paged_copy", caches);
+  if (any) moved("q3attn::paged_copy", caches);
 }
 
 Tensor compact_autograd(at::TensorList caches, const Tensor& keep, const Tensor& lens, const Tensor& bt, at::TensorList scales) {
-  check_moved(caches);
+  const bool any = check_moved(caches);
   const Tensor out = compact_in_place(caches, keep, lens, bt, scales);
-  moved("q3attn::paged_compact", caches);
+  if (any) moved("q3attn::paged_compact", caches);
   return out;
 }
 
