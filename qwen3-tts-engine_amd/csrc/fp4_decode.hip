@@ -680,10 +680,15 @@ void launch(const TreeArgs& a, dim3 grid, hipStream_t stream) {
   else hipLaunchKernelGGL((fp4_decode_kernel<kMode, kT, kW, kChunked, false>), grid, dim3(64 * kW), 0, stream, a);
 }
 // Four waves a workgroup.  Eight for chunks of 5 to 8 query heads, whose registers leave room for 12 waves on a compute unit: one workgroup
-// of eight does as much as three of four with a third of the records (5 rows of 20000 to 65000 tokens 23.0 us; two of four 26.4, three 24.0).
-// Eight also for whole rows that leave each compute unit one workgroup at most (1 row x 1500 tokens 9.9 us, with four 11.0; 24 rows x 1500
-// 11.5 and 12.6, of 188 to 1500 10.4 and 12.0; 32 x 2000 15.2 and 15.1; of 8 query heads a KV head 1 x 1500 11.9 and 13.6, 32 x 2000 16.6
-// and 17.9).  More rows lose by it, for what a wave does once for its row is as long as two steps: 576 rows 52 us with four, 61 with eight.
+// of eight does as much as three of four with a third of the records (5 rows of 20000 to 65000 tokens 23.0 us in the kernel; two of four
+// 26.4, three 24.0).
+// Eight also for whole rows that leave each compute unit one workgroup at most.  More rows lose by it where they are ragged or have 5 to 8
+// query heads to a KV head, for what a wave does once for its row is as long as two steps.  A call's us with the step's write, 8 KV heads,
+// with eight waves and with four:
+//   2 query heads each   1 x 1500 tokens 8.9 and 10.5, 16 x 1000 8.4 and 8.9, 24 x 1500 10.1 and 10.9, 24 x 188 to 1500 9.6 and 10.7,
+//                        32 x 2000 12.9 and 13.1; past the limit 33 x 1000 11.2 and 11.4, 33 x 2000 17.8 and 18.7, 33 x 100 to 1500
+//                        11.9 and 11.1, 64 x 1000 13.6 and 13.5, 64 x 2000 23.4 and 23.9, 100 x 100 to 1500 21.3 and 18.2
+//   8 query heads each   1 x 1500 11.1 and 12.9, 32 x 2000 14.5 and 15.9; past the limit 33 x 1000 17.1 and 13.7, 64 x 2000 29.2 and 26.9
 template <int kMode, int kT>
 void launch(const TreeArgs& a, dim3 grid, hipStream_t stream) {
   const int groups = a.batch * a.hkv;

@@ -3,6 +3,9 @@
 //
 // Nothing is computed, so HBM bounds both, and at few pages the launch does: a call moves every cache in one launch, where one
 // launch a cache would take 56 for 28 layers.  The caches' addresses go in with the kernel's arguments.
+// Compaction has one workgroup a (cache, KV head, row), which goes through its row chunk by chunk: with few of them that chain is the time,
+// not HBM (rows of 4000 tokens of which 2400 stay, bf16, 8 KV heads: one row in one layer, 16 workgroups, 52.7 us where its bytes take 4.1;
+// 16 rows in one layer, 256 workgroups, 64.6 and 65.5 at a large copy's rate; one row in 28 layers 105.8 and 115).
 // What is moved passes once: non-temporal stores, and loads in copies (600 pages in 28 layers, 1.1 GB, 212 us or 5.2 TB/s, 224 without
 // both; a copy of 4 GiB by the library 4.8 TB/s.  48 rows compacted, 3.1 GB, 656 us or 4.8 TB/s and 672 without; with the loads as well
 // 643, but one row 24.9 instead of 21.7).

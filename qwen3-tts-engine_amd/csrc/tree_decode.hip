@@ -1129,9 +1129,11 @@ Plan plan_of(int batch, int nodes, int hq, int hkv, int64_t capacity, bool fp4 =
   // of up to 1500 18.9 and 23.2.  Rows that are more than the chip holds at once balance by themselves.
   const int64_t groups = (int64_t)batch * hkv * p.mblocks;
   if (batch > 1024 || capacity * num_cus() <= 700 * (num_cus() + groups)) return p;
-  // Over 4 bits a step of the longest row is short, and the join is not: up to 2048 tokens whole rows win (a call's us in all, whole and in
-  // chunks, of rows of one length with the step's write: 1 x 1000 8.9 and 11.0, 1 x 1500 9.9 and 11.7, 8 x 2000 11.9 and 13.0, 32 x 2000
-  // 15.1 and 20; 1 x 4000 17.8 and 11.5, 16 x 4000 19.4 and 19.5).
+  // Over 4 bits a step of the longest row is short, and the join is not: up to 2048 tokens whole rows win, and past that few rows lose
+  // by them.  A call's us, whole and in chunks, of rows of one length with the step's write, 8 KV heads of 2 query heads: 1 x 1000 8.0 and
+  // 10.5, 1 x 2000 10.2 and 10.5, 8 x 2000 10.2 and 11.5, 32 x 2000 12.9 and 16.8; 1 x 2500 11.3 and 10.6, 8 x 2500 12.1 and 13.0, 8 x 3000
+  // 13.8 and 12.9, 8 x 4000 16.6 and 13.3.  The limit does not know the batch: from some 32 rows on whole ones would still win behind it (32 x
+  // 2100 13.6 and 17.2, 32 x 4000 23.3 and 26.2, 64 x 4000 44.9 and 48.2; of 8 query heads 32 x 2100 14.8 and 24.1).
   if (fp4 && capacity <= 2048) return p;
   // (Three workgroups a compute unit: decode 3 % slower, trees of 32 query rows 6 to 25 %.)
   auto target = [&](int each) {

@@ -22,6 +22,9 @@ def paged_copy(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Ten
     their scales where they have some; src, dst [pairs] int32 on their device, as ``PagePool.fork``, ``unshare`` and ``defragment``
     return them.
 
+    A page has to be made of runs of memory in at most two dimensions (a head-major view, some of the heads), addresses, runs and
+    strides multiples of 4 bytes (of 16 in all caches: faster), and a call copies less than 8 GiB in a cache.
+
     Pages outside a cache (-1) are left out.  A page may be the source of several pairs; one that is the destination of two, or of one
     and another's source, holds a mix afterwards."""
     _copy(caches, src, dst)
