@@ -552,8 +552,8 @@ int q3a_paged_decode_fp4_append(
 
 /*
  * Copies whole pages inside caches: page dst[i] becomes what page src[i] is, for each of num_pairs pairs in each of num_caches caches
- * (a pool's layers, their K and V, and their scales) in as few launches as their addresses take: 128 caches of up to 4 shapes in a row
- * each.  For forks of a sequence, whose last page each of them goes on writing, for pages that move together, and for a page that is
+ * (a pool's layers, their K and V, and their scales) in as few launches as their addresses take: 128 caches of up to 4 shapes, in any
+ * order, each.  For forks of a sequence, whose last page each of them goes on writing, for pages that move together, and for a page that is
  * shared and about to be written.  No counterpart in the reference, whose seats own fixed pages (engine/talker.py:23-31, 42).
  *
  *   caches   host array.  A page of a cache is n_1 x n_0 runs of run_bytes, stride_1 and stride_0 apart, and pages are stride_page

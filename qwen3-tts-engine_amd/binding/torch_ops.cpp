@@ -302,16 +302,23 @@ void paged_copy(at::TensorList caches, const Tensor& src, const Tensor& dst) {
   check_pages(who, "dst", d, dst);
   TORCH_CHECK(src.size(0) == dst.size(0), who, ": ", src.size(0), " source pages for ", dst.size(0));
   c10::SmallVector<q3a_page_cache, 64> list;
-  const Tensor* last = nullptr;  // (layers are alike: their shape is worked out once)
-  q3a_page_cache c = {};
+  c10::SmallVector<std::pair<const Tensor*, q3a_page_cache>, 4> known;  // (layers are alike: a shape is worked out once)
+  size_t k = 0;                                                         // the last cache's
+  const auto alike = [](const Tensor& t, const Tensor& u) {
+    return t.element_size() == u.element_size() && t.sizes() == u.sizes() && t.strides() == u.strides();
+  };
   for (const Tensor& t : caches) {
-    if (last != nullptr && t.device() == d && t.element_size() == last->element_size() && t.sizes() == last->sizes() &&
-        t.strides() == last->strides())
-      c.base = t.data_ptr();
-    else
-      c = page_cache(who, d, t);
-    last = &t;
-    if (t.numel() > 0) list.push_back(c);
+    if (known.empty() || !alike(t, *known[k].first)) {
+      k = 0;
+      while (k < known.size() && !alike(t, *known[k].first)) ++k;
+    }
+    if (k == known.size() || t.device() != d) {
+      known.emplace_back(&t, page_cache(who, d, t));
+      k = known.size() - 1;
+    }
+    if (t.numel() == 0) continue;
+    list.push_back(known[k].second);
+    list.back().base = t.data_ptr();
   }
   if (list.empty()) return;
   const c10::DeviceGuard guard(d);

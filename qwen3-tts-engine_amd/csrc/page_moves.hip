@@ -34,7 +34,7 @@ struct PageShape {
   Divisor per_page, per_run, per_n0;
   int num_pages;
   uint32_t blocks;         // workgroups a cache takes
-  int end;                 // caches up to here have this shape
+  int end;                 // caches up to here have this shape, from the last shape's on
 };
 struct CopyArgs {
   uint8_t* base[kMaxCopies];
@@ -249,13 +249,23 @@ extern "C" int q3a_paged_copy(const q3a_page_cache* caches, int num_caches, cons
     a.src = src;
     a.dst = dst;
     a.pairs = (uint32_t)num_pairs;
+    // The launch's caches in the list's order, which may go from shape to shape (a layer's K, V and their scales, the next layer's).
+    uint8_t of[kMaxCopies];                     // each one's shape
+    const q3a_page_cache* like[kMaxShapes];     // and a cache of it
+    int many[kMaxShapes] = {};
     int n = 0, shapes = 0;
     uint32_t most = 0;
     while (at + n < num_caches && n < kMaxCopies) {
       const q3a_page_cache& c = caches[at + n];
-      if (n == 0 || !same_shape(c, caches[at + n - 1])) {
+      int k = n > 0 ? of[n - 1] : 0;
+      if (n == 0 || !same_shape(c, *like[k])) {
+        k = 0;
+        while (k < shapes && !same_shape(c, *like[k])) ++k;
+      }
+      if (k == shapes) {
         if (shapes == kMaxShapes) break;
-        PageShape& s = a.shape[shapes++];
+        PageShape& s = a.shape[shapes];
+        like[shapes++] = &c;
         const int64_t run = c.run_bytes / unit;
         s.page = c.stride_page;
         s.s1 = c.stride_1;
@@ -268,9 +278,16 @@ extern "C" int q3a_paged_copy(const q3a_page_cache* caches, int num_caches, cons
         s.blocks = (uint32_t)((units + kThreads * kCopyUnits - 1) / (kThreads * kCopyUnits));
         most = std::max(most, s.blocks);
       }
-      a.base[n++] = (uint8_t*)c.base;
-      for (int i = shapes - 1; i < kMaxShapes; ++i) a.shape[i].end = n;
+      ++many[k];
+      of[n++] = (uint8_t)k;
     }
+    int next[kMaxShapes], end = 0;
+    for (int k = 0; k < kMaxShapes; ++k) {
+      next[k] = end;
+      end += many[k];
+      a.shape[k].end = end;
+    }
+    for (int i = 0; i < n; ++i) a.base[next[of[i]]++] = (uint8_t*)caches[at + i].base;
     const dim3 grid(most, (unsigned)n);
     const hipStream_t st = (hipStream_t)stream;
     if (by16 && dense) hipLaunchKernelGGL((copy_pages_kernel<u32x4, true>), grid, dim3(kThreads), 0, st, a);

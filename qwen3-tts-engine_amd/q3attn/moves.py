@@ -18,7 +18,7 @@ _compact = torch_op("paged_compact", lambda caches, keep, cache_seqlens, block_t
 
 def paged_copy(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor) -> None:
     """Page ``dst[i]`` of every cache becomes what its page ``src[i]`` is: ``cache[dst] = cache[src]`` for the whole list in one launch
-    (of up to 128 caches of up to 4 shapes).  ``caches``: tensors [num_pages, ...] of any type, the pools of all layers, K and V, with
+    (of up to 128 caches of up to 4 shapes, in any order).  ``caches``: tensors [num_pages, ...] of any type, the pools of all layers, K and V, with
     their scales where they have some; src, dst [pairs] int32 on their device, as ``PagePool.fork``, ``unshare`` and ``defragment``
     return them.
 
